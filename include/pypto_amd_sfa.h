@@ -41,6 +41,9 @@
  *       dispatch point: the projection stage that produces the attention's query
  *       (absorbed nope part and rope part), the int8 query latent the indexer prolog
  *       consumes, and the new rows of the latent / rope / scale caches.
+ *   pto_rotary_tables_launch, pto_rotary_launch, pto_cache_write_launch,
+ *   pto_cache_read_launch, pto_prompt_attention_launch
+ *       nothing in the reference: what a prompt needs around these operators.
  *   pto_*_workspace_bytes
  *       the workspace query the reference runtime performs before a launch
  *       (python/pypto/runtime.py:151-152, GetWorkSpaceSize).
@@ -441,6 +444,198 @@ typedef struct PtoMlaIndexerPrologQuantArgs {
 
 int pto_mla_indexer_prolog_quant_workspace_bytes(const PtoMlaIndexerPrologQuantArgs *args, size_t *bytes);
 int pto_mla_indexer_prolog_quant_launch(const PtoMlaIndexerPrologQuantArgs *args, void *hip_stream);
+
+/*
+ * ---- Around a prompt: rotary positions, writing and reading the latent cache, attention over whole sequences.
+ * These have no counterpart among the reference's operators of this path.  Strides are in elements; a tensor's last
+ * dimension is contiguous.  An empty call (no token, no row) does nothing.
+ */
+
+#define PTO_ROPE_HALF 0           /* pairs (i, i + pairs)                                              */
+#define PTO_ROPE_INTERLEAVED 1    /* pairs (2i, 2i + 1)                                                */
+#define PTO_ROPE_DEINTERLEAVED 2  /* pairs (2i, 2i + 1) come in, (i, i + pairs) go out: the MLA prolog's */
+
+/*
+ * cos and sin of positions[t] * frequencies[i], each times factor: what the prologs take as cos / sin.
+ *
+ *   positions    [t]           int64 or int32 (positions_int64), any sign
+ *   frequencies  [pairs]       fp64, radians per position
+ *   cos, sin     [t, 2*pairs]  dtype (PTO_DT_*), columns i and i + pairs alike
+ *
+ * Angles are taken in 64 bits.  Constraints: pairs a multiple of 4, up to 128.
+ */
+typedef struct PtoRotaryTablesArgs {
+    const void *positions;
+    const double *frequencies;
+    void *cos;
+    void *sin;
+    int64_t t;
+    int64_t pairs;
+    double factor;
+    int32_t positions_int64;
+    int32_t dtype;
+} PtoRotaryTablesArgs;
+
+int pto_rotary_tables_launch(const PtoRotaryTablesArgs *args, void *hip_stream);
+
+/*
+ * Rotation of queries and, in the same launch, keys (key.in NULL: none).
+ *
+ *   in, out  [t, heads, dim] dtype; channels offset .. offset + 2*pairs - 1 turn by positions[t] * frequencies[i]:
+ *            (a, b) -> (a c - b s, b c + a s), c and s times factor.  out may be in: the other channels then stay, else
+ *            they are copied.  out and in must not overlap otherwise.
+ *
+ * Constraints: pairs a multiple of 8, up to 128; heads up to 65536; dim up to 65536.  Alignment: the element's.
+ */
+typedef struct PtoRotaryTensor {
+    const void *in;
+    void *out;
+    int64_t heads;
+    int64_t dim;
+    int64_t offset;
+    int64_t in_stride_t, in_stride_h;
+    int64_t out_stride_t, out_stride_h;
+} PtoRotaryTensor;
+
+typedef struct PtoRotaryArgs {
+    PtoRotaryTensor query;
+    PtoRotaryTensor key;
+    const void *positions;
+    const double *frequencies;
+    int64_t t;
+    int64_t pairs;
+    double factor;
+    int32_t layout;           /* PTO_ROPE_* */
+    int32_t positions_int64;
+    int32_t dtype;            /* PTO_DT_* */
+    int32_t reserved;
+} PtoRotaryArgs;
+
+int pto_rotary_launch(const PtoRotaryArgs *args, void *hip_stream);
+
+/*
+ * Quantises latents as they are written into the cache of the sparse attention: of every 128 channels
+ * steps = 127 * (1 / max|v|), code = rint(v * steps), scale = 1 / steps in fp32, each operation rounded (the MLA prolog
+ * divides 127 by the maximum at once: a code may be one step away from the prolog's in rare entries).
+ *
+ *   latent       [t, 512], rope [t, 64]   dtype (PTO_DT_*)
+ *   cache_index  [t]  int64, physical row of each token; rows outside [0, cache_rows) are skipped.  No row may be named twice:
+ *                what such a row then holds is unspecified.
+ *   nope, rope_cache, scales   the three arrays of PtoSfaQuantArgs (512 int8, 64 bf16, 4 fp32 a row), or packed: nope alone,
+ *                the 656-byte rows of PtoSaAntiquantArgs, the other two NULL
+ *   values       [t, 512] bf16 or NULL: what the rows written stand for, bf16(code * scale), for skipped tokens too
+ *
+ * A group that holds an infinity or something that is no number gets codes 0 and a scale that is no number, so that it reads as
+ * such; a group whose largest magnitude is below 127 / FLT_MAX is written as zeros with scale 0.
+ * Alignment: cache arrays 16 bytes, the others their element's.
+ */
+typedef struct PtoCacheWriteArgs {
+    const void *latent;
+    const void *rope;
+    const int64_t *cache_index;
+    void *nope;
+    void *rope_cache;
+    void *scales;
+    void *values;
+    int64_t t;
+    int64_t cache_rows;
+    int64_t latent_stride, rope_stride, values_stride;
+    int32_t dtype;
+    int32_t packed;
+} PtoCacheWriteArgs;
+
+int pto_cache_write_launch(const PtoCacheWriteArgs *args, void *hip_stream);
+
+/*
+ * Reads sequences' positions back out of that cache, de-quantised as the attention does, one sequence behind the other:
+ * row cu_seqlens[i] + j of the outputs is position first[i] + j of sequence i.
+ *
+ *   block_table  [b, max_blocknum_perbatch] int32;  cu_seqlens [b + 1] int32, ascending;  first [b] int32 or NULL (zeros)
+ *   latent       [rows, 512] bf16, key_rope [rows, 64] bf16; rows in front of cu_seqlens[0] and from cu_seqlens[b] on stay as
+ *                they were.  A position whose page the table does not hold (outside it, or a page outside the cache) reads
+ *                as zeros.
+ */
+typedef struct PtoCacheReadArgs {
+    const void *nope;
+    const void *rope_cache;
+    const void *scales;
+    const int32_t *block_table;
+    const int32_t *cu_seqlens;
+    const int32_t *first;
+    void *latent;
+    void *key_rope;
+    int64_t b;
+    int64_t rows;
+    int64_t cache_rows;
+    int64_t block_size;
+    int64_t max_blocknum_perbatch;
+    int64_t latent_stride, key_rope_stride;
+    int32_t packed;
+    int32_t reserved;
+} PtoCacheReadArgs;
+
+int pto_cache_read_launch(const PtoCacheReadArgs *args, void *hip_stream);
+
+/*
+ * Attention over whole sequences, packed one behind the other.
+ *
+ *   query [total_q, heads, d], key and value [total_k, kv_heads, d]   bf16 or fp16 (fp16 != 0)
+ *   query_rope [total_q, heads, 64], key_rope [total_k, 64] (key_rope_stride_h 0) or [total_k, kv_heads, 64], or both NULL
+ *   cu_seqlens_q, cu_seqlens_k [b + 1] int32, ascending: sequence i has query rows cu_seqlens_q[i] .. and key rows cu_seqlens_k[i] ..
+ *   out [total_q, heads, d];  lse [total_q, heads] fp32 or NULL: the natural logarithm of the sum of exp of a row's scores
+ *
+ * Head h uses key head h / (heads / kv_heads).  s = softmax_scale * (q . k + q_rope . k_rope).  causal: the last query of a
+ * sequence sees all of its keys, each one before it one key less; otherwise every query sees all keys.  Rows that see no key are
+ * zeros, their lse -infinity; query rows of no sequence stay as they were.  Keys and values of rows past a sequence's last are
+ * not looked at.  The values of a sequence's keys that a row does not see have to be finite.
+ * Beginnings outside the tensors are moved into them.
+ *
+ * Constraints: d 64 or 128, rope parts with d 128 only; heads a multiple of kv_heads; strides of 64 key rows below 4 GiB.
+ * Alignment: keys and values 16 bytes, their strides multiples of 8 elements; the others their element's.
+ * The workspace holds the partial results of rows whose keys are divided over workgroups.
+ */
+typedef struct PtoPromptAttentionArgs {
+    const void *query;
+    const void *key;
+    const void *value;
+    const void *query_rope;
+    const void *key_rope;
+    const int32_t *cu_seqlens_q;
+    const int32_t *cu_seqlens_k;
+    void *out;
+    float *lse;
+    void *workspace;
+    size_t workspace_bytes;
+    int64_t b;
+    int64_t total_q;
+    int64_t total_k;
+    int64_t heads;
+    int64_t kv_heads;
+    int64_t d;
+    int64_t query_stride_t, query_stride_h;
+    int64_t key_stride_t, key_stride_h;
+    int64_t value_stride_t, value_stride_h;
+    int64_t query_rope_stride_t, query_rope_stride_h;
+    int64_t key_rope_stride_t, key_rope_stride_h;
+    int64_t out_stride_t, out_stride_h;
+    float softmax_scale;
+    int32_t causal;
+    int32_t fp16;
+    int32_t reserved;
+} PtoPromptAttentionArgs;
+
+int pto_prompt_attention_workspace_bytes(const PtoPromptAttentionArgs *args, size_t *bytes);
+
+/* How pto_prompt_attention_launch divides such a call on the current device (on a host without one: of 256 compute units).  No
+ * pointer of args is looked at and nothing is launched. */
+typedef struct PtoPromptPlan {
+    int64_t rows_per_workgroup; /* (query, head of a group) pairs */
+    int64_t key_splits;         /* most pieces that a workgroup's keys are divided into */
+    int64_t split_keys;         /* keys of a sequence from which a further piece begins */
+    int64_t items;              /* workgroups per key head, at most */
+} PtoPromptPlan;
+int pto_prompt_attention_plan(const PtoPromptAttentionArgs *args, PtoPromptPlan *plan);
+int pto_prompt_attention_launch(const PtoPromptAttentionArgs *args, void *hip_stream);
 
 /* Thread-local description of the last error on this thread ("" if none). */
 const char *pto_last_error(void);

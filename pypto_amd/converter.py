@@ -71,6 +71,57 @@ def as_torch(x, what: str) -> torch.Tensor:
     raise TypeError(f"{what}: input type is not currently supported.")
 
 
+def as_rows(x, what: str) -> torch.Tensor:
+    """Unwrapping for the operators that take strided tensors: the last dimension alone has to be contiguous."""
+    t = x.torch() if isinstance(x, Tensor) else x
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{what}: input type is not currently supported.")
+    if t.dim() and t.stride(-1) != 1 and t.shape[-1] > 1:
+        raise RuntimeError(f"{what}: the last dimension must be contiguous")
+    return t
+
+
+def extent(t: torch.Tensor):
+    """First and one past the last byte that a tensor's elements lie in."""
+    if t.numel() == 0:
+        return t.data_ptr(), t.data_ptr()
+    return t.data_ptr(), t.data_ptr() + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()
+
+
+def same_rows(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors of one shape and type are the same memory, element by element."""
+    return a.data_ptr() == b.data_ptr() and all(x == y for n, x, y in zip(a.shape, a.stride(), b.stride()) if n > 1)
+
+
+def side_by_side(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors are different columns of rows that lie equally far apart (slices of one tensor)."""
+    if min(a.dim(), b.dim()) < 2 or min(a.shape[0], b.shape[0]) < 2:
+        return False
+    pitch = a.stride(0) * a.element_size()
+    if pitch != b.stride(0) * b.element_size() or pitch <= 0:
+        return False
+    (lo, hi), (lo2, hi2) = extent(a[0]), extent(b[0])
+    at = (lo2 - lo) % pitch                                # where b's columns begin, seen from a's
+    return at >= hi - lo and at + (hi2 - lo2) <= pitch
+
+
+def refuse_overlap(out: torch.Tensor, other: torch.Tensor, what: str) -> None:
+    """Outputs have memory of their own.  Views that interleave in one allocation count as overlapping, but for different columns of the
+    same rows."""
+    (lo, hi), (lo2, hi2) = extent(out), extent(other)
+    if lo < hi2 and lo2 < hi and not side_by_side(out, other):
+        raise ValueError(f"{what} overlap in memory")
+
+
+def check_writable(t: torch.Tensor, what: str) -> None:
+    """No two elements of an output may share memory."""
+    reach = 1
+    for stride, n in sorted((s, n) for n, s in zip(t.shape, t.stride()) if n > 1):
+        if stride < reach:
+            raise ValueError(f"{what}: elements share memory")
+        reach += (n - 1) * stride
+
+
 def copy_unless_same(dst: torch.Tensor, src: torch.Tensor, what: str) -> None:
     """The cache-out arguments of the prolog operators: normally the very tensor passed as cache-in (the
     kernels then update the rows named by the cache index in place and nothing is copied).  A different

@@ -11,6 +11,7 @@
 #include <cstring>
 #include <mutex>
 
+#include "capi_error.h"
 #include "li_kernels.h"
 #include "lip_kernels.h"
 #include "prolog_fused.h"
@@ -28,6 +29,9 @@ namespace {
 
 thread_local char g_err[512] = "";
 
+}  // namespace
+
+namespace pto {
 int fail(int code, const char *fmt, ...)
 {
     va_list ap;
@@ -37,9 +41,6 @@ int fail(int code, const char *fmt, ...)
     return code;
 }
 
-}  // namespace
-
-namespace pto {
 // compute units of the current device (one query per device ordinal, then cached)
 int cu_count()
 {
@@ -60,6 +61,7 @@ int cu_count()
 namespace {
 
 using pto::cu_count;
+using pto::fail;
 
 // device address of this device's copy of the scratch array (NULL and *err set on failure)
 void *scratch_of(int dev, hipError_t *err)

@@ -37,7 +37,7 @@ struct Call {
     bool ok = true;
     c10::Device device{c10::DeviceType::CPU, -1};
 
-    const at::Tensor &tensor(const int i)
+    const at::Tensor &tensor(const int i, const bool strided = false)
     {
         static const at::Tensor none;
         PyObject *o = args[i];
@@ -55,7 +55,7 @@ struct Call {
             return none;
         }
         const at::Tensor &t = THPVariable_Unpack(o);
-        if (t.layout() != c10::kStrided || !t.is_contiguous() || !t.device().is_cuda() || !t.has_storage()) {
+        if (t.layout() != c10::kStrided || (!strided && !t.is_contiguous()) || !t.device().is_cuda() || !t.has_storage()) {
             ok = false;
             return none;
         }
@@ -76,6 +76,14 @@ struct Call {
         ok = ok && t.scalar_type() == type && t.sizes() == c10::IntArrayRef(sizes.begin(), sizes.size());
         return t;
     }
+    // a tensor whose last dimension alone has to be contiguous: [rows, heads, channels], or [rows, channels] as one head
+    const at::Tensor &rows_of(const int i, const c10::ScalarType type, const int64_t channels = -1)
+    {
+        const at::Tensor &t = tensor(i, true);
+        if (!ok || t.scalar_type() != type || t.dim() < 2 || t.dim() > 3 || t.stride(-1) != 1 || (channels >= 0 && t.size(-1) != channels)) ok = false;
+        return t;
+    }
+    bool none(const int i) const { return args[i] == Py_None; }
     // the address of a tensor that was checked: ptr for what the kernels read, out for what they write (a tensor that shares
     // its memory copy-on-write gets memory of its own here)
     template <typename T> T *ptr(const at::Tensor &t) { return ok ? static_cast<T *>(const_cast<void *>(t.const_data_ptr())) : nullptr; }
@@ -360,6 +368,241 @@ PyObject *fused_prolog_call(PyObject *, PyObject *const *args, Py_ssize_t n)
     });
 }
 
+// Strides, heads and extent of a [rows, heads, channels] or [rows, channels] tensor; dimensions of one element have none.
+int64_t heads_of(const at::Tensor &t) { return t.dim() == 3 ? t.size(1) : 1; }
+int64_t row_stride(const at::Tensor &t) { return t.size(0) > 1 ? t.stride(0) : 0; }
+int64_t head_stride(const at::Tensor &t) { return t.dim() == 3 && t.size(1) > 1 ? t.stride(1) : 0; }
+
+// whether no two elements of a written tensor share memory (as far as the strides tell by nesting)
+bool writable(const at::Tensor &t)
+{
+    const int64_t n0 = t.size(0), n1 = heads_of(t), s0 = row_stride(t), s1 = head_stride(t), c = t.size(-1);
+    if (n0 == 0 || n1 == 0) return true;
+    auto nested = [&](const int64_t na, const int64_t sa, const int64_t nb, const int64_t sb) {
+        return (na <= 1 || sa >= c) && (nb <= 1 || sb >= (na - 1) * sa + c);
+    };
+    return nested(n1, s1, n0, s0) || nested(n0, s0, n1, s1);
+}
+
+// whether a written tensor and another one meet in memory; where_same: not if they are the same rows
+bool clash(const at::Tensor &out, const at::Tensor &in, const bool where_same = true)
+{
+    if (out.numel() == 0 || in.numel() == 0) return false;
+    const char *a = static_cast<const char *>(out.const_data_ptr()), *b = static_cast<const char *>(in.const_data_ptr());
+    if (!where_same && a == b && row_stride(out) == row_stride(in) && head_stride(out) == head_stride(in)) return false;
+    auto bytes = [](const at::Tensor &t, const int64_t from) {          // that the dimensions from this one on reach over
+        int64_t n = 1;
+        for (int64_t d = from; d < t.dim(); ++d) n += (t.size(d) - 1) * t.stride(d);
+        return n * static_cast<int64_t>(t.element_size());
+    };
+    if (out.dim() >= 2 && in.dim() >= 2 && out.size(0) > 1 && in.size(0) > 1) {
+        // different columns of the same rows (slices of one tensor) do not meet
+        const int64_t pitch = out.stride(0) * static_cast<int64_t>(out.element_size());
+        if (pitch > 0 && pitch == in.stride(0) * static_cast<int64_t>(in.element_size())) {
+            const int64_t at = (((b - a) % pitch) + pitch) % pitch;
+            if (at >= bytes(out, 1) && at + bytes(in, 1) <= pitch) return false;
+        }
+    }
+    return a < b + bytes(in, 0) && b < a + bytes(out, 0);
+}
+
+template <typename Args, typename Launch>
+PyObject *enqueue_without_workspace(const c10::Device &device, const Args &a, Launch launch)
+{
+    c10::DeviceGuard guard(device);
+    const int rc = launch(&a, c10::hip::getCurrentHIPStream(device.index()).stream());
+    if (rc != PTO_OK) return raise_status(rc);
+    Py_RETURN_TRUE;
+}
+
+// positions [t] int64 or int32, frequencies [pairs] fp64
+bool turns_of(Call &c, const int at, const void *&positions, const double *&frequencies, int64_t &t, int64_t &pairs, int32_t &wide)
+{
+    const at::Tensor &pos = c.tensor(at), &freq = c.of(at + 1, at::kDouble);
+    if (!c.ok || !dims(pos, 1) || !dims(freq, 1) || (pos.scalar_type() != I64 && pos.scalar_type() != I32)) return false;
+    positions = c.ptr<void>(pos), frequencies = c.ptr<double>(freq);
+    t = pos.size(0), pairs = freq.size(0), wide = pos.scalar_type() == I64;
+    return true;
+}
+
+// positions, frequencies, cos_out, sin_out, factor
+PyObject *rotary_tables_call(PyObject *, PyObject *const *args, Py_ssize_t n)
+{
+    if (n != 5) return declined();
+    return guarded([&]() -> PyObject * {
+        Call c{args};
+        PtoRotaryTablesArgs a{};
+        a.factor = c.real(4);
+        if (!turns_of(c, 0, a.positions, a.frequencies, a.t, a.pairs, a.positions_int64)) return declined();
+        const at::Tensor &cos = c.tensor(2), &sin = c.tensor(3);
+        if (!c.ok || !dims(cos, 2) || cos.size(0) != a.t || cos.size(1) != 2 * a.pairs || sin.sizes() != cos.sizes() || sin.scalar_type() != cos.scalar_type() ||
+            clash(cos, sin))
+            return declined();
+        a.dtype = dtype_code(cos, c.ok);
+        a.cos = c.out<void>(cos), a.sin = c.out<void>(sin);
+        if (!c.ok) return declined();
+        return enqueue_without_workspace(c.device, a, pto_rotary_tables_launch);
+    });
+}
+
+// query, key (or None), positions, frequencies, query_out, key_out (or None), layout, query_offset, key_offset, factor
+PyObject *rotary_embedding_call(PyObject *, PyObject *const *args, Py_ssize_t n)
+{
+    if (n != 10) return declined();
+    return guarded([&]() -> PyObject * {
+        Call c{args};
+        PtoRotaryArgs a{};
+        a.layout = static_cast<int32_t>(c.integer(6)), a.factor = c.real(9);
+        if (!turns_of(c, 2, a.positions, a.frequencies, a.t, a.pairs, a.positions_int64) || c.none(1) != c.none(5)) return declined();
+        const at::Tensor *seen[4];
+        const int sides = c.none(1) ? 1 : 2;
+        for (int k = 0; k < sides; ++k) {
+            PtoRotaryTensor &r = k == 0 ? a.query : a.key;
+            const at::Tensor &in = c.tensor(k, true);
+            if (!c.ok) return declined();
+            a.dtype = dtype_code(in, c.ok);
+            const c10::ScalarType type = in.scalar_type();
+            c.rows_of(k, type);
+            const at::Tensor &out = c.rows_of(4 + k, type);
+            if (!c.ok || in.sizes() != out.sizes() || in.size(0) != a.t || (k == 1 && type != seen[0]->scalar_type()) || !writable(out)) return declined();
+            r.heads = heads_of(in), r.dim = in.size(-1), r.offset = c.integer(7 + k);
+            r.in_stride_t = row_stride(in), r.in_stride_h = head_stride(in), r.out_stride_t = row_stride(out), r.out_stride_h = head_stride(out);
+            seen[k] = &in, seen[2 + k] = &out;
+            if (clash(out, in, false)) return declined();
+        }
+        if (sides == 2) {
+            const bool in_place = seen[0]->const_data_ptr() == seen[2]->const_data_ptr() && seen[1]->const_data_ptr() == seen[3]->const_data_ptr();
+            if (!in_place && (clash(*seen[2], *seen[1]) || clash(*seen[3], *seen[0]) || clash(*seen[2], *seen[3]))) return declined();
+        }
+        for (int k = 0; k < sides; ++k) {
+            PtoRotaryTensor &r = k == 0 ? a.query : a.key;
+            r.out = c.out<void>(*seen[2 + k]), r.in = c.ptr<void>(*seen[k]);
+        }
+        if (!c.ok) return declined();
+        return enqueue_without_workspace(c.device, a, pto_rotary_launch);
+    });
+}
+
+// the cache at args[i .. i + 2]: three arrays, or one packed array and two times None
+bool cache_args(Call &c, const int i, const at::Tensor *(&parts)[3], int64_t &rows, int32_t &packed)
+{
+    packed = c.none(i + 1) && c.none(i + 2);
+    parts[0] = &c.of(i, I8);
+    const int64_t width = packed ? 656 : 512;
+    if (!c.ok || parts[0]->dim() < 2 || parts[0]->size(-1) != width) return false;
+    rows = parts[0]->numel() / width;
+    parts[1] = parts[2] = nullptr;
+    if (!packed) parts[1] = &c.of(i + 1, BF16, rows * 64), parts[2] = &c.of(i + 2, FP32, rows * 4);
+    return c.ok;
+}
+
+// latent, key_rope, cache_index, nope, rope, scales (or packed, None, None), values (or None)
+PyObject *cache_write_call(PyObject *, PyObject *const *args, Py_ssize_t n)
+{
+    if (n != 7) return declined();
+    return guarded([&]() -> PyObject * {
+        Call c{args};
+        PtoCacheWriteArgs a{};
+        const at::Tensor &latent = c.tensor(0, true);
+        if (!c.ok) return declined();
+        a.dtype = dtype_code(latent, c.ok);
+        const c10::ScalarType type = latent.scalar_type();
+        c.rows_of(0, type, 512);
+        const at::Tensor &rope = c.rows_of(1, type, 64), &index = c.of(2, I64);
+        const at::Tensor *parts[3];
+        if (!c.ok || !dims(latent, 2) || !dims(rope, 2) || rope.size(0) != latent.size(0) || index.numel() != latent.size(0) ||
+            !cache_args(c, 3, parts, a.cache_rows, a.packed))
+            return declined();
+        a.t = latent.size(0), a.latent_stride = row_stride(latent), a.rope_stride = row_stride(rope);
+        for (const at::Tensor *p : parts)
+            if (p && (clash(*p, latent) || clash(*p, rope))) return declined();
+        if (!c.none(6)) {
+            const at::Tensor &values = c.rows_of(6, BF16, 512);
+            if (!c.ok || values.sizes() != latent.sizes() || !writable(values) || clash(values, latent, type != BF16) || clash(values, rope)) return declined();
+            for (const at::Tensor *p : parts)
+                if (p && clash(*p, values)) return declined();
+            a.values = c.out<void>(values), a.values_stride = row_stride(values);
+        }
+        a.nope = c.out<void>(*parts[0]);
+        if (!a.packed) a.rope_cache = c.out<void>(*parts[1]), a.scales = c.out<void>(*parts[2]);
+        a.latent = c.ptr<void>(latent), a.rope = c.ptr<void>(rope), a.cache_index = c.ptr<int64_t>(index);
+        return enqueue_without_workspace(c.device, a, pto_cache_write_launch);
+    });
+}
+
+// nope, rope, scales (or packed, None, None), block_table, cu_seqlens, first (or None), latent_out, key_rope_out, block_size
+PyObject *cache_read_call(PyObject *, PyObject *const *args, Py_ssize_t n)
+{
+    if (n != 9) return declined();
+    return guarded([&]() -> PyObject * {
+        Call c{args};
+        PtoCacheReadArgs a{};
+        a.block_size = c.integer(8);
+        const at::Tensor *parts[3];
+        if (!cache_args(c, 0, parts, a.cache_rows, a.packed)) return declined();
+        const at::Tensor &bt = c.of(3, I32), &cu = c.of(4, I32), &latent = c.rows_of(6, BF16, 512), &rope = c.rows_of(7, BF16, 64);
+        if (!c.ok || !dims(bt, 2) || !dims(cu, 1) || !dims(latent, 2) || !dims(rope, 2) || rope.size(0) != latent.size(0) || bt.size(0) < 1 ||
+            cu.size(0) != bt.size(0) + 1 || !writable(latent) || !writable(rope) || clash(latent, rope))
+            return declined();
+        a.b = bt.size(0), a.max_blocknum_perbatch = bt.size(1), a.rows = latent.size(0);
+        for (const at::Tensor *p : parts)
+            if (p && (clash(latent, *p) || clash(rope, *p))) return declined();
+        if (!c.none(5)) a.first = c.ptr<int32_t>(c.shaped(5, I32, {a.b}));
+        a.nope = c.ptr<void>(*parts[0]);
+        if (!a.packed) a.rope_cache = c.ptr<void>(*parts[1]), a.scales = c.ptr<void>(*parts[2]);
+        a.block_table = c.ptr<int32_t>(bt), a.cu_seqlens = c.ptr<int32_t>(cu);
+        a.latent = c.out<void>(latent), a.key_rope = c.out<void>(rope);
+        a.latent_stride = row_stride(latent), a.key_rope_stride = row_stride(rope);
+        if (!c.ok) return declined();
+        return enqueue_without_workspace(c.device, a, pto_cache_read_launch);
+    });
+}
+
+// query, key, value, cu_seqlens_q, cu_seqlens_k, attention_out, softmax_scale, query_rope, key_rope, softmax_lse (each or
+// None), causal
+PyObject *prompt_attention_call(PyObject *, PyObject *const *args, Py_ssize_t n)
+{
+    if (n != 11) return declined();
+    return guarded([&]() -> PyObject * {
+        Call c{args};
+        PtoPromptAttentionArgs a{};
+        a.softmax_scale = static_cast<float>(c.real(6));
+        if (args[10] != Py_True && args[10] != Py_False) return declined();
+        a.causal = args[10] == Py_True;
+        const at::Tensor &q = c.tensor(0, true), &cu_q = c.of(3, I32), &cu_k = c.of(4, I32);
+        if (!c.ok || !dims(q, 3) || !dims(cu_q, 1) || !dims(cu_k, 1) || cu_q.size(0) != cu_k.size(0) || cu_q.size(0) < 2) return declined();
+        const c10::ScalarType type = q.scalar_type();
+        if (type != BF16 && type != FP16) return declined();
+        a.d = q.size(2);
+        c.rows_of(0, type);
+        const at::Tensor &k = c.rows_of(1, type, a.d), &v = c.rows_of(2, type, a.d), &out = c.rows_of(5, type, a.d);
+        if (!c.ok || !dims(k, 3) || k.sizes() != v.sizes() || out.sizes() != q.sizes() || !writable(out) || clash(out, q) || clash(out, k) || clash(out, v) ||
+            c.none(7) != c.none(8))
+            return declined();
+        a.fp16 = type == FP16;
+        a.b = cu_q.size(0) - 1, a.total_q = q.size(0), a.total_k = k.size(0), a.heads = q.size(1), a.kv_heads = k.size(1);
+        a.query_stride_t = row_stride(q), a.query_stride_h = head_stride(q), a.key_stride_t = row_stride(k), a.key_stride_h = head_stride(k);
+        a.value_stride_t = row_stride(v), a.value_stride_h = head_stride(v), a.out_stride_t = row_stride(out), a.out_stride_h = head_stride(out);
+        if (!c.none(7)) {
+            const at::Tensor &qr = c.rows_of(7, type, 64), &kr = c.rows_of(8, type, 64);
+            if (!c.ok || !dims(qr, 3) || qr.size(0) != a.total_q || qr.size(1) != a.heads || kr.size(0) != a.total_k ||
+                (heads_of(kr) != 1 && heads_of(kr) != a.kv_heads) || clash(out, qr) || clash(out, kr))
+                return declined();
+            a.query_rope = c.ptr<void>(qr), a.query_rope_stride_t = row_stride(qr), a.query_rope_stride_h = head_stride(qr);
+            a.key_rope = c.ptr<void>(kr), a.key_rope_stride_t = row_stride(kr), a.key_rope_stride_h = head_stride(kr);
+        }
+        if (!c.none(9)) {
+            const at::Tensor &lse = c.shaped(9, FP32, {a.total_q, a.heads});
+            if (!c.ok || clash(lse, out) || clash(lse, q) || clash(lse, k) || clash(lse, v)) return declined();
+            a.lse = c.out<float>(lse);
+        }
+        a.query = c.ptr<void>(q), a.key = c.ptr<void>(k), a.value = c.ptr<void>(v), a.out = c.out<void>(out);
+        a.cu_seqlens_q = c.ptr<int32_t>(cu_q), a.cu_seqlens_k = c.ptr<int32_t>(cu_k);
+        if (!c.ok) return declined();
+        return enqueue(c.device, a, pto_prompt_attention_workspace_bytes, pto_prompt_attention_launch);
+    });
+}
+
 // the wrapper class whose instances stand for their torch tensor, and the name of the slot that holds it
 PyObject *set_wrapper(PyObject *, PyObject *const *args, Py_ssize_t n)
 {
@@ -378,7 +621,8 @@ PyObject *set_wrapper(PyObject *, PyObject *const *args, Py_ssize_t n)
 
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST(sfa_call),       FAST(sa_antiquant_call), FAST(li_decode_call), FAST(mla_prolog_call),
-                         FAST(li_prolog_call), FAST(fused_prolog_call), FAST(set_wrapper),    {nullptr, nullptr, 0, nullptr}};
+                         FAST(li_prolog_call), FAST(fused_prolog_call), FAST(set_wrapper),    FAST(rotary_tables_call),
+                         FAST(rotary_embedding_call), FAST(cache_write_call), FAST(cache_read_call), FAST(prompt_attention_call), {nullptr, nullptr, 0, nullptr}};
 #undef FAST
 
 }  // namespace
