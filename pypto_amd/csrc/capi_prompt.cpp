@@ -99,7 +99,7 @@ int attention_check(const PtoPromptAttentionArgs *a)
 }
 
 struct PromptPlan {
-    int waves, splits, split_tiles;
+    int splits, split_tiles;
     long long items;
     size_t o_bytes, ml_bytes;
 };
@@ -109,8 +109,7 @@ PromptPlan attention_plan(const PtoPromptAttentionArgs *a)
     PromptPlan pl{};
     const int cus = cu_count() > 0 ? cu_count() : 256;
     const long long rows = a->total_q * (a->heads / a->kv_heads);
-    pl.waves = 8;
-    const long long tile = 32 * pl.waves;
+    const long long tile = pto::PA_ROWS;
     const long long tiles = rows / tile + a->b;            // of a key head, at most
     const long long per_seq = (rows + tile - 1) / tile;    // of one sequence, at most
     const long long key_tiles = (a->total_k + pto::PA_KEYS - 1) / pto::PA_KEYS + a->b;
@@ -281,7 +280,7 @@ int pto_prompt_attention_plan(const PtoPromptAttentionArgs *a, PtoPromptPlan *pl
     const int rc = attention_check(a);
     if (rc != PTO_OK) return rc;
     const PromptPlan pl = attention_plan(a);
-    plan->rows_per_workgroup = 32 * pl.waves;
+    plan->rows_per_workgroup = pto::PA_ROWS;
     plan->key_splits = pl.splits;
     plan->split_keys = (int64_t)pl.split_tiles * pto::PA_KEYS;
     plan->items = pl.items;
@@ -338,7 +337,8 @@ int pto_prompt_attention_launch(const PtoPromptAttentionArgs *a, void *hip_strea
     p.rope = a->query_rope != nullptr;
     p.fp16 = a->fp16 != 0;
     p.causal = a->causal != 0;
-    p.waves = pl.waves;
+    p.q_whole = aligned(a->query, 16) && aligned(a->query_rope, 16) && a->query_stride_t % 8 == 0 && a->query_stride_h % 8 == 0 &&
+                a->query_rope_stride_t % 8 == 0 && a->query_rope_stride_h % 8 == 0;
     p.splits = pl.splits;
     p.split_tiles = pl.split_tiles;
     p.items = pl.items;

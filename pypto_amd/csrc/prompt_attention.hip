@@ -12,6 +12,7 @@
 // The rope part of queries and keys is a separate product over 64 more channels, whose keys all heads may share: nothing is
 // concatenated in memory.
 #include <cmath>
+#include <type_traits>
 
 #include "common.h"
 #include "prompt_device.h"
@@ -26,9 +27,11 @@ constexpr int PA_ROPE = 64;
 
 __device__ __forceinline__ void pa_barrier()
 {
+    __builtin_amdgcn_sched_barrier(0);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
 }
 
 __device__ __forceinline__ float pa_other_max(const float x)
@@ -53,17 +56,40 @@ struct BF16 {
     static __device__ __forceinline__ uint32_t pack(const float lo, const float hi) { return pack_bf16x2(lo, hi); }
 };
 
+__device__ __forceinline__ uint32_t opaque(uint32_t x)
+{
+    asm("" : "+v"(x));
+    return x;
+}
+template <typename T>
+__device__ __forceinline__ T lds_frag(const uint32_t at)
+{
+    return *(const __attribute__((address_space(3))) T *)(at);
+}
+__device__ __forceinline__ s16x4 lds_tr16(const uint32_t at) { return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(at)); }
+
 // A sequence as the kernels take it: whatever the tables of beginnings say, inside the tensors.
 struct Span {
-    long long begin;
-    int len;
+    int begin, len;
 };
-__device__ __forceinline__ Span span_of(const int32_t *cu, const int b, const long long total)
+__device__ __forceinline__ Span span_of(const int32_t *cu, const int b, const int total)
 {
-    long long lo = cu[b], hi = cu[b + 1];
+    int lo = cu[b], hi = cu[b + 1];
     lo = lo < 0 ? 0 : (lo > total ? total : lo);
     hi = hi < lo ? lo : (hi > total ? total : hi);
-    return {lo, (int)(hi - lo)};
+    return {lo, hi - lo};
+}
+
+// sums of x over this lane and all lanes before it
+__device__ __forceinline__ int wave_sums(int x)
+{
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);     // row_shr:1, 2, 4, 8: within rows of sixteen lanes
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);     // row_bcast:15: rows 0 and 2 into 1 and 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);     // row_bcast:31: the lower half into the upper
+    return x;
 }
 
 // Keys that local token t of a sequence sees.
@@ -74,79 +100,70 @@ __device__ __forceinline__ int pa_visible(const int t, const int lq, const int l
     return n < 0 ? 0 : (n > lk ? lk : n);
 }
 
-// 16-byte pieces of a tile in LDS: piece c of row r lies at c ^ swizzle(r), so that neither 16 lanes that read one piece of 16
-// key rows nor 16 lanes that read four rows' 32 value channels meet in a bank.  DMA writes pieces in order, so the permutation is in
-// what each lane asks for.
-__device__ __forceinline__ int pa_swizzle_k128(const int r) { return r & 15; }
-__device__ __forceinline__ int pa_swizzle_k64(const int r) { return (r >> 1) & 7; }
-__device__ __forceinline__ int pa_swizzle_v128(const int r) { return 4 * (r & 3); }
-__device__ __forceinline__ int pa_swizzle_v64(const int r) { return 4 * ((r >> 1) & 1); }
+// A tile in LDS.  Rows of 64 channels (eight 16-byte pieces) lie one behind the other, piece c of row r at c ^ (r / 2) % 8 (keys) or
+// c ^ 4 * ((r / 2) % 2) (values).  Rows of 128 channels lie in blocks of four, 1040 bytes apart: [piece / 8][row][piece % 8], the last index ^ 4 in
+// the lower two rows.  Then neither 16 lanes that read one piece of 16 key rows nor 16 lanes that read 32 value channels of four
+// rows meet in a bank, and (128 channels) the pieces that a lane reads one after the other are constants away from one of two addresses.  A
+// DMA request writes 1024 bytes in the order of its lanes, so the order of the pieces is in what each lane asks for; eight lanes ask for a
+// whole cache line.
+constexpr int PA_BLOCK = 1040;
 
-template <typename E, int D, int R, int W>
-__global__ __launch_bounds__(64 * W, 2) void prompt_attention_kernel(const PaParams p)
+template <typename E, int D, int R>
+__global__ __launch_bounds__(64 * PA_WAVES, 2) void prompt_attention_kernel(const PaParams p)
 {
-    constexpr int ROWS = 32 * W;
+    constexpr int W = PA_WAVES, ROWS = PA_ROWS;
     constexpr int KP = D * 2;                              // bytes of a key row, and of a value row
-    constexpr int K_BYTES = PA_KEYS * KP, R_BYTES = PA_KEYS * R * 2;
-    constexpr int STAGE = 2 * K_BYTES + R_BYTES;           // [keys | rope keys | values]
+    constexpr int REQ = D == 128 ? PA_BLOCK : 1024;        // bytes from one request's rows to the next one's
+    constexpr int K_REQS = PA_KEYS * KP / 1024, R_REQS = PA_KEYS * R * 2 / 1024;
+    constexpr int K_BYTES = K_REQS * REQ, R_BYTES = R_REQS * 1024;
+    constexpr int K_STAGE = K_BYTES + R_BYTES;             // [keys | rope keys] of a tile
+    constexpr int STAGES = 3, AHEAD = 5;
     constexpr int KS = D / 16, RS = R / 16, CT = D / 32;
-    constexpr int NK = K_BYTES / 1024 / W, NR = R_BYTES / 1024 / W;   // requests of a wave per tile: keys (as many values), rope keys
-    static_assert(K_BYTES % (1024 * W) == 0 && R_BYTES % (1024 * W) == 0, "whole requests for every wave");
+    constexpr int NK = K_REQS / W, NR = R_REQS / W;   // requests of a wave per tile: keys (as many values), rope keys
+    static_assert(K_REQS % W == 0 && R_REQS % W == 0, "whole requests for every wave");
     typedef typename E::frag frag;
 
-    __shared__ __attribute__((aligned(1024))) uint8_t pool[2 * STAGE];
+    __shared__ __attribute__((aligned(1024))) uint8_t pool[STAGES * (K_STAGE + K_BYTES)];   // keys of three tiles, then their values
 
     const int tid = threadIdx.x, l = tid & 63, n = l & 31, half = l >> 5;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
 
     // Workgroup -> (key head, sequence, row tile, split).  An XCD takes consecutive items, so that workgroups which read the same
-    // head's keys share an L2; a sequence's last rows, which see the most keys, come first.
-    const long long per_xcd = (p.items * p.kv_heads + 7) / 8;
-    const long long item = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
-    if (item >= p.items * p.kv_heads || (blockIdx.x >> 3) >= per_xcd) return;
-    const int kvh = (int)(item / p.items);
-    long long rest = item - kvh * p.items;
-    int b = -1, lq = 0, lk = 0, tiles = 0, splits = 1;
-    long long q0 = 0, k0 = 0;
+    // head's keys share an L2; a sequence's last rows, which see the most keys, come first.  (Fewer than 2^31 items: the host.)
+    const int per_xcd = (int)((p.items * p.kv_heads + 7) / 8), slot = blockIdx.x >> 3;
+    const int item = (blockIdx.x & 7) * per_xcd + slot;
+    if (item >= p.items * p.kv_heads || slot >= per_xcd) return;
+    const int kvh = item / (int)p.items;
+    int rest = item - kvh * (int)p.items;
+    int b = -1, lq = 0, lk = 0, q0 = 0, k0 = 0, tiles = 0, splits = 1;
     for (int base = 0; base < p.B; base += 64) {
-        const int mine = base + l;
-        Span sq = {0, 0}, sk = {0, 0};
-        int mt = 0, ms = 1;
-        if (mine < p.B) {
-            sq = span_of(p.cu_q, mine, p.total_q);
-            sk = span_of(p.cu_k, mine, p.total_k);
-            mt = (int)(((long long)sq.len * p.group + ROWS - 1) / ROWS);
-            ms = pa_splits_of((sk.len + PA_KEYS - 1) / PA_KEYS, p.split_tiles, p.splits);
-        }
-        long long upto = (long long)mt * ms;               // items of this and all sequences before it (of these 64)
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const long long o = __shfl_up(upto, d);
-            upto += l >= d ? o : 0;
-        }
+        const int mine = base + l < p.B ? base + l : p.B - 1;
+        const Span sq = span_of(p.cu_q, mine, (int)p.total_q), sk = span_of(p.cu_k, mine, (int)p.total_k);
+        const int mt = base + l < p.B ? (sq.len * p.group + ROWS - 1) / ROWS : 0;
+        const int ms = pa_splits_of((sk.len + PA_KEYS - 1) / PA_KEYS, p.split_tiles, p.splits);
+        const int upto = wave_sums(mt * ms);               // items of this and all sequences before it (of these 64)
         const uint64_t past = __ballot(upto > rest);
         if (past != 0) {
             const int who = __builtin_ctzll(past);
             b = base + who;
-            rest -= who > 0 ? __shfl(upto, who - 1) : 0;
-            lq = __shfl(sq.len, who), lk = __shfl(sk.len, who);
-            q0 = __shfl(sq.begin, who), k0 = __shfl(sk.begin, who);
-            tiles = __shfl(mt, who), splits = __shfl(ms, who);
+            rest -= who > 0 ? __builtin_amdgcn_readlane(upto, who - 1) : 0;
+            lq = __builtin_amdgcn_readlane(sq.len, who), lk = __builtin_amdgcn_readlane(sk.len, who);
+            q0 = __builtin_amdgcn_readlane(sq.begin, who), k0 = __builtin_amdgcn_readlane(sk.begin, who);
+            tiles = __builtin_amdgcn_readlane(mt, who), splits = __builtin_amdgcn_readlane(ms, who);
             break;
         }
-        rest -= __shfl(upto, 63);
+        rest -= __builtin_amdgcn_readlane(upto, 63);
     }
     if (b < 0) return;
-    lq = __builtin_amdgcn_readfirstlane(lq), lk = __builtin_amdgcn_readfirstlane(lk), splits = __builtin_amdgcn_readfirstlane(splits);
-    const int which = __builtin_amdgcn_readfirstlane((int)(rest / splits));
-    const int split = __builtin_amdgcn_readfirstlane((int)rest - which * splits);
-    const int tile = p.causal ? __builtin_amdgcn_readfirstlane(tiles) - 1 - which : which;
+    const int which = splits > 1 ? rest / splits : rest;
+    const int split = rest - which * splits;
+    const int tile = p.causal ? tiles - 1 - which : which;
 
     // This lane's row, and how many keys it sees.  Rows past the last one stand in with it and are never stored.
     const int rows = lq * p.group;
     const int row = tile * ROWS + 32 * w + n;
     const int row_in = row < rows ? row : rows - 1;
-    const int tok = row_in / p.group, head = kvh * p.group + row_in - tok * p.group;
+    const int tok = p.group > 1 ? row_in / p.group : row_in, head = kvh * p.group + row_in - tok * p.group;
     const int sees = pa_visible(tok, lq, lk, p.causal);
     const int last_row = tile * ROWS + ROWS - 1 < rows ? tile * ROWS + ROWS - 1 : rows - 1;
     const int wg_sees = pa_visible(last_row / p.group, lq, lk, p.causal);
@@ -158,27 +175,6 @@ __global__ __launch_bounds__(64 * W, 2) void prompt_attention_kernel(const PaPar
     const int t_begin = split * split_len;
     const int t_end = t_begin + split_len < key_tiles ? t_begin + split_len : key_tiles;
 
-    frag qf[KS + RS];
-    {
-        const uint16_t *qrow = p.q + (q0 + tok) * p.q_t + head * p.q_h + 8 * half;
-#pragma unroll
-        for (int i = 0; i < KS; ++i) qf[i] = __builtin_bit_cast(frag, (u32x4) * reinterpret_cast<const u32x4_a2 *>(qrow + 16 * i));
-        if (R > 0) {
-            const uint16_t *rrow = p.qr + (q0 + tok) * p.qr_t + head * p.qr_h + 8 * half;
-#pragma unroll
-            for (int i = 0; i < RS; ++i) qf[KS + i] = __builtin_bit_cast(frag, (u32x4) * reinterpret_cast<const u32x4_a2 *>(rrow + 16 * i));
-        }
-    }
-    // Scores are scaled inside the exponent.  That wants a positive scale: the sign of a negative one moves into Q^T, and a zero one
-    // becomes the smallest normal number, under which every finite score scales to the same probabilities.
-    float scale = p.scale_log2;
-    if (scale < 0.f) {
-        scale = -scale;
-#pragma unroll
-        for (int i = 0; i < KS + RS; ++i) qf[i] = __builtin_bit_cast(frag, __builtin_bit_cast(u32x4, qf[i]) ^ 0x80008000u);
-    }
-    if (scale == 0.f) scale = 1.17549435e-38f;
-
     // Requests of a tile: a wave's request brings 1024 bytes of whole rows.  Keys past the sequence's last one stand in with it (their
     // probabilities are zero, and what lies behind the sequence is never touched).
     const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_byte_t *)pool;
@@ -186,32 +182,99 @@ __global__ __launch_bounds__(64 * W, 2) void prompt_attention_kernel(const PaPar
     const uint8_t *const v_base = reinterpret_cast<const uint8_t *>(p.v + k0 * p.v_t + kvh * p.v_h);
     const uint8_t *const r_base = R > 0 ? reinterpret_cast<const uint8_t *>(p.kr + k0 * p.kr_t + kvh * p.kr_h) : nullptr;
     constexpr int PER = 1024 / KP;                         // rows of a request
-    const int krow = l / (KP / 16), kpiece = l % (KP / 16);
-    const int rrow = l / 8, rpiece = l % 8;
-    auto request = [&](const int t, const int stage) __attribute__((always_inline)) {
-        const int left = lk - t * PA_KEYS;
-        const uint8_t *kb = k_base + (long long)t * PA_KEYS * p.k_t * 2, *vb = v_base + (long long)t * PA_KEYS * p.v_t * 2;
-        const uint32_t dst = lds0 + stage * STAGE;
+    const int row_of = D == 128 ? (l >> 3) & 3 : l >> 3;   // this lane's row of a request, and its pieces: of keys, values, rope keys
+    const int k_piece = D == 128 ? 8 * (l >> 5) + ((l & 7) ^ (4 * (row_of >> 1))) : (l & 7) ^ (((PER * w + row_of) >> 1) & 7);
+    const int v_piece = D == 128 ? k_piece : (l & 7) ^ (4 * ((row_of >> 1) & 1));
+    const int r_piece = (l & 7) ^ (((8 * w + (l >> 3)) >> 1) & 7);
+    static_assert(W % 2 == 0, "a wave's requests, W * 8 rows apart, have their pieces in the same places");
+    const uint32_t k_off = (uint32_t)row_of * (uint32_t)(p.k_t * 2) + 16 * k_piece, v_off = (uint32_t)row_of * (uint32_t)(p.v_t * 2) + 16 * v_piece;
+    const uint32_t r_off = (uint32_t)(l >> 3) * (uint32_t)(p.kr_t * 2) + 16 * r_piece;
+    // the next tile's first row of this wave, of keys, rope keys and values, and which tiles these are
+    const uint8_t *k_next = k_base + ((long long)t_begin * PA_KEYS + PER * w) * p.k_t * 2, *v_next = v_base + ((long long)t_begin * PA_KEYS + PER * w) * p.v_t * 2;
+    const uint8_t *r_next = R > 0 ? r_base + ((long long)t_begin * PA_KEYS + 8 * w) * p.kr_t * 2 : nullptr;
+    int k_tile = t_begin, v_tile = t_begin;
+    // one request of a tile all of whose keys there are: NK of its keys, NR of its rope keys, NK of its values
+    auto request_whole = [&](const int i, const int k_stage, const int v_stage) __attribute__((always_inline)) {
+        if (i < NK) dma16_base(k_next + (long long)i * W * PER * p.k_t * 2, k_off, lds0 + k_stage * K_STAGE + (i * W + w) * REQ);
+        else if (i < NK + NR) dma16_base(r_next + (long long)(i - NK) * W * 8 * p.kr_t * 2, r_off, lds0 + k_stage * K_STAGE + K_BYTES + ((i - NK) * W + w) * 1024);
+        else dma16_base(v_next + (long long)(i - NK - NR) * W * PER * p.v_t * 2, v_off, lds0 + STAGES * K_STAGE + v_stage * K_BYTES + ((i - NK - NR) * W + w) * REQ);
+    };
+    // the requests of a sequence's last tile, from its last key on the same row again
+    auto request_last = [&](const uint8_t *at, const long long pitch, const int piece, const int row_in, const uint32_t dst, const int left, const int i, const int each, const int bytes)
+                            __attribute__((always_inline)) {
+        const int r = (i * W + w) * each + row_in, from = r < left ? r : left - 1;
+        dma16_base(at - (long long)each * w * pitch * 2, (uint32_t)from * (uint32_t)(pitch * 2) + 16 * piece, dst + (i * W + w) * bytes);
+    };
+    auto whole = [&](const int tile_of) { return lk - tile_of * PA_KEYS >= PA_KEYS; };
+    auto next_keys = [&]() __attribute__((always_inline)) {
+        k_next += PA_KEYS * 2 * p.k_t;
+        if (R > 0) r_next += PA_KEYS * 2 * p.kr_t;
+        ++k_tile;
+    };
+    auto next_values = [&]() __attribute__((always_inline)) {
+        v_next += PA_KEYS * 2 * p.v_t;
+        ++v_tile;
+    };
+    auto request_keys = [&](const int stage) __attribute__((always_inline)) {
+        const int left = lk - k_tile * PA_KEYS;
+        if (whole(k_tile)) {
 #pragma unroll
-        for (int i = 0; i < NK; ++i) {
-            const int req = i * W + w, r = req * PER + krow;
-            const int from = r < left ? r : left - 1;
-            const int ck = kpiece ^ (D == 128 ? pa_swizzle_k128(r) : pa_swizzle_k64(r)), cv = kpiece ^ (D == 128 ? pa_swizzle_v128(r) : pa_swizzle_v64(r));
-            dma16_base(kb, (uint32_t)from * (uint32_t)(p.k_t * 2) + 16 * ck, dst + req * 1024);
-            dma16_base(vb, (uint32_t)from * (uint32_t)(p.v_t * 2) + 16 * cv, dst + K_BYTES + R_BYTES + req * 1024);
+            for (int i = 0; i < NK + NR; ++i) request_whole(i, stage, 0);
+        } else {
+#pragma unroll
+            for (int i = 0; i < NK; ++i) request_last(k_next, p.k_t, k_piece, row_of, lds0 + stage * K_STAGE, left, i, PER, REQ);
+#pragma unroll
+            for (int i = 0; i < NR; ++i) request_last(r_next, p.kr_t, r_piece, l >> 3, lds0 + stage * K_STAGE + K_BYTES, left, i, 8, 1024);
         }
-        if (R > 0) {
-            const uint8_t *rb = r_base + (long long)t * PA_KEYS * p.kr_t * 2;
+        next_keys();
+    };
+    auto request_values = [&](const int stage) __attribute__((always_inline)) {
+        if (whole(v_tile)) {
 #pragma unroll
-            for (int i = 0; i < NR; ++i) {
-                const int req = i * W + w, r = req * 8 + rrow;
-                const int from = r < left ? r : left - 1;
-                dma16_base(rb, (uint32_t)from * (uint32_t)(p.kr_t * 2) + 16 * (rpiece ^ pa_swizzle_k64(r)), dst + K_BYTES + req * 1024);
-            }
+            for (int i = 0; i < NK; ++i) request_whole(NK + NR + i, 0, stage);
+        } else {
+#pragma unroll
+            for (int i = 0; i < NK; ++i) request_last(v_next, p.v_t, v_piece, row_of, lds0 + STAGES * K_STAGE + stage * K_BYTES, lk - v_tile * PA_KEYS, i, PER, REQ);
+        }
+        next_values();
+    };
+
+    // Queries into registers.  As the products want them a wave would ask for 32 bytes of each of its rows at a time; so they come through
+    // LDS, whole cache lines to a request, into memory that later tiles use.  Queries that promise less than 16 bytes' alignment come
+    // straight.
+    frag qf[KS + RS];
+    const long long q_at = (long long)(q0 + tok) * p.q_t + (long long)head * p.q_h, qr_at = R > 0 ? (long long)(q0 + tok) * p.qr_t + (long long)head * p.qr_h : 0;
+    constexpr int Q_WAVE = 32 * (KP + 2 * R);
+    static_assert(K_STAGE + W * Q_WAVE <= STAGES * (K_STAGE + K_BYTES), "the queries fit beside the first tile's keys");
+    const uint32_t q_lds = lds0 + K_STAGE + w * Q_WAVE;
+    auto request_queries = [&]() __attribute__((always_inline)) {
+        auto of_row = [](const long long at, const int r) { return (uint64_t)(uint32_t)__shfl((int)at, r) | ((uint64_t)(uint32_t)__shfl((int)(at >> 32), r) << 32); };
+#pragma unroll
+        for (int i = 0; i < 32 * KP / 1024; ++i) {
+            const int r = i * PER + l / (KP / 16), piece = (l % (KP / 16)) ^ (D == 128 ? r & 15 : (r >> 1) & 7);
+            dma16(p.q + of_row(q_at, r) + 8 * piece, q_lds + i * 1024);
+        }
+#pragma unroll
+        for (int i = 0; i < 32 * 2 * R / 1024; ++i) {
+            const int r = i * 8 + l / 8, piece = (l % 8) ^ ((r >> 1) & 7);
+            dma16(p.qr + of_row(qr_at, r) + 8 * piece, q_lds + 32 * KP + i * 1024);
         }
     };
-    constexpr int REQUESTS = 2 * NK + NR;
+    auto read_queries = [&]() __attribute__((always_inline)) {
+        if (p.q_whole) {
+#pragma unroll
+            for (int i = 0; i < KS; ++i) qf[i] = lds_frag<frag>(q_lds + n * KP + 16 * ((2 * i + half) ^ (D == 128 ? n & 15 : (n >> 1) & 7)));
+#pragma unroll
+            for (int i = 0; i < RS; ++i) qf[KS + i] = lds_frag<frag>(q_lds + 32 * KP + n * (2 * R) + 16 * ((2 * i + half) ^ ((n >> 1) & 7)));
+        } else {
+#pragma unroll
+            for (int i = 0; i < KS; ++i) qf[i] = __builtin_bit_cast(frag, (u32x4) * reinterpret_cast<const u32x4_a2 *>(p.q + q_at + 8 * half + 16 * i));
+#pragma unroll
+            for (int i = 0; i < RS; ++i) qf[KS + i] = __builtin_bit_cast(frag, (u32x4) * reinterpret_cast<const u32x4_a2 *>(p.qr + qr_at + 8 * half + 16 * i));
+        }
+    };
 
+    float scale = p.scale_log2;
     f32x16 o[CT];
 #pragma unroll
     for (int c = 0; c < CT; ++c)
@@ -219,89 +282,187 @@ __global__ __launch_bounds__(64 * W, 2) void prompt_attention_kernel(const PaPar
         for (int i = 0; i < 16; ++i) o[c][i] = 0.f;
     float m_run = PA_LOW, l_run = 0.f;                     // the row's reference maximum (log2), this lane's share of its sum
 
-    // LDS addresses of the operand reads: key row n, pieces 2 * ks + half; values: keys 4 * half + (l % 16) / 4 (+ 8), channels
+    // LDS addresses of the operand reads in stage 0: key row n, pieces 2 * ks + half; values: keys 4 * half + (l % 16) / 4 (+ 8), channels
     // 16 * ((l / 16) & 1) + 4 * (l % 4)
-    const int ksw = (D == 128 ? pa_swizzle_k128(n) : pa_swizzle_k64(n)) ^ half, rsw = pa_swizzle_k64(n) ^ half;
-    const int vkey = 4 * half + ((l & 15) >> 2);
-    const int vsw = D == 128 ? pa_swizzle_v128(vkey) : pa_swizzle_v64(vkey);
-    const int vlow = 2 * ((l >> 4) & 1) + ((l & 3) >> 1);
+    constexpr int KA = D == 128 ? 2 : KS;
+    uint32_t k_lane[KA], r_lane[R > 0 ? RS : 1], v_lane[2];
+#pragma unroll
+    for (int i = 0; i < KA; ++i)
+        k_lane[i] = lds0 + (D == 128 ? (n >> 2) * REQ + (n & 3) * 128 + 16 * half + 64 * (i ^ ((n >> 1) & 1)) : n * KP + 16 * ((2 * i + half) ^ ((n >> 1) & 7)));
+#pragma unroll
+    for (int i = 0; i < RS; ++i) r_lane[i] = lds0 + K_BYTES + n * (R * 2) + 16 * ((2 * i + half) ^ ((n >> 1) & 7));
+    {
+        const int row = (l & 15) >> 2, low = 2 * ((l >> 4) & 1) + ((l & 3) >> 1);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            v_lane[i] = lds0 + STAGES * K_STAGE + 8 * (l & 1) +
+                        (D == 128 ? half * REQ + row * 128 + 64 * (i ^ (row >> 1)) + 16 * low : (4 * half + row) * KP + 16 * ((4 * i + low) ^ (4 * (row >> 1))));
+    }
+    constexpr int V_EIGHT = D == 128 ? 2 * REQ : 8 * KP;   // to the value row eight keys on
 
-    if (t_begin < t_end) request(t_begin, 0);
-    for (int t = t_begin; t < t_end; ++t) {
-        const int stage = (t - t_begin) & 1;
-        if (t + 1 < t_end) {
-            request(t + 1, stage ^ 1);
-            __builtin_amdgcn_s_waitcnt(vmcnt_imm(REQUESTS));
-        } else {
+    f32x16 s[2];                                           // scores of the tile in hand
+    frag pf[4];                                            // probabilities of the tile before it
+    // The products of a tile: scores of the tile in one stage and, spread between them, the probabilities of the tile before it times its
+    // values, in another; operands are read AHEAD products before their use.
+    auto products = [&](auto with_scores, auto with_values, const int k_stage, const int v_stage) __attribute__((always_inline)) {
+        constexpr int NQ = decltype(with_scores)::value ? 2 * (KS + RS) : 0, NP = decltype(with_values)::value ? 4 * CT : 0, N = NQ + NP;
+        uint32_t kb[KA], rb[R > 0 ? RS : 1], vb[2];        // (what the compiler cannot take apart: the rest of an address is an instruction's constant)
+        if (NQ > 0) {
+#pragma unroll
+            for (int i = 0; i < KA; ++i) kb[i] = opaque(k_lane[i] + k_stage * K_STAGE);
+#pragma unroll
+            for (int i = 0; i < RS; ++i) rb[i] = opaque(r_lane[i] + k_stage * K_STAGE);
+        }
+        if (NP > 0) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) vb[i] = opaque(v_lane[i] + v_stage * K_BYTES);
+        }
+        frag a[N];
+        auto is_value = [](const int j) { return (j + 1) * NP / N > j * NP / N; };
+        auto read = [&](const int j) __attribute__((always_inline)) {
+            const int pv = j * NP / N, qk = j - pv;        // products of either kind before this one
+            if (is_value(j)) {
+                const int ks = pv / CT, c = pv % CT;
+                const uint32_t at = vb[c & 1] + (D == 128 ? ks * 4 * REQ + (c >> 1) * 512 : 16 * ks * KP);
+                const s16x4 lo = lds_tr16(at), hi = lds_tr16(at + V_EIGHT);
+                a[j] = __builtin_bit_cast(frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+            } else {
+                const int h = qk & 1, i = qk >> 1;
+                a[j] = lds_frag<frag>(i >= KS ? rb[(i - KS) % (R > 0 ? RS : 1)] + h * 32 * (R * 2)
+                                              : D == 128 ? kb[(i >> 1) & 1] + h * 8 * REQ + (i >> 2) * 512 + (i & 1) * 32 : kb[i % KA] + h * 32 * KP);
+            }
+        };
+        const f32x16 zero = {};
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) read(j);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int pv = j * NP / N, qk = j - pv;
+            if (is_value(j)) o[pv % CT] = E::mfma(a[j], pf[pv / CT], o[pv % CT]);
+            else s[qk & 1] = E::mfma(a[j], qf[qk >> 1], qk < 2 ? zero : s[qk & 1]);
+            __builtin_amdgcn_sched_barrier(0);
+            if (j + AHEAD < N) read(j + AHEAD);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    // The softmax of tile t: scores to probabilities.
+    auto softmax = [&](const int t) __attribute__((always_inline)) {
+        if ((t + 1) * PA_KEYS > wave_least) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (t * PA_KEYS + 32 * h + 8 * (i >> 2) + 4 * half + (i & 3) >= sees) s[h][i] = -INFINITY;
+        }
+        float mx = s[0][0];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[h][i]);
+        mx = pa_other_max(mx) * scale;
+        if (__any(mx > m_run + PA_TAU)) {                  // rare: the reference follows the true maximum lazily
+            const float m_new = fmaxf(m_run, mx), alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+            m_run = m_new;
+            l_run *= alpha;
+#pragma unroll
+            for (int c = 0; c < CT; ++c)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[c][i] *= alpha;
+        }
+        float sum[2] = {0.f, 0.f};
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                float e[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[h][8 * g + i], scale, -m_run));
+                    sum[i & 1] += e[i];
+                }
+                const u32x4 pk = {E::pack(e[0], e[1]), E::pack(e[2], e[3]), E::pack(e[4], e[5]), E::pack(e[6], e[7])};
+                pf[2 * h + g] = __builtin_bit_cast(frag, pk);
+            }
+        l_run += sum[0] + sum[1];
+    };
+
+    // Two waves share a SIMD, and while one multiplies the other does the softmax of its tile: the second half of the waves is one phase
+    // behind, and a barrier ends every phase.  First half: phase 2t products of tile t (and t - 1), phase 2t + 1 its softmax.  A wave asks
+    // for its part of the keys of tile t + 2 and the values of tile t + 1 where it has time, at the beginning of its softmax of tile t (in
+    // phase 2t + 1 or 2t + 2: the last readers of those buffers, of the keys of tile t - 1 and the values of tile t - 2, were done with
+    // phase 2t - 1), and waits for them at the end of its products of tile t + 1 (phase 2t + 2 or 2t + 3; the first reader's phase is
+    // 2t + 4).  Asked for among the products they held up the first half's by 550 of 2050 clocks.
+    const bool late = w >= W / 2;
+    const std::integral_constant<bool, true> yes;
+    const std::integral_constant<bool, false> no;
+    if (t_begin < t_end) {
+        int s0 = 0, s1 = 1, s2 = 2;                        // stages of tiles t, t + 1 and t + 2 (or t - 1)
+        auto end_products = [&]() __attribute__((always_inline)) {
             __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+            pa_barrier();
+        };
+        auto request_next = [&]() __attribute__((always_inline)) {
+            if (k_tile < t_end) request_keys(s2);
+            if (v_tile < t_end) request_values(s1);
+        };
+        auto turn = [&]() __attribute__((always_inline)) {
+            const int s = s0;
+            s0 = s1, s1 = s2, s2 = s;
+        };
+        // tiles that this wave's rows see end here; in later ones it asks for its part of the tile and keeps step
+        int own_end = (wave_most + PA_KEYS - 1) / PA_KEYS;
+        own_end = own_end < t_end ? own_end : t_end;
+        request_keys(s0);
+        if (p.q_whole) request_queries();
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+        asm volatile("" ::: "memory");
+        read_queries();
+        // Scores are scaled inside the exponent.  That wants a positive scale: the sign of a negative one moves into Q^T, and a zero one
+        // becomes the smallest normal number, under which every finite score scales to the same probabilities.
+        if (scale < 0.f) {
+            scale = -scale;
+    #pragma unroll
+            for (int i = 0; i < KS + RS; ++i) qf[i] = __builtin_bit_cast(frag, __builtin_bit_cast(u32x4, qf[i]) ^ 0x80008000u);
         }
-        pa_barrier();                                      // every wave's part of tile t has landed
-        if (t * PA_KEYS < wave_most) {                     // (of a tile that a wave's rows do not see the wave does nothing)
-            const uint8_t *kt = pool + stage * STAGE, *rt = kt + K_BYTES, *vt = rt + R_BYTES;
-            f32x16 s[2];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) s[h][i] = 0.f;
-#pragma unroll
-                for (int i = 0; i < KS; ++i) s[h] = E::mfma(*reinterpret_cast<const frag *>(kt + (32 * h + n) * KP + 16 * ((2 * i) ^ ksw)), qf[i], s[h]);
-#pragma unroll
-                for (int i = 0; i < RS; ++i) s[h] = E::mfma(*reinterpret_cast<const frag *>(rt + (32 * h + n) * (R * 2) + 16 * ((2 * i) ^ rsw)), qf[KS + i], s[h]);
+        if (scale == 0.f) scale = 1.17549435e-38f;
+        pa_barrier();                                      // the first tile's keys have landed, the queries are in registers
+        request_values(s0);
+        if (k_tile < t_end) request_keys(s1);
+        if (late) pa_barrier();
+        int t = t_begin;
+        if (t < own_end) {
+            products(yes, no, s0, s2);
+            end_products();
+            request_next();
+            softmax(t);
+            pa_barrier();
+            turn();
+            for (++t; t < own_end; ++t) {
+                __builtin_amdgcn_s_setprio(1);
+                products(yes, yes, s0, s2);
+                __builtin_amdgcn_s_setprio(0);
+                end_products();
+                request_next();
+                softmax(t);
+                pa_barrier();
+                turn();
             }
-            if ((t + 1) * PA_KEYS > wave_least) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if (t * PA_KEYS + 32 * h + 8 * (i >> 2) + 4 * half + (i & 3) >= sees) s[h][i] = -INFINITY;
-            }
-            float mx = s[0][0];
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[h][i]);
-            mx = pa_other_max(mx) * scale;
-            if (__any(mx > m_run + PA_TAU)) {              // rare: the reference follows the true maximum lazily
-                const float m_new = fmaxf(m_run, mx), alpha = __builtin_amdgcn_exp2f(m_run - m_new);
-                m_run = m_new;
-                l_run *= alpha;
-#pragma unroll
-                for (int c = 0; c < CT; ++c)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) o[c][i] *= alpha;
-            }
-            frag pf[4];
-            float sum = 0.f;
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int g = 0; g < 2; ++g) {
-                    float e[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[h][8 * g + i], scale, -m_run));
-                        sum += e[i];
-                    }
-                    const u32x4 pk = {E::pack(e[0], e[1]), E::pack(e[2], e[3]), E::pack(e[4], e[5]), E::pack(e[6], e[7])};
-                    pf[2 * h + g] = __builtin_bit_cast(frag, pk);
-                }
-            l_run += sum;
-#pragma unroll
-            for (int ks = 0; ks < 4; ++ks)
-#pragma unroll
-                for (int c = 0; c < CT; ++c) {
-                    const uint8_t *at = vt + (16 * ks + vkey) * KP + 16 * ((4 * c + vlow) ^ vsw) + 8 * (l & 1);
-                    const s16x4 lo = lds_read_tr16(reinterpret_cast<const uint16_t *>(at)), hi = lds_read_tr16(reinterpret_cast<const uint16_t *>(at + 8 * KP));
-                    o[c] = E::mfma(__builtin_bit_cast(frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7)), pf[ks], o[c]);
-                }
+            products(no, yes, s0, s2);
         }
-        pa_barrier();                                      // tile t's buffer may be written again
+        for (; t < t_end; ++t) {
+            end_products();
+            request_next();
+            pa_barrier();
+            turn();
+        }
+        if (!late) pa_barrier();                 // (as many as the other half)
     }
 
     const float total = pa_other_sum(l_run);
-    if (row >= rows) return;
+    const long long row_at = (long long)(q0 + tok) * (p.kv_heads * p.group) + head;
     if (splits > 1) {
-        const long long at = ((q0 + tok) * p.kv_heads * p.group + head) * p.splits + split;
+        if (row >= rows) return;
+        const long long at = row_at * p.splits + split;
         float *po = p.part_o + at * D;
 #pragma unroll
         for (int c = 0; c < CT; ++c)
@@ -316,9 +477,13 @@ __global__ __launch_bounds__(64 * W, 2) void prompt_attention_kernel(const PaPar
         }
         return;
     }
-    // a row that sees no key is zeros
+    // Results through LDS (each wave in memory of its own, which no wave reads any more), so that a store writes whole rows.  A row that
+    // sees no key is zeros.
     const float inv = sees > 0 ? 1.0f / total : 0.f;
-    uint16_t *orow = p.out + (q0 + tok) * p.o_t + head * p.o_h + 8 * half;
+    if (p.lse && half == 0 && row < rows) p.lse[row_at] = sees > 0 ? (m_run + __builtin_amdgcn_logf(total)) * 0.693147180559945f : -INFINITY;
+    static_assert(W * 32 * KP <= STAGES * (K_STAGE + K_BYTES), "the results fit");
+    pa_barrier();
+    const uint32_t o_lds = lds0 + w * (32 * KP);
 #pragma unroll
     for (int c = 0; c < CT; ++c)
 #pragma unroll
@@ -331,10 +496,17 @@ __global__ __launch_bounds__(64 * W, 2) void prompt_attention_kernel(const PaPar
                 for (int i = 0; i < 2; ++i) x[k][i] = E::pack(o[c][8 * j + 4 * k + 2 * i] * inv, o[c][8 * j + 4 * k + 2 * i + 1] * inv);
             const auto r0 = __builtin_amdgcn_permlane32_swap(x[0][0], x[1][0], false, false), r1 = __builtin_amdgcn_permlane32_swap(x[0][1], x[1][1], false, false);
             const u32x4 v = {r0[0], r1[0], r0[1], r1[1]};
-            *reinterpret_cast<u32x4_a2 *>(orow + 32 * c + 16 * j) = v;
+            *(__attribute__((address_space(3))) u32x4 *)(o_lds + n * KP + 16 * ((4 * c + 2 * j + half) ^ (D == 128 ? n & 15 : (n >> 1) & 7))) = v;
         }
-    if (p.lse && half == 0)
-        p.lse[(q0 + tok) * p.kv_heads * p.group + head] = sees > 0 ? (m_run + __builtin_amdgcn_logf(total)) * 0.693147180559945f : -INFINITY;
+    asm volatile("" ::: "memory");
+    const long long o_at = (long long)(q0 + tok) * p.o_t + (long long)head * p.o_h;
+#pragma unroll
+    for (int i = 0; i < 32 * KP / 1024; ++i) {
+        const int r = i * PER + l / (KP / 16), piece = l % (KP / 16);
+        const u32x4 v = lds_frag<u32x4>(o_lds + r * KP + 16 * (piece ^ (D == 128 ? r & 15 : (r >> 1) & 7)));
+        const long long at = (long long)((uint64_t)(uint32_t)__shfl((int)o_at, r) | ((uint64_t)(uint32_t)__shfl((int)(o_at >> 32), r) << 32));
+        if (tile * ROWS + 32 * w + r < rows) *reinterpret_cast<u32x4_a2 *>(p.out + at + 8 * piece) = v;
+    }
 }
 
 // The pieces of split rows: a wave per row.  out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i.
@@ -384,8 +556,7 @@ template <typename E, int D, int R>
 hipError_t launch_of(const PaParams &p, hipStream_t stream)
 {
     const unsigned grid = (unsigned)((p.items * p.kv_heads + 7) / 8 * 8);
-    if (p.waves == 8) hipLaunchKernelGGL((prompt_attention_kernel<E, D, R, 8>), dim3(grid), dim3(512), 0, stream, p);
-    else hipLaunchKernelGGL((prompt_attention_kernel<E, D, R, 4>), dim3(grid), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((prompt_attention_kernel<E, D, R>), dim3(grid), dim3(64 * PA_WAVES), 0, stream, p);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.splits <= 1) return e;
     const long long rows = p.total_q * p.kv_heads * p.group;

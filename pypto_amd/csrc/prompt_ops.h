@@ -72,6 +72,8 @@ hipError_t cache_read_launch(const CacheReadParams &p, hipStream_t stream);
 // ---- prompt attention (prompt_attention.hip)
 
 constexpr int PA_KEYS = 64;               // keys of a tile
+constexpr int PA_WAVES = 8;               // of a workgroup, 32 rows each
+constexpr int PA_ROWS = 32 * PA_WAVES;
 
 struct PaParams {
     const uint16_t *q, *qr, *k, *kr, *v;
@@ -82,7 +84,7 @@ struct PaParams {
     long long q_t, q_h, qr_t, qr_h, k_t, k_h, kr_t, kr_h, v_t, v_h, o_t, o_h;   // strides in elements
     long long total_q, total_k;
     int B, kv_heads, group, d, rope, fp16, causal;
-    int waves;                            // of a workgroup: 32 rows each
+    int q_whole;                          // queries come in whole 16-byte pieces
     int splits, split_tiles;              // most splits of a row tile's keys; tiles from which a further split begins
     long long items;                      // most (row tile, split) pairs of a key head
     float scale_log2;
