@@ -191,17 +191,11 @@ int pto_rotary_launch(const PtoRotaryArgs *a, void *hip_stream)
     p.dtype = a->dtype;
     p.layout = a->layout;
     p.factor = (float)a->factor;
-    // A workgroup takes as many tokens as leave four workgroups to a compute unit, up to eight, and all of their heads; with fewer
-    // tokens than that the heads are divided, a pass of rows to a workgroup at least.
-    const long long wanted = 4ll * cu_count();
-    const long long tokens = a->t / wanted;
-    p.tokens_per_wg = (int)(tokens < 1 ? 1 : (tokens > 8 ? 8 : tokens));
-    const long long heads = a->query.heads + (a->key.in ? a->key.heads : 0);
+    // A workgroup takes as many tokens as leave four workgroups to a compute unit, up to four.
     const long long pass = 256 / (a->pairs <= 8 ? 1 : a->pairs <= 16 ? 2 : a->pairs <= 32 ? 4 : a->pairs <= 64 ? 8 : 16);
-    const long long wgs = (a->t + p.tokens_per_wg - 1) / p.tokens_per_wg;
-    long long parts = (heads + pass - 1) / pass;
-    if (parts > wanted / wgs) parts = wanted / wgs < 1 ? 1 : wanted / wgs;
-    p.head_parts = (int)parts;
+    const long long parts = (a->query.heads + pass - 1) / pass + (a->key.in ? (a->key.heads + pass - 1) / pass : 0);
+    const long long tokens = a->t * parts / (4ll * cu_count());
+    p.tokens_per_wg = (int)(tokens < 1 ? 1 : (tokens > pto::ROT_MAX_TOKENS ? pto::ROT_MAX_TOKENS : tokens));
     const hipError_t e = pto::rotary_launch(p, static_cast<hipStream_t>(hip_stream));
     if (e != hipSuccess) return fail(PTO_E_LAUNCH, "rotary: launch failed: %s", hipGetErrorString(e));
     return PTO_OK;
@@ -259,6 +253,8 @@ int pto_cache_read_launch(const PtoCacheReadArgs *a, void *hip_stream)
     p.B = (int)a->b;
     p.maxblk = (int)a->max_blocknum_perbatch;
     p.bs = (int)a->block_size;
+    // Four batches of rows to a wave where that leaves a wave to every SIMD: the next one's rows are then asked for before one is stored.
+    p.batches = a->rows >= 32ll * 4 * cu_count() ? 4 : 1;
     const hipError_t e = pto::cache_read_launch(p, static_cast<hipStream_t>(hip_stream));
     if (e != hipSuccess) return fail(PTO_E_LAUNCH, "cache_read: launch failed: %s", hipGetErrorString(e));
     return PTO_OK;

@@ -100,65 +100,83 @@ __global__ __launch_bounds__(256) void cache_write_kernel(const CacheWriteParams
     if (p.values) *reinterpret_cast<u32x4_a2 *>(p.values + t * p.values_t + 8 * l) = u32x4{value[0], value[1], value[2], value[3]};
 }
 
-// A wave reads eight consecutive rows, two at a time: 32 lanes to a row, sixteen codes and (sixteen of them) four rope channels to a
-// lane; all of its requests of a kind are on their way at once.  Three latencies follow each other: the sequence's
-// beginning, its page, the row.
+// A wave reads batches of eight consecutive rows, two at a time: 32 lanes to a row, of either half of its latent eight channels to a lane
+// (so that a store writes whole cache lines), four rope channels to sixteen of them.  The cache rows of all batches are looked up first, one to
+// a lane: three latencies after one another, of the sequence's beginning, of its page and of the rows.  Then a batch's rows are
+// asked for before those of the batch in front of it are de-quantised and stored.
 constexpr int READ_ROWS = 8;
 
+template <int NB>
 __global__ __launch_bounds__(256) void cache_read_kernel(const CacheReadParams p)
 {
     const int l = threadIdx.x & 63, half = l >> 5, i = l & 31;
-    const long long r0 = ((long long)blockIdx.x * 4 + (threadIdx.x >> 6)) * READ_ROWS;
+    const long long r0 = ((long long)blockIdx.x * 4 + (threadIdx.x >> 6)) * (READ_ROWS * NB);
     if (r0 >= p.rows) return;
     const int s0 = sequence_of(p.cu, p.B, r0);
     if (s0 >= p.B) return;                                 // behind the last sequence
-    constexpr int N = READ_ROWS / 2;
-    long long slot[N];                                     // cache row; -1: no such row; -2: nothing to write
-    int s = s0;
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-        const long long r = r0 + 2 * j + half;
+    int slot = -2;                                         // cache row of output row r0 + l; -1: no such row; -2: nothing to write
+    if (l < READ_ROWS * NB) {
+        const long long r = r0 + l;
+        int s = s0;
         while (s < p.B && p.cu[s + 1] <= r) ++s;
-        slot[j] = -2;
         if (r < p.rows && s < p.B && r >= p.cu[s]) {
             const long long at = r - p.cu[s] + (p.first ? p.first[s] : 0);
-            slot[j] = -1;
+            slot = -1;
             if (at >= 0 && at < (long long)p.maxblk * p.bs) {
-                const int block = (int)(at / p.bs);
+                const int block = (int)((uint64_t)at / (uint32_t)p.bs);
                 const long long page = p.bt[(long long)s * p.maxblk + block];
                 const long long row = page * p.bs + (at - (long long)block * p.bs);
-                if (page >= 0 && row < p.cache.rows) slot[j] = row;
+                if (page >= 0 && row < p.cache.rows) slot = (int)row;
             }
         }
     }
-    u32x4 code[N];
-    u32x2 rope[N];
-    float scale[N];
+    constexpr int N = READ_ROWS / 2;
+    struct Batch {
+        int slot[N];
+        u32x2 code[N][2], rope[N];
+        f32x4 scale[N];
+    };
+    Batch batch[2];
+    auto request = [&](Batch &x, const int nb) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-        code[j] = u32x4{0, 0, 0, 0};
-        rope[j] = u32x2{0, 0};
-        scale[j] = 0.0f;
-        if (slot[j] >= 0) {
-            code[j] = *reinterpret_cast<const u32x4 *>(p.cache.nope + slot[j] * p.cache.nope_pitch + 16 * i);
-            scale[j] = *reinterpret_cast<const float *>(p.cache.scale + slot[j] * p.cache.scale_pitch + 4 * (i >> 3));
-            if (i < 16) rope[j] = *reinterpret_cast<const u32x2 *>(p.cache.rope + slot[j] * p.cache.rope_pitch + 8 * i);
+        for (int j = 0; j < N; ++j) {
+            x.slot[j] = __shfl(slot, nb * READ_ROWS + 2 * j + half);
+            x.code[j][0] = x.code[j][1] = x.rope[j] = u32x2{0, 0};
+            x.scale[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (x.slot[j] >= 0) {
+                const uint8_t *row = p.cache.nope + (long long)x.slot[j] * p.cache.nope_pitch;
+                x.code[j][0] = *reinterpret_cast<const u32x2 *>(row + 8 * i);
+                x.code[j][1] = *reinterpret_cast<const u32x2 *>(row + 256 + 8 * i);
+                x.scale[j] = *reinterpret_cast<const f32x4 *>(p.cache.scale + (long long)x.slot[j] * p.cache.scale_pitch);
+                if (i < 16) x.rope[j] = *reinterpret_cast<const u32x2 *>(p.cache.rope + (long long)x.slot[j] * p.cache.rope_pitch + 8 * i);
+            }
         }
-    }
+    };
+    auto finish = [&](const Batch &x, const int nb) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-        if (slot[j] < -1) continue;
-        const long long r = r0 + 2 * j + half;
-        u32x4 out[2];
+        for (int j = 0; j < N; ++j) {
+            if (x.slot[j] < -1) continue;
+            const long long r = r0 + nb * READ_ROWS + 2 * j + half;
+            uint16_t *dst = p.latent + r * p.latent_t + 8 * i;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const uint32_t w = code[j][k >> 1] >> (16 * (k & 1));
-            out[k >> 2][k & 3] = pack_bf16x2((float)(int8_t)(w & 0xff) * scale[j], (float)(int8_t)((w >> 8) & 0xff) * scale[j]);
+            for (int h = 0; h < 2; ++h) {
+                const float scale = i < 16 ? x.scale[j][2 * h] : x.scale[j][2 * h + 1];
+                u32x4 out;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const uint32_t w = x.code[j][h][k >> 1] >> (16 * (k & 1));
+                    out[k] = pack_bf16x2((float)(int8_t)(w & 0xff) * scale, (float)(int8_t)((w >> 8) & 0xff) * scale);
+                }
+                __builtin_nontemporal_store((u32x4_a2)out, reinterpret_cast<u32x4_a2 *>(dst + 256 * h));
+            }
+            if (i < 16) __builtin_nontemporal_store((u32x2_a2)x.rope[j], reinterpret_cast<u32x2_a2 *>(p.rope + r * p.rope_t + 4 * i));
         }
-        uint16_t *dst = p.latent + r * p.latent_t + 16 * i;
-        *reinterpret_cast<u32x4_a2 *>(dst) = out[0];
-        *reinterpret_cast<u32x4_a2 *>(dst + 8) = out[1];
-        if (i < 16) *reinterpret_cast<u32x2_a2 *>(p.rope + r * p.rope_t + 4 * i) = rope[j];
+    };
+    request(batch[0], 0);
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+        if (nb + 1 < NB) request(batch[(nb + 1) & 1], nb + 1);
+        finish(batch[nb & 1], nb);
     }
 }
 
@@ -175,8 +193,10 @@ hipError_t cache_write_launch(const CacheWriteParams &p, hipStream_t stream)
 
 hipError_t cache_read_launch(const CacheReadParams &p, hipStream_t stream)
 {
-    constexpr int rows = 4 * READ_ROWS;
-    hipLaunchKernelGGL(cache_read_kernel, dim3((unsigned)((p.rows + rows - 1) / rows)), dim3(256), 0, stream, p);
+    const int rows = 4 * READ_ROWS * p.batches;
+    const dim3 grid((unsigned)((p.rows + rows - 1) / rows));
+    if (p.batches == 4) hipLaunchKernelGGL(cache_read_kernel<4>, grid, dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL(cache_read_kernel<1>, grid, dim3(256), 0, stream, p);
     return hipGetLastError();
 }
 

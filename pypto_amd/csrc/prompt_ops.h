@@ -9,6 +9,7 @@ namespace pto {
 // ---- rotary positions (rotary_kernels.hip)
 
 constexpr int ROT_MAX_PAIRS = 128;
+constexpr int ROT_MAX_TOKENS = 4;         // of a workgroup
 
 struct RotaryTablesParams {
     const void *positions;    // [T] int64 or int32
@@ -34,7 +35,8 @@ struct RotaryParams {
     long long T;
     int pairs, wide, dtype, layout;
     float factor;
-    int tokens_per_wg, head_parts;
+    int tokens_per_wg;
+    int query_parts, key_parts;           // workgroups that share a token's heads (set by rotary_launch)
 };
 hipError_t rotary_launch(const RotaryParams &p, hipStream_t stream);
 
@@ -66,6 +68,7 @@ struct CacheReadParams {
     long long latent_t, rope_t;           // strides in elements
     long long rows;                       // of the outputs
     int B, maxblk, bs;
+    int batches;                          // of eight rows to a wave: 1 or 4
 };
 hipError_t cache_read_launch(const CacheReadParams &p, hipStream_t stream);
 

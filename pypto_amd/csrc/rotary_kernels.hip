@@ -37,43 +37,54 @@ __device__ __forceinline__ double position_of(const void *positions, const int w
 typedef uint32_t u32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
 
 template <int DT>
-struct Eight {
-    float v[8];
+struct Raw {
+    u32x4 w[DT == PTO_DT_FP32 ? 2 : 1];
     __device__ __forceinline__ void load(const void *base, const long long at)
     {
         if (DT == PTO_DT_FP32) {
             const float *p = static_cast<const float *>(base) + at;
-            const u32x4_a4 a = *reinterpret_cast<const u32x4_a4 *>(p), b = *reinterpret_cast<const u32x4_a4 *>(p + 4);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(a[i]), v[4 + i] = __uint_as_float(b[i]);
+            w[0] = *reinterpret_cast<const u32x4_a4 *>(p), w[DT == PTO_DT_FP32] = *reinterpret_cast<const u32x4_a4 *>(p + 4);
         } else {
-            const u32x4 a = *reinterpret_cast<const u32x4_a2 *>(static_cast<const uint16_t *>(base) + at);
+            w[0] = *reinterpret_cast<const u32x4_a2 *>(static_cast<const uint16_t *>(base) + at);
+        }
+    }
+};
+
+template <int DT>
+struct Eight {
+    float v[8];
+    __device__ __forceinline__ Eight() {}
+    __device__ __forceinline__ explicit Eight(const Raw<DT> &r)
+    {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (DT == PTO_DT_BF16) {
-                    v[2 * i] = __uint_as_float(a[i] << 16), v[2 * i + 1] = __uint_as_float(a[i] & 0xffff0000u);
-                } else {
-                    const f16x2 h = __builtin_bit_cast(f16x2, (uint32_t)a[i]);
-                    v[2 * i] = (float)h[0], v[2 * i + 1] = (float)h[1];
-                }
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t a = r.w[0][i];
+            if (DT == PTO_DT_FP32) {
+                v[i] = __uint_as_float(a), v[4 + i] = __uint_as_float(r.w[DT == PTO_DT_FP32][i]);
+            } else if (DT == PTO_DT_BF16) {
+                v[2 * i] = __uint_as_float(a << 16), v[2 * i + 1] = __uint_as_float(a & 0xffff0000u);
+            } else {
+                const f16x2 h = __builtin_bit_cast(f16x2, a);
+                v[2 * i] = (float)h[0], v[2 * i + 1] = (float)h[1];
             }
         }
     }
+    // (to be thrown out of the caches first: 34 us, where ordinary stores push the rows still to be read out, 37)
     __device__ __forceinline__ void store(void *base, const long long at) const
     {
         if (DT == PTO_DT_FP32) {
-            float *p = static_cast<float *>(base) + at;
+            u32x4_a4 *p = reinterpret_cast<u32x4_a4 *>(static_cast<float *>(base) + at);
             u32x4_a4 a, b;
 #pragma unroll
             for (int i = 0; i < 4; ++i) a[i] = __float_as_uint(v[i]), b[i] = __float_as_uint(v[4 + i]);
-            *reinterpret_cast<u32x4_a4 *>(p) = a;
-            *reinterpret_cast<u32x4_a4 *>(p + 4) = b;
+            __builtin_nontemporal_store(a, p);
+            __builtin_nontemporal_store(b, p + 1);
         } else {
             u32x4 a;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 a[i] = DT == PTO_DT_BF16 ? pack_bf16x2(v[2 * i], v[2 * i + 1]) : pack_f16x2(v[2 * i], v[2 * i + 1]);
-            *reinterpret_cast<u32x4_a2 *>(static_cast<uint16_t *>(base) + at) = a;
+            __builtin_nontemporal_store((u32x4_a2)a, reinterpret_cast<u32x4_a2 *>(static_cast<uint16_t *>(base) + at));
         }
     }
 };
@@ -122,91 +133,104 @@ __global__ __launch_bounds__(256) void rotary_tables_kernel(const RotaryTablesPa
     }
 }
 
-// A workgroup makes the turns of a few tokens once, in LDS, and takes them through all heads, queries' and keys' rows one after
-// the other.  A row is a group of LPR lanes of one wave, eight pairs to a lane: every lane's loads precede the row's
-// stores, so a row may be turned where it lies whatever its layout.
+// A workgroup makes the turns of up to four tokens once, in LDS, and takes them through its heads.  A row (a token's head) is a group of LPR
+// lanes of one wave, eight pairs to a lane; a group takes a head through all of the tokens at once, and every lane's loads precede its
+// group's stores: so a row may be turned where it lies whatever its layout.
+// Bound by memory: 64 of 192 channels of 4096 tokens of 128 heads, bf16, 135 MB in 30 us = 4.5 TB/s, where a plain copy of as much takes 27;
+// one row of a group at a time 43 us, results stored as if they were wanted soon 34.
 template <int DT, int LPR>
 __global__ __launch_bounds__(256) void rotary_kernel(const RotaryParams p)
 {
-    __shared__ Turn turns[8 * ROT_MAX_PAIRS];              // at most eight tokens to a workgroup
+    __shared__ Turn turns[ROT_MAX_TOKENS * ROT_MAX_PAIRS];
     const int tid = threadIdx.x;
-    const long long t0 = (long long)blockIdx.x * p.tokens_per_wg;
+    const int parts = p.query_parts + p.key_parts, part = (int)(blockIdx.x % (unsigned)parts);    // (a token's heads side by side)
+    const long long t0 = (long long)(blockIdx.x / (unsigned)parts) * p.tokens_per_wg;
     const int tokens = p.T - t0 < p.tokens_per_wg ? (int)(p.T - t0) : p.tokens_per_wg;
-    for (int i = tid; i < tokens * p.pairs; i += 256) {
-        const int t = i / p.pairs;
-        turns[i] = turn_of(position_of(p.positions, p.wide, t0 + t), p.freq[i - t * p.pairs], p.factor);
-    }
-    __syncthreads();
 
     const int lane = tid & (LPR - 1);
     const bool mine = 8 * lane < p.pairs;                  // (of a group some lanes may have no pairs)
     const int pair = mine ? 8 * lane : 0;
-    const int heads = p.side[0].heads + p.side[1].heads;
-    // this workgroup's share of every token's heads
-    const int share = (heads + p.head_parts - 1) / p.head_parts;
-    const int h_begin = blockIdx.y * share;
-    const int h_end = h_begin + share < heads ? h_begin + share : heads;
-    const int width = h_end - h_begin;
-    if (width <= 0) return;
-    const int rows = tokens * width;
-    for (int r = tid / LPR; r < rows; r += 256 / LPR) {
-        const int t = r / width;
-        int h = h_begin + r - t * width;
-        const bool key = h >= p.side[0].heads;
-        const RotarySide &s = p.side[key ? 1 : 0];
-        h -= key ? p.side[0].heads : 0;
-        const long long from = (t0 + t) * s.in_t + h * s.in_h, to = (t0 + t) * s.out_t + h * s.out_h;
-        Eight<DT> a, b;
-        if (mine) {
-            const long long at = from + s.offset;
-            a.load(s.in, at + (p.layout == PTO_ROPE_HALF ? pair : 2 * pair));
-            b.load(s.in, at + (p.layout == PTO_ROPE_HALF ? pair + p.pairs : 2 * pair + 8));
-            if (p.layout != PTO_ROPE_HALF) {               // first and second halves of the eight pairs
-                Eight<DT> x, y;
+    const bool half = p.layout == PTO_ROPE_HALF;
+    const int first = half ? pair : 2 * pair, second = half ? pair + p.pairs : 2 * pair + 8;
+    const bool halves = p.layout != PTO_ROPE_INTERLEAVED;  // of what is stored
+    const int first_out = halves ? pair : 2 * pair, second_out = halves ? pair + p.pairs : 2 * pair + 8;
+    // this workgroup's heads: of the queries, or behind them of the keys
+    const bool key = part >= p.query_parts;
+    const RotarySide &s = p.side[key ? 1 : 0];
+    const int h = (part - (key ? p.query_parts : 0)) * (256 / LPR) + tid / LPR;
+    const bool there = h < s.heads;
+    const long long from = t0 * s.in_t + (there ? h : 0) * s.in_h, to = t0 * s.out_t + (there ? h : 0) * s.out_h;
+
+    Raw<DT> ra[ROT_MAX_TOKENS], rb[ROT_MAX_TOKENS];
+    if (mine && there) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) x.v[i] = a.v[2 * i], x.v[4 + i] = b.v[2 * i], y.v[i] = a.v[2 * i + 1], y.v[4 + i] = b.v[2 * i + 1];
-                a = x, b = y;
+        for (int j = 0; j < ROT_MAX_TOKENS; ++j)
+            if (j < tokens) {
+                const long long at = from + j * s.in_t + s.offset;
+                ra[j].load(s.in, at + first);
+                rb[j].load(s.in, at + second);
             }
-            const Turn *w = turns + t * p.pairs + pair;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float x = a.v[i], y = b.v[i], c = w[i].c, z = w[i].s;
-                a.v[i] = x * c - y * z;
-                b.v[i] = y * c + x * z;
-            }
-            if (p.layout == PTO_ROPE_INTERLEAVED) {
-                Eight<DT> x, y;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) x.v[2 * i] = a.v[i], x.v[2 * i + 1] = b.v[i], y.v[2 * i] = a.v[4 + i], y.v[2 * i + 1] = b.v[4 + i];
-                a = x, b = y;
-            }
-        }
-        if (s.copies) {                                    // the channels around the part that turns
-            const int rest = s.dim - 2 * p.pairs;
+    }
+    for (int i = tid; i < tokens * p.pairs; i += 256) {    // (the rows are on their way)
+        const int t = i / p.pairs;
+        turns[i] = turn_of(position_of(p.positions, p.wide, t0 + t), p.freq[i - t * p.pairs], p.factor);
+    }
+    __syncthreads();
+    if (!there) return;
+    if (s.copies) {                                        // the channels around the part that turns
+        const int rest = s.dim - 2 * p.pairs;
+        for (int j = 0; j < tokens; ++j)
             for (int c = lane; c < rest; c += LPR) {
                 const int ch = c < s.offset ? c : c + 2 * p.pairs;
-                copy_one<DT>(s.in, from + ch, s.out, to + ch);
+                copy_one<DT>(s.in, from + j * s.in_t + ch, s.out, to + j * s.out_t + ch);
             }
+    }
+#pragma unroll
+    for (int j = 0; j < ROT_MAX_TOKENS; ++j) {
+        if (!mine || j >= tokens) continue;
+        Eight<DT> x(ra[j]), y(rb[j]), c, d;
+        if (half) {
+            c = x, d = y;
+        } else {                                           // first and second members of the eight pairs
+#pragma unroll
+            for (int i = 0; i < 4; ++i) c.v[i] = x.v[2 * i], c.v[4 + i] = y.v[2 * i], d.v[i] = x.v[2 * i + 1], d.v[4 + i] = y.v[2 * i + 1];
         }
-        if (mine) {
-            const long long at = to + s.offset;
-            const bool halves = p.layout != PTO_ROPE_INTERLEAVED;
-            a.store(s.out, at + (halves ? pair : 2 * pair));
-            b.store(s.out, at + (halves ? pair + p.pairs : 2 * pair + 8));
+        const Turn *w = turns + j * p.pairs + pair;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float u = c.v[i], v = d.v[i], co = w[i].c, si = w[i].s;
+            c.v[i] = u * co - v * si;
+            d.v[i] = v * co + u * si;
         }
+        if (!halves) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x.v[2 * i] = c.v[i], x.v[2 * i + 1] = d.v[i], y.v[2 * i] = c.v[4 + i], y.v[2 * i + 1] = d.v[4 + i];
+            c = x, d = y;
+        }
+        const long long at = to + j * s.out_t + s.offset;
+        c.store(s.out, at + first_out);
+        d.store(s.out, at + second_out);
     }
 }
 
+template <int DT, int LPR>
+hipError_t rotary_with(RotaryParams p, hipStream_t stream)
+{
+    constexpr int rows = 256 / LPR;
+    p.query_parts = (p.side[0].heads + rows - 1) / rows;
+    p.key_parts = (p.side[1].heads + rows - 1) / rows;
+    const long long grid = (p.T + p.tokens_per_wg - 1) / p.tokens_per_wg * (p.query_parts + p.key_parts);
+    if (grid > 0x7fffffffll) return hipErrorInvalidConfiguration;
+    hipLaunchKernelGGL((rotary_kernel<DT, LPR>), dim3((unsigned)grid), dim3(256), 0, stream, p);
+    return hipGetLastError();
+}
+
 template <int DT>
-hipError_t rotary_of(const RotaryParams &p, const dim3 grid, hipStream_t stream)
+hipError_t rotary_of(const RotaryParams &p, hipStream_t stream)
 {
     const int lanes = p.pairs / 8;
-    if (lanes <= 1) hipLaunchKernelGGL((rotary_kernel<DT, 1>), grid, dim3(256), 0, stream, p);
-    else if (lanes <= 2) hipLaunchKernelGGL((rotary_kernel<DT, 2>), grid, dim3(256), 0, stream, p);
-    else if (lanes <= 4) hipLaunchKernelGGL((rotary_kernel<DT, 4>), grid, dim3(256), 0, stream, p);
-    else if (lanes <= 8) hipLaunchKernelGGL((rotary_kernel<DT, 8>), grid, dim3(256), 0, stream, p);
-    else hipLaunchKernelGGL((rotary_kernel<DT, 16>), grid, dim3(256), 0, stream, p);
-    return hipGetLastError();
+    return lanes <= 1 ? rotary_with<DT, 1>(p, stream) : lanes <= 2 ? rotary_with<DT, 2>(p, stream) : lanes <= 4 ? rotary_with<DT, 4>(p, stream)
+         : lanes <= 8 ? rotary_with<DT, 8>(p, stream) : rotary_with<DT, 16>(p, stream);
 }
 
 }  // namespace
@@ -223,10 +247,9 @@ hipError_t rotary_tables_launch(const RotaryTablesParams &p, hipStream_t stream)
 
 hipError_t rotary_launch(const RotaryParams &p, hipStream_t stream)
 {
-    const dim3 grid((unsigned)((p.T + p.tokens_per_wg - 1) / p.tokens_per_wg), (unsigned)p.head_parts);
-    if (p.dtype == PTO_DT_FP32) return rotary_of<PTO_DT_FP32>(p, grid, stream);
-    if (p.dtype == PTO_DT_BF16) return rotary_of<PTO_DT_BF16>(p, grid, stream);
-    return rotary_of<PTO_DT_FP16>(p, grid, stream);
+    if (p.dtype == PTO_DT_FP32) return rotary_of<PTO_DT_FP32>(p, stream);
+    if (p.dtype == PTO_DT_BF16) return rotary_of<PTO_DT_BF16>(p, stream);
+    return rotary_of<PTO_DT_FP16>(p, stream);
 }
 
 }  // namespace pto
