@@ -97,7 +97,7 @@ __global__ __launch_bounds__(256) void cache_write_kernel(const CacheWriteParams
         *reinterpret_cast<uint16_t *>(p.cache.rope + row * p.cache.rope_pitch + 2 * l) = (uint16_t)pack_bf16x2(rope, rope);
         if ((l & 15) == 0) *reinterpret_cast<float *>(p.cache.scale + row * p.cache.scale_pitch + (l >> 2)) = scale;
     }
-    if (p.values) *reinterpret_cast<u32x4_a2 *>(p.values + t * p.values_t + 8 * l) = u32x4{value[0], value[1], value[2], value[3]};
+    if (p.values) __builtin_nontemporal_store((u32x4_a2)u32x4{value[0], value[1], value[2], value[3]}, reinterpret_cast<u32x4_a2 *>(p.values + t * p.values_t + 8 * l));
 }
 
 // A wave reads batches of eight consecutive rows, two at a time: 32 lanes to a row, of either half of its latent eight channels to a lane
