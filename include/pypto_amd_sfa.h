@@ -632,7 +632,7 @@ typedef struct PtoPromptPlan {
     int64_t rows_per_workgroup; /* (query, head of a group) pairs */
     int64_t key_splits;         /* most pieces that a workgroup's keys are divided into */
     int64_t split_keys;         /* keys of a sequence from which a further piece begins */
-    int64_t items;              /* workgroups per key head, at most */
+    int64_t workgroups;         /* of the launch */
 } PtoPromptPlan;
 int pto_prompt_attention_plan(const PtoPromptAttentionArgs *args, PtoPromptPlan *plan);
 int pto_prompt_attention_launch(const PtoPromptAttentionArgs *args, void *hip_stream);

@@ -100,37 +100,61 @@ int attention_check(const PtoPromptAttentionArgs *a)
 
 struct PromptPlan {
     int splits, split_tiles;
-    long long items;
+    long long workgroups;
     size_t o_bytes, ml_bytes;
 };
+
+// Dividing a call's keys.  The host knows how many rows, keys and sequences there are, not which sequence has how many, and takes them for
+// dealt out evenly.  In microseconds: a workgroup starts and ends in `fixed`, takes `tile` for 64 keys, and partial results are written
+// and read back by a launch of their own, a tenth of a microsecond to a piece.  With s pieces to the longest row tile a launch takes the longest workgroup and then, for the rounds
+// of the chip behind the first, the mean one.  Cheapest s first; what is fixed is the length of a piece, so a sequence longer than the mean
+// is divided into more.  Where the cheapest is one piece and the workgroups are few and long, sequences a quarter longer than the mean are
+// divided all the same, and where they are very long all are, in pieces of half of the mean: one that is much longer would be there alone at the
+// end (32 sequences of 700 to 12000 keys, 8 key heads: 200 us, now 187).  A launch has a workgroup for each row tile, or piece of one, that there can be, and the device starts the next as one
+// ends; where that could be more than four for each compute unit, the workgroups of a divided launch take the pieces there are in turn.
+constexpr size_t PA_MOST_PARTIALS = (size_t)256 << 20;
 
 PromptPlan attention_plan(const PtoPromptAttentionArgs *a)
 {
     PromptPlan pl{};
-    const int cus = cu_count() > 0 ? cu_count() : 256;
+    const long long cus = cu_count() > 0 ? cu_count() : 256;
     const long long rows = a->total_q * (a->heads / a->kv_heads);
-    const long long tile = pto::PA_ROWS;
-    const long long tiles = rows / tile + a->b;            // of a key head, at most
-    const long long per_seq = (rows + tile - 1) / tile;    // of one sequence, at most
-    const long long key_tiles = (a->total_k + pto::PA_KEYS - 1) / pto::PA_KEYS + a->b;
+    const long long most_tiles = rows / pto::PA_ROWS + a->b;                                // of a key head
+    const long long key_tiles = (a->total_k + pto::PA_KEYS - 1) / pto::PA_KEYS;             // of one sequence, at most
     pl.splits = 1;
     pl.split_tiles = 1 << 24;
-    pl.items = tiles;
-    const long long wanted = 2ll * cus;                    // workgroups
-    const long long least = rows / tile + 1;               // row tiles that there surely are
-    if (least * a->kv_heads < cus) {
-        // tiles of a piece: so many that the launch has about `wanted` pieces, four at least
-        long long len = (key_tiles * per_seq * a->kv_heads + wanted - 1) / wanted;
-        len = len < 4 ? 4 : len;
-        long long most = (key_tiles + len - 1) / len;
-        most = most > 128 ? 128 : most;
-        if (most > 1) {
-            pl.splits = (int)most;
+    pl.workgroups = most_tiles * a->kv_heads;
+
+    const double seq_rows = (double)rows / a->b;
+    const double items = (seq_rows <= pto::PA_ROWS ? (double)a->b : (double)rows / pto::PA_ROWS + (a->b > 1 ? 0.5 * a->b : 0.0)) * a->kv_heads;
+    const double longest = std::ceil((double)a->total_k / a->b / pto::PA_KEYS);
+    const double mean = a->causal && a->total_k >= a->total_q ? ((double)a->total_k - 0.5 * a->total_q) / a->b / pto::PA_KEYS : longest;
+    if (items < 2.0 * cus && longest > 1.0) {
+        const double fixed = 9.0, tile = a->d == 64 ? 1.1 : (a->query_rope ? 2.05 : 1.65);
+        const double partial = (double)a->total_q * a->heads * (a->d + 2) * sizeof(float);
+        auto pieces_of = [&](const long long len) { return (key_tiles + len - 1) / len; };
+        auto cost = [&](const double s) {
+            const double len = std::ceil(longest / s), rounds = std::ceil(std::ceil(items) * s / cus);
+            return fixed + tile * len + (rounds - 1.0) * (fixed + tile * mean / s) + (s > 1.0 ? 3.5 + s * (0.1 + partial * 0.5e-6) : 0.0);
+        };
+        double best = cost(1.0), s_best = 1.0;
+        for (double s = 2.0; s <= longest && s <= pto::PA_MAX_SPLITS; s += 1.0)
+            if (cost(s) < best) best = cost(s), s_best = s;
+        long long len = (long long)std::ceil(longest / s_best);
+        if (s_best == 1.0) {
+            const bool uneven = a->b > 1 && items <= 1.5 * cus;
+            len = uneven && tile * longest >= 8.0 * fixed ? (len + 1) / 2 : uneven && tile * longest >= 3.0 * fixed ? len + len / 4 + 1 : key_tiles;
+        }
+        while (pieces_of(len) > pto::PA_MAX_SPLITS || (len < key_tiles && partial * (double)pieces_of(len) > (double)PA_MOST_PARTIALS)) len += (len + 3) / 4;
+        if (pieces_of(len) > 1) {
+            pl.splits = (int)pieces_of(len);
             pl.split_tiles = (int)len;
-            const long long by_tiles = tiles * most, by_keys = per_seq * (key_tiles / len + 1 + a->b);
-            pl.items = by_tiles < by_keys ? by_tiles : by_keys;
+            const long long by_tiles = most_tiles * pl.splits, by_keys = ((rows + pto::PA_ROWS - 1) / pto::PA_ROWS) * (key_tiles / len + a->b + 1);
+            pl.workgroups = (by_tiles < by_keys ? by_tiles : by_keys) * a->kv_heads;
+            if (pl.workgroups > 4 * cus) pl.workgroups = 4 * cus;
         }
     }
+    pl.workgroups = (pl.workgroups + 7) / 8 * 8;
     if (pl.splits > 1) {
         pl.o_bytes = (size_t)a->total_q * a->heads * pl.splits * a->d * sizeof(float);
         pl.ml_bytes = (size_t)a->total_q * a->heads * pl.splits * 2 * sizeof(float);
@@ -279,7 +303,7 @@ int pto_prompt_attention_plan(const PtoPromptAttentionArgs *a, PtoPromptPlan *pl
     plan->rows_per_workgroup = pto::PA_ROWS;
     plan->key_splits = pl.splits;
     plan->split_keys = (int64_t)pl.split_tiles * pto::PA_KEYS;
-    plan->items = pl.items;
+    plan->workgroups = pl.workgroups;
     return PTO_OK;
 }
 
@@ -304,7 +328,7 @@ int pto_prompt_attention_launch(const PtoPromptAttentionArgs *a, void *hip_strea
     if (need > 0 && (!a->workspace || a->workspace_bytes < need))
         return fail(PTO_E_WORKSPACE, "prompt_attention: workspace of %zu bytes required, %zu given", need, a->workspace ? a->workspace_bytes : (size_t)0);
     if (!aligned(a->workspace, 16)) return fail(PTO_E_INVALID_ARG, "prompt_attention: the workspace must be 16-byte aligned");
-    if (pl.items * a->kv_heads > 0x7ffffff0ll || a->total_q * a->heads / 4 > 0x7ffffff0ll)
+    if (pl.workgroups > 0x7ffffff0ll || a->total_q * a->heads / 4 > 0x7ffffff0ll)
         return fail(PTO_E_INVALID_ARG, "prompt_attention: the call exceeds the largest launch");
 
     pto::PaParams p{};
@@ -337,7 +361,7 @@ int pto_prompt_attention_launch(const PtoPromptAttentionArgs *a, void *hip_strea
                 a->query_rope_stride_t % 8 == 0 && a->query_rope_stride_h % 8 == 0;
     p.splits = pl.splits;
     p.split_tiles = pl.split_tiles;
-    p.items = pl.items;
+    p.grid = (int)pl.workgroups;
     p.scale_log2 = a->softmax_scale * 1.4426950408889634f;
     const hipError_t e = pto::prompt_attention_launch(p, static_cast<hipStream_t>(hip_stream));
     if (e != hipSuccess) return fail(PTO_E_LAUNCH, "prompt_attention: launch failed: %s", hipGetErrorString(e));

@@ -118,46 +118,58 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void prompt_attention_kernel(cons
     constexpr int K_BYTES = K_REQS * REQ, R_BYTES = R_REQS * 1024;
     constexpr int K_STAGE = K_BYTES + R_BYTES;             // [keys | rope keys] of a tile
     constexpr int STAGES = 3, AHEAD = 5;
+    constexpr int POOL = STAGES * (K_STAGE + K_BYTES) > W * 32 * 256 ? STAGES * (K_STAGE + K_BYTES) : W * 32 * 256;   // (results: 256 bytes to a row)
     constexpr int KS = D / 16, RS = R / 16, CT = D / 32;
     constexpr int NK = K_REQS / W, NR = R_REQS / W;   // requests of a wave per tile: keys (as many values), rope keys
     static_assert(K_REQS % W == 0 && R_REQS % W == 0, "whole requests for every wave");
     typedef typename E::frag frag;
 
-    __shared__ __attribute__((aligned(1024))) uint8_t pool[STAGES * (K_STAGE + K_BYTES)];   // keys of three tiles, then their values
+    __shared__ __attribute__((aligned(1024))) uint8_t pool[POOL];   // keys of three tiles, then their values
 
-    const int tid = threadIdx.x, l = tid & 63, n = l & 31, half = l >> 5;
+    const int tid = threadIdx.x;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
 
-    // Workgroup -> (key head, sequence, row tile, split).  An XCD takes consecutive items, so that workgroups which read the same
-    // head's keys share an L2; a sequence's last rows, which see the most keys, come first.  (Fewer than 2^31 items: the host.)
-    const int per_xcd = (int)((p.items * p.kv_heads + 7) / 8), slot = blockIdx.x >> 3;
-    const int item = (blockIdx.x & 7) * per_xcd + slot;
-    if (item >= p.items * p.kv_heads || slot >= per_xcd) return;
-    const int kvh = item / (int)p.items;
-    int rest = item - kvh * (int)p.items;
-    int b = -1, lq = 0, lk = 0, q0 = 0, k0 = 0, tiles = 0, splits = 1;
-    for (int base = 0; base < p.B; base += 64) {
-        const int mine = base + l < p.B ? base + l : p.B - 1;
-        const Span sq = span_of(p.cu_q, mine, (int)p.total_q), sk = span_of(p.cu_k, mine, (int)p.total_k);
-        const int mt = base + l < p.B ? (sq.len * p.group + ROWS - 1) / ROWS : 0;
-        const int ms = pa_splits_of((sk.len + PA_KEYS - 1) / PA_KEYS, p.split_tiles, p.splits);
-        const int upto = wave_sums(mt * ms);               // items of this and all sequences before it (of these 64)
-        const uint64_t past = __ballot(upto > rest);
-        if (past != 0) {
-            const int who = __builtin_ctzll(past);
-            b = base + who;
-            rest -= who > 0 ? __builtin_amdgcn_readlane(upto, who - 1) : 0;
-            lq = __builtin_amdgcn_readlane(sq.len, who), lk = __builtin_amdgcn_readlane(sk.len, who);
-            q0 = __builtin_amdgcn_readlane(sq.begin, who), k0 = __builtin_amdgcn_readlane(sk.begin, who);
-            tiles = __builtin_amdgcn_readlane(mt, who), splits = __builtin_amdgcn_readlane(ms, who);
-            break;
-        }
-        rest -= __builtin_amdgcn_readlane(upto, 63);
+    // Items of work: (key head, sequence, row tile, piece of its keys), counted from the lengths.  An XCD takes consecutive ones, so that
+    // workgroups which read the same head's keys share an L2; a sequence's last rows, which see the most keys, come first.
+    struct Scan {                                          // of 64 sequences, one to a lane
+        Span sq, sk;
+        int tiles, splits, upto;                           // upto: items of a key head in this and all sequences before it (of these 64)
+    };
+    auto scan = [&](const int base) __attribute__((always_inline)) {
+        Scan c;
+        const int l = tid & 63, mine = base + l < p.B ? base + l : p.B - 1;
+        c.sq = span_of(p.cu_q, mine, (int)p.total_q), c.sk = span_of(p.cu_k, mine, (int)p.total_k);
+        c.tiles = base + l < p.B ? (c.sq.len * p.group + ROWS - 1) / ROWS : 0;
+        c.splits = pa_splits_of((c.sk.len + PA_KEYS - 1) / PA_KEYS, p.split_tiles, p.splits);
+        c.upto = wave_sums(c.tiles * c.splits);
+        return c;
+    };
+    Scan c = scan(0);
+    int per_head = __builtin_amdgcn_readlane(c.upto, 63);
+    for (int base = 64; base < p.B; base += 64) per_head += __builtin_amdgcn_readlane(scan(base).upto, 63);
+    const int items = per_head * p.kv_heads, per_xcd = (items + 7) / 8, first = (blockIdx.x & 7) * per_xcd;
+    const int here = items - first < per_xcd ? items - first : per_xcd;                     // items of this XCD
+  for (int slot = blockIdx.x >> 3; slot < here; slot += gridDim.x >> 3) {
+    // An XCD deals its workgroups to four groups of compute units in turn, whichever is free: every second four go backwards, so that
+    // where a head has 4 n row tiles the same group does not get the longest of all of them (128 heads of 16 tiles 676 us, now 651).
+    const int item = first + ((slot & 4) != 0 && (slot | 3) < here ? slot ^ 3 : slot);
+    const int kvh = item / per_head;
+    // (nothing that hangs on the lane alone is kept from one item to the next: it would take the registers of the products' operands)
+    const int l = (int)opaque(tid & 63), n = l & 31, half = l >> 5;
+    int rest = item - kvh * per_head, base = 0;
+    while (rest >= __builtin_amdgcn_readlane(c.upto, 63)) {
+        rest -= __builtin_amdgcn_readlane(c.upto, 63);
+        base += 64;
+        c = scan(base);
     }
-    if (b < 0) return;
+    const int who = __builtin_ctzll(__ballot(c.upto > rest));
+    rest -= who > 0 ? __builtin_amdgcn_readlane(c.upto, who - 1) : 0;
+    const int lq = __builtin_amdgcn_readlane(c.sq.len, who), lk = __builtin_amdgcn_readlane(c.sk.len, who);
+    const int q0 = __builtin_amdgcn_readlane(c.sq.begin, who), k0 = __builtin_amdgcn_readlane(c.sk.begin, who);
+    const int splits = __builtin_amdgcn_readlane(c.splits, who);
     const int which = splits > 1 ? rest / splits : rest;
     const int split = rest - which * splits;
-    const int tile = p.causal ? tiles - 1 - which : which;
+    const int tile = p.causal ? __builtin_amdgcn_readlane(c.tiles, who) - 1 - which : which;
 
     // This lane's row, and how many keys it sees.  Rows past the last one stand in with it and are never stored.
     const int rows = lq * p.group;
@@ -245,10 +257,10 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void prompt_attention_kernel(cons
     frag qf[KS + RS];
     const long long q_at = (long long)(q0 + tok) * p.q_t + (long long)head * p.q_h, qr_at = R > 0 ? (long long)(q0 + tok) * p.qr_t + (long long)head * p.qr_h : 0;
     constexpr int Q_WAVE = 32 * (KP + 2 * R);
-    static_assert(K_STAGE + W * Q_WAVE <= STAGES * (K_STAGE + K_BYTES), "the queries fit beside the first tile's keys");
+    static_assert(K_STAGE + W * Q_WAVE <= POOL, "the queries fit beside the first tile's keys");
     const uint32_t q_lds = lds0 + K_STAGE + w * Q_WAVE;
+    auto of_row = [](const long long at, const int r) { return (long long)((uint64_t)(uint32_t)__shfl((int)at, r) | ((uint64_t)(uint32_t)__shfl((int)(at >> 32), r) << 32)); };
     auto request_queries = [&]() __attribute__((always_inline)) {
-        auto of_row = [](const long long at, const int r) { return (uint64_t)(uint32_t)__shfl((int)at, r) | ((uint64_t)(uint32_t)__shfl((int)(at >> 32), r) << 32); };
 #pragma unroll
         for (int i = 0; i < 32 * KP / 1024; ++i) {
             const int r = i * PER + l / (KP / 16), piece = (l % (KP / 16)) ^ (D == 128 ? r & 15 : (r >> 1) & 7);
@@ -458,96 +470,139 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void prompt_attention_kernel(cons
         if (!late) pa_barrier();                 // (as many as the other half)
     }
 
+    // Results through LDS (each wave in memory of its own, which no wave reads any more), 256 bytes of a row at a time, so that a store writes
+    // whole cache lines.
     const float total = pa_other_sum(l_run);
     const long long row_at = (long long)(q0 + tok) * (p.kv_heads * p.group) + head;
+    const int rows_here = rows - (tile * ROWS + 32 * w);   // of this wave's 32
+    constexpr int OP = D == 128 ? 256 : 128;               // bytes of a row of results
+    const uint32_t o_lds = lds0 + w * (32 * 256);
+    pa_barrier();
     if (splits > 1) {
-        if (row >= rows) return;
         const long long at = row_at * p.splits + split;
-        float *po = p.part_o + at * D;
 #pragma unroll
-        for (int c = 0; c < CT; ++c)
+        for (int part = 0; part < CT / 2; ++part) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const f32x4 x = {o[c][4 * j], o[c][4 * j + 1], o[c][4 * j + 2], o[c][4 * j + 3]};
-                *reinterpret_cast<f32x4 *>(po + 32 * c + 8 * j + 4 * half) = x;
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const f32x16 &x = o[2 * part + c];
+                    const f32x4 v = {x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]};
+                    *(__attribute__((address_space(3))) f32x4 *)(o_lds + n * 256 + 16 * ((8 * c + 2 * j + half) ^ (n & 15))) = v;
+                }
+            asm volatile("" ::: "memory");
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int r = 4 * i + l / 16, piece = l % 16;
+                const f32x4 v = lds_frag<f32x4>(o_lds + r * 256 + 16 * (piece ^ (r & 15)));
+                const long long to = of_row(at, r);
+                if (r < rows_here) *reinterpret_cast<f32x4 *>(p.part_o + to * D + 64 * part + 4 * piece) = v;
             }
-        if (half == 0) {
+            asm volatile("" ::: "memory");
+        }
+        if (half == 0 && n < rows_here) {
             const f32x2 ml = {m_run, total};
             *reinterpret_cast<f32x2 *>(p.part_ml + at * 2) = ml;
         }
-        return;
-    }
-    // Results through LDS (each wave in memory of its own, which no wave reads any more), so that a store writes whole rows.  A row that
-    // sees no key is zeros.
-    const float inv = sees > 0 ? 1.0f / total : 0.f;
-    if (p.lse && half == 0 && row < rows) p.lse[row_at] = sees > 0 ? (m_run + __builtin_amdgcn_logf(total)) * 0.693147180559945f : -INFINITY;
-    static_assert(W * 32 * KP <= STAGES * (K_STAGE + K_BYTES), "the results fit");
-    pa_barrier();
-    const uint32_t o_lds = lds0 + w * (32 * KP);
+    } else {
+        // a row that sees no key is zeros
+        const float inv = sees > 0 ? 1.0f / total : 0.f;
+        if (p.lse && half == 0 && n < rows_here) p.lse[row_at] = sees > 0 ? (m_run + __builtin_amdgcn_logf(total)) * 0.693147180559945f : -INFINITY;
 #pragma unroll
-    for (int c = 0; c < CT; ++c)
+        for (int c = 0; c < CT; ++c)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            // the halves exchange what makes eight neighbouring channels of either
-            uint32_t x[2][2];
+            for (int j = 0; j < 2; ++j) {
+                // the halves exchange what makes eight neighbouring channels of either
+                uint32_t x[2][2];
 #pragma unroll
-            for (int k = 0; k < 2; ++k)
+                for (int k = 0; k < 2; ++k)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) x[k][i] = E::pack(o[c][8 * j + 4 * k + 2 * i] * inv, o[c][8 * j + 4 * k + 2 * i + 1] * inv);
-            const auto r0 = __builtin_amdgcn_permlane32_swap(x[0][0], x[1][0], false, false), r1 = __builtin_amdgcn_permlane32_swap(x[0][1], x[1][1], false, false);
-            const u32x4 v = {r0[0], r1[0], r0[1], r1[1]};
-            *(__attribute__((address_space(3))) u32x4 *)(o_lds + n * KP + 16 * ((4 * c + 2 * j + half) ^ (D == 128 ? n & 15 : (n >> 1) & 7))) = v;
+                    for (int i = 0; i < 2; ++i) x[k][i] = E::pack(o[c][8 * j + 4 * k + 2 * i] * inv, o[c][8 * j + 4 * k + 2 * i + 1] * inv);
+                const auto r0 = __builtin_amdgcn_permlane32_swap(x[0][0], x[1][0], false, false), r1 = __builtin_amdgcn_permlane32_swap(x[0][1], x[1][1], false, false);
+                const u32x4 v = {r0[0], r1[0], r0[1], r1[1]};
+                *(__attribute__((address_space(3))) u32x4 *)(o_lds + n * OP + 16 * ((4 * c + 2 * j + half) ^ (D == 128 ? n & 15 : (n >> 1) & 7))) = v;
+            }
+        asm volatile("" ::: "memory");
+        const long long o_at = (long long)(q0 + tok) * p.o_t + (long long)head * p.o_h;
+#pragma unroll
+        for (int i = 0; i < 32 * OP / 1024; ++i) {
+            const int r = i * PER + l / (OP / 16), piece = l % (OP / 16);
+            const u32x4 v = lds_frag<u32x4>(o_lds + r * OP + 16 * (piece ^ (D == 128 ? r & 15 : (r >> 1) & 7)));
+            const long long to = of_row(o_at, r);
+            if (r < rows_here) *reinterpret_cast<u32x4_a2 *>(p.out + to + 8 * piece) = v;
         }
-    asm volatile("" ::: "memory");
-    const long long o_at = (long long)(q0 + tok) * p.o_t + (long long)head * p.o_h;
-#pragma unroll
-    for (int i = 0; i < 32 * KP / 1024; ++i) {
-        const int r = i * PER + l / (KP / 16), piece = l % (KP / 16);
-        const u32x4 v = lds_frag<u32x4>(o_lds + r * KP + 16 * (piece ^ (D == 128 ? r & 15 : (r >> 1) & 7)));
-        const long long at = (long long)((uint64_t)(uint32_t)__shfl((int)o_at, r) | ((uint64_t)(uint32_t)__shfl((int)(o_at >> 32), r) << 32));
-        if (tile * ROWS + 32 * w + r < rows) *reinterpret_cast<u32x4_a2 *>(p.out + at + 8 * piece) = v;
     }
+    if (slot + (int)(gridDim.x >> 3) < here) {
+        pa_barrier();                                      // (its requests write over the results)
+        c = scan(0);
+    }
+  }
 }
 
-// The pieces of split rows: a wave per row.  out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i.
+// The pieces of split rows: a wave per row.  out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i.  A lane works out the weight of a piece; then
+// eight pieces' outputs are on their way at a time.
 template <typename E, int D>
 __global__ __launch_bounds__(256) void prompt_merge_kernel(const PaParams p)
 {
-    constexpr int PER = D / 64;
+    constexpr int LANES = D / 4, AT_ONCE = 64 / LANES;     // lanes to a piece, four channels each; pieces to a load
     const int l = threadIdx.x & 63;
     const int heads = p.kv_heads * p.group;
     const long long r = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (r >= p.total_q * heads) return;
-    const long long tq = r / heads;
-    const int head = (int)(r - tq * heads);
+    const int tq = (int)(r / heads), head = (int)(r - (long long)tq * heads);
     const int b = sequence_of(p.cu_q, p.B, tq);
     if (b >= p.B) return;
-    const Span sq = span_of(p.cu_q, b, p.total_q), sk = span_of(p.cu_k, b, p.total_k);
+    const Span sq = span_of(p.cu_q, b, (int)p.total_q), sk = span_of(p.cu_k, b, (int)p.total_k);
     if (tq < sq.begin || tq >= sq.begin + sq.len) return;
     const int splits = pa_splits_of((sk.len + PA_KEYS - 1) / PA_KEYS, p.split_tiles, p.splits);
     if (splits <= 1) return;                               // written by the attention kernel
-    const int sees = pa_visible((int)(tq - sq.begin), sq.len, sk.len, p.causal);
+    const int sees = pa_visible(tq - sq.begin, sq.len, sk.len, p.causal);
+    const f32x2 *const ml = reinterpret_cast<const f32x2 *>(p.part_ml) + r * p.splits;
+    f32x2 mine[PA_MAX_SPLITS / 64];
     float top = PA_LOW;
-    for (int i = l; i < splits; i += 64) top = fmaxf(top, p.part_ml[(r * p.splits + i) * 2]);
+#pragma unroll
+    for (int i = 0; i < PA_MAX_SPLITS / 64; ++i) {
+        mine[i] = f32x2{PA_LOW, 0.f};
+        if (64 * i + l < splits) mine[i] = ml[64 * i + l];
+        top = fmaxf(top, mine[i][0]);
+    }
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
-    float acc[PER], total = 0.f;
+    float total = 0.f, weight[PA_MAX_SPLITS / 64];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) acc[i] = 0.f;
-    for (int i = 0; i < splits; ++i) {
-        const float *ml = p.part_ml + (r * p.splits + i) * 2, *po = p.part_o + (r * p.splits + i) * D + PER * l;
-        const float a = __builtin_amdgcn_exp2f(ml[0] - top);
-        total += a * ml[1];
-#pragma unroll
-        for (int j = 0; j < PER; ++j) acc[j] += a * po[j];
+    for (int i = 0; i < PA_MAX_SPLITS / 64; ++i) {
+        weight[i] = __builtin_amdgcn_exp2f(mine[i][0] - top);
+        total += weight[i] * mine[i][1];
     }
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) total += __shfl_xor(total, d);
+
+    const int part = l / LANES, ch = 4 * (l % LANES);
+    const float *po = p.part_o + r * p.splits * D + ch;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int i0 = 0; i0 < splits; i0 += 4 * AT_ONCE) {
+        f32x4 x[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int i = i0 + j * AT_ONCE + part;
+            x[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (i < splits) x[j] = *reinterpret_cast<const f32x4 *>(po + (long long)i * D);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int i = i0 + j * AT_ONCE + part;         // (of the same 64 for all lanes)
+            const float a = __shfl(i0 < 64 ? weight[0] : weight[PA_MAX_SPLITS / 64 - 1], i & 63);
+            if (i < splits) acc += a * x[j];
+        }
+    }
+#pragma unroll
+    for (int d = LANES; d < 64; d *= 2)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[j] += __shfl_xor(acc[j], d);
     const float inv = sees > 0 ? 1.0f / total : 0.f;
-    uint16_t *dst = p.out + tq * p.o_t + head * p.o_h + PER * l;
-    if (PER == 2) {
-        const uint32_t x = E::pack(acc[0] * inv, acc[PER - 1] * inv);
-        dst[0] = (uint16_t)x, dst[1] = (uint16_t)(x >> 16);
-    } else {
-        dst[0] = (uint16_t)E::pack(acc[0] * inv, 0.f);
+    if (part == 0) {
+        uint16_t *dst = p.out + (long long)tq * p.o_t + (long long)head * p.o_h + ch;
+        *reinterpret_cast<u32x2_a2 *>(dst) = u32x2{E::pack(acc[0] * inv, acc[1] * inv), E::pack(acc[2] * inv, acc[3] * inv)};
     }
     if (p.lse && l == 0) p.lse[r] = sees > 0 ? (top + __builtin_amdgcn_logf(total)) * 0.693147180559945f : -INFINITY;
 }
@@ -555,8 +610,7 @@ __global__ __launch_bounds__(256) void prompt_merge_kernel(const PaParams p)
 template <typename E, int D, int R>
 hipError_t launch_of(const PaParams &p, hipStream_t stream)
 {
-    const unsigned grid = (unsigned)((p.items * p.kv_heads + 7) / 8 * 8);
-    hipLaunchKernelGGL((prompt_attention_kernel<E, D, R>), dim3(grid), dim3(64 * PA_WAVES), 0, stream, p);
+    hipLaunchKernelGGL((prompt_attention_kernel<E, D, R>), dim3((unsigned)p.grid), dim3(64 * PA_WAVES), 0, stream, p);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.splits <= 1) return e;
     const long long rows = p.total_q * p.kv_heads * p.group;

@@ -77,6 +77,7 @@ hipError_t cache_read_launch(const CacheReadParams &p, hipStream_t stream);
 constexpr int PA_KEYS = 64;               // keys of a tile
 constexpr int PA_WAVES = 8;               // of a workgroup, 32 rows each
 constexpr int PA_ROWS = 32 * PA_WAVES;
+constexpr int PA_MAX_SPLITS = 128;
 
 struct PaParams {
     const uint16_t *q, *qr, *k, *kr, *v;
@@ -89,7 +90,7 @@ struct PaParams {
     int B, kv_heads, group, d, rope, fp16, causal;
     int q_whole;                          // queries come in whole 16-byte pieces
     int splits, split_tiles;              // most splits of a row tile's keys; tiles from which a further split begins
-    long long items;                      // most (row tile, split) pairs of a key head
+    int grid;                             // workgroups, a multiple of eight
     float scale_log2;
 };
 hipError_t prompt_attention_launch(const PaParams &p, hipStream_t stream);

@@ -394,9 +394,9 @@ PYBIND11_MODULE(_C, m)
                                                           idx_heads, idx_cache_rows, idx_eps, idx_sum_mode);
               check(pto_mla_indexer_prolog_quant_launch(&a, ptr<void>(stream)));
           });
-    m.def("prompt_attention_plan", [](int64_t b, int64_t total_q, int64_t total_k, int64_t heads, int64_t kv_heads, int64_t d, bool rope) {
+    m.def("prompt_attention_plan", [](int64_t b, int64_t total_q, int64_t total_k, int64_t heads, int64_t kv_heads, int64_t d, bool rope, bool causal) {
         PtoPromptAttentionArgs a{};
-        a.b = b, a.total_q = total_q, a.total_k = total_k, a.heads = heads, a.kv_heads = kv_heads, a.d = d, a.softmax_scale = 1.0f;
+        a.b = b, a.total_q = total_q, a.total_k = total_k, a.heads = heads, a.kv_heads = kv_heads, a.d = d, a.softmax_scale = 1.0f, a.causal = causal;
         a.query_rope = a.key_rope = rope ? &a : nullptr;       // (only whether there are any is looked at)
         PtoPromptPlan plan{};
         size_t bytes = 0;
@@ -406,7 +406,7 @@ PYBIND11_MODULE(_C, m)
         r["rows_per_workgroup"] = plan.rows_per_workgroup;
         r["key_splits"] = plan.key_splits;
         r["split_keys"] = plan.split_keys;
-        r["items"] = plan.items;
+        r["workgroups"] = plan.workgroups;
         r["workspace_bytes"] = bytes;
         return r;
     });

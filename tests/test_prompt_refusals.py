@@ -187,7 +187,8 @@ def items_of(lens_q, lens_k, group, plan):
 
 @pytest.mark.parametrize("heads,kv", [(1, 1), (16, 16), (64, 8), (128, 128), (56, 8), (128, 1)])
 def test_plans_hold_every_division_of_the_rows_over_sequences(heads, kv):
-    """However the rows and keys are dealt out to the sequences, the launch has a workgroup for every piece."""
+    """However the rows and keys are dealt out to the sequences: a launch that divides no keys has a workgroup for every row tile, one that
+    does has no more pieces than its workspace holds, and workgroups for all or for four rounds."""
     g = torch.Generator().manual_seed(heads)
     rnd = lambda lo, hi: int(torch.randint(lo, hi + 1, (1,), generator=g))  # noqa: E731
     for _ in range(300):
@@ -198,16 +199,17 @@ def test_plans_hold_every_division_of_the_rows_over_sequences(heads, kv):
             lens_k[rnd(0, b - 1)] = 100000
         if rnd(0, 3) == 0:
             lens_q[rnd(0, b - 1)] = 3000
-        plan = _C.prompt_attention_plan(b, sum(lens_q), sum(lens_k), heads, kv, 128, True)
-        assert items_of(lens_q, lens_k, heads // kv, plan) <= plan["items"], (lens_q, lens_k, plan)
-        assert plan["key_splits"] >= 1 and plan["split_keys"] % 64 == 0
+        plan = _C.prompt_attention_plan(b, sum(lens_q), sum(lens_k), heads, kv, 128, True, rnd(0, 1) == 1)
+        items = items_of(lens_q, lens_k, heads // kv, plan) * kv
+        assert plan["workgroups"] % 8 == 0 and plan["workgroups"] >= (items if plan["key_splits"] == 1 else min(items, 1024)), (lens_q, lens_k, plan)
+        assert 1 <= plan["key_splits"] <= 128 and plan["split_keys"] % 64 == 0
         need = sum(lens_q) * heads * plan["key_splits"] * (128 + 2) * 4 if plan["key_splits"] > 1 else 0
-        assert plan["workspace_bytes"] == need <= 1 << 30, plan
+        assert plan["workspace_bytes"] == need <= 260 << 20, plan
 
 
 def test_large_calls_are_not_divided_and_small_ones_are():
-    assert _C.prompt_attention_plan(1, 4096, 4096, 128, 128, 128, True)["key_splits"] == 1
-    assert _C.prompt_attention_plan(1, 1, 65536, 16, 1, 128, False)["key_splits"] > 16
+    assert _C.prompt_attention_plan(1, 4096, 4096, 128, 128, 128, True, True)["key_splits"] == 1
+    assert _C.prompt_attention_plan(1, 1, 65536, 16, 1, 128, False, True)["key_splits"] > 16
 
 
 # ---------------------------------------------------------------- the C entries
