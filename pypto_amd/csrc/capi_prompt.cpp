@@ -106,12 +106,14 @@ struct PromptPlan {
 
 // Dividing a call's keys.  The host knows how many rows, keys and sequences there are, not which sequence has how many, and takes them for
 // dealt out evenly.  In microseconds: a workgroup starts and ends in `fixed`, takes `tile` for 64 keys, and partial results are written
-// and read back by a launch of their own, a tenth of a microsecond to a piece.  With s pieces to the longest row tile a launch takes the longest workgroup and then, for the rounds
-// of the chip behind the first, the mean one.  Cheapest s first; what is fixed is the length of a piece, so a sequence longer than the mean
-// is divided into more.  Where the cheapest is one piece and the workgroups are few and long, sequences a quarter longer than the mean are
-// divided all the same, and where they are very long all are, in pieces of half of the mean: one that is much longer would be there alone at the
-// end (32 sequences of 700 to 12000 keys, 8 key heads: 200 us, now 187).  A launch has a workgroup for each row tile, or piece of one, that there can be, and the device starts the next as one
-// ends; where that could be more than four for each compute unit, the workgroups of a divided launch take the pieces there are in turn.
+// and read back by a launch of their own, `merge` and a tenth of a microsecond to a piece.  With s pieces to the longest row tile a launch
+// takes the longest workgroup and then, for the rounds of the chip behind the first, the mean one; the cheapest s is taken if it saves a
+// tenth (2 tokens over 6180 keys, 4 heads: 115 us in one piece, now 17; 294 over 4732, 8 heads: 92, now 28).  What is fixed is the
+// length of a piece, so a sequence longer than the mean is divided into more.  Where the cheapest is one piece and the workgroups are few
+// and very long, all sequences are divided, in pieces of half of the mean: one that is much longer would be there alone at the end (32
+// sequences of 700 to 12000 keys, 8 key heads: 200 us, now 187).
+// A launch has a workgroup for each row tile, or piece of one, that there can be, and the device starts the next as one ends; where that
+// could be more than four for each compute unit, the workgroups of a divided launch take the pieces there are in turn.
 constexpr size_t PA_MOST_PARTIALS = (size_t)256 << 20;
 
 PromptPlan attention_plan(const PtoPromptAttentionArgs *a)
@@ -132,18 +134,20 @@ PromptPlan attention_plan(const PtoPromptAttentionArgs *a)
     if (items < 2.0 * cus && longest > 1.0) {
         const double fixed = 9.0, tile = a->d == 64 ? 1.1 : (a->query_rope ? 2.05 : 1.65);
         const double partial = (double)a->total_q * a->heads * (a->d + 2) * sizeof(float);
+        const double merge = 4.0 + 3.0 * (double)a->total_q * a->heads / (32.0 * cus);
         auto pieces_of = [&](const long long len) { return (key_tiles + len - 1) / len; };
         auto cost = [&](const double s) {
             const double len = std::ceil(longest / s), rounds = std::ceil(std::ceil(items) * s / cus);
-            return fixed + tile * len + (rounds - 1.0) * (fixed + tile * mean / s) + (s > 1.0 ? 3.5 + s * (0.1 + partial * 0.5e-6) : 0.0);
+            return fixed + tile * len + (rounds - 1.0) * (fixed + tile * mean / s) + (s > 1.0 ? merge + s * (0.1 + partial * 0.5e-6) : 0.0);
         };
         double best = cost(1.0), s_best = 1.0;
         for (double s = 2.0; s <= longest && s <= pto::PA_MAX_SPLITS; s += 1.0)
             if (cost(s) < best) best = cost(s), s_best = s;
+        if (best > 0.9 * cost(1.0)) s_best = 1.0;
         long long len = (long long)std::ceil(longest / s_best);
         if (s_best == 1.0) {
             const bool uneven = a->b > 1 && items <= 1.5 * cus;
-            len = uneven && tile * longest >= 8.0 * fixed ? (len + 1) / 2 : uneven && tile * longest >= 3.0 * fixed ? len + len / 4 + 1 : key_tiles;
+            len = uneven && tile * longest >= 8.0 * fixed ? (len + 1) / 2 : key_tiles;
         }
         while (pieces_of(len) > pto::PA_MAX_SPLITS || (len < key_tiles && partial * (double)pieces_of(len) > (double)PA_MOST_PARTIALS)) len += (len + 3) / 4;
         if (pieces_of(len) > 1) {
@@ -215,11 +219,7 @@ int pto_rotary_launch(const PtoRotaryArgs *a, void *hip_stream)
     p.dtype = a->dtype;
     p.layout = a->layout;
     p.factor = (float)a->factor;
-    // A workgroup takes as many tokens as leave four workgroups to a compute unit, up to four.
-    const long long pass = 256 / (a->pairs <= 8 ? 1 : a->pairs <= 16 ? 2 : a->pairs <= 32 ? 4 : a->pairs <= 64 ? 8 : 16);
-    const long long parts = (a->query.heads + pass - 1) / pass + (a->key.in ? (a->key.heads + pass - 1) / pass : 0);
-    const long long tokens = a->t * parts / (4ll * cu_count());
-    p.tokens_per_wg = (int)(tokens < 1 ? 1 : (tokens > pto::ROT_MAX_TOKENS ? pto::ROT_MAX_TOKENS : tokens));
+    p.cus = cu_count();
     const hipError_t e = pto::rotary_launch(p, static_cast<hipStream_t>(hip_stream));
     if (e != hipSuccess) return fail(PTO_E_LAUNCH, "rotary: launch failed: %s", hipGetErrorString(e));
     return PTO_OK;
@@ -277,8 +277,6 @@ int pto_cache_read_launch(const PtoCacheReadArgs *a, void *hip_stream)
     p.B = (int)a->b;
     p.maxblk = (int)a->max_blocknum_perbatch;
     p.bs = (int)a->block_size;
-    // Four batches of rows to a wave where that leaves a wave to every SIMD: the next one's rows are then asked for before one is stored.
-    p.batches = a->rows >= 32ll * 4 * cu_count() ? 4 : 1;
     const hipError_t e = pto::cache_read_launch(p, static_cast<hipStream_t>(hip_stream));
     if (e != hipSuccess) return fail(PTO_E_LAUNCH, "cache_read: launch failed: %s", hipGetErrorString(e));
     return PTO_OK;
@@ -328,7 +326,7 @@ int pto_prompt_attention_launch(const PtoPromptAttentionArgs *a, void *hip_strea
     if (need > 0 && (!a->workspace || a->workspace_bytes < need))
         return fail(PTO_E_WORKSPACE, "prompt_attention: workspace of %zu bytes required, %zu given", need, a->workspace ? a->workspace_bytes : (size_t)0);
     if (!aligned(a->workspace, 16)) return fail(PTO_E_INVALID_ARG, "prompt_attention: the workspace must be 16-byte aligned");
-    if (pl.workgroups > 0x7ffffff0ll || a->total_q * a->heads / 4 > 0x7ffffff0ll)
+    if (pl.workgroups > 0x7ffffff0ll)
         return fail(PTO_E_INVALID_ARG, "prompt_attention: the call exceeds the largest launch");
 
     pto::PaParams p{};
@@ -362,6 +360,7 @@ int pto_prompt_attention_launch(const PtoPromptAttentionArgs *a, void *hip_strea
     p.splits = pl.splits;
     p.split_tiles = pl.split_tiles;
     p.grid = (int)pl.workgroups;
+    p.cus = cu_count();
     p.scale_log2 = a->softmax_scale * 1.4426950408889634f;
     const hipError_t e = pto::prompt_attention_launch(p, static_cast<hipStream_t>(hip_stream));
     if (e != hipSuccess) return fail(PTO_E_LAUNCH, "prompt_attention: launch failed: %s", hipGetErrorString(e));

@@ -9,7 +9,6 @@ namespace pto {
 // ---- rotary positions (rotary_kernels.hip)
 
 constexpr int ROT_MAX_PAIRS = 128;
-constexpr int ROT_MAX_TOKENS = 4;         // of a workgroup
 
 struct RotaryTablesParams {
     const void *positions;    // [T] int64 or int32
@@ -27,6 +26,7 @@ struct RotarySide {           // the queries or the keys: [T, heads, dim]
     int heads, dim, offset;   // channels offset .. offset + 2 * pairs - 1 turn, the others are copied (in place: left alone)
     int copies;               // out is not in, and there are other channels
     long long in_t, in_h, out_t, out_h;   // strides in elements
+    int parts;                // workgroups that share a token's heads (set by rotary_launch)
 };
 struct RotaryParams {
     RotarySide side[2];       // queries, keys (heads 0: none)
@@ -35,8 +35,8 @@ struct RotaryParams {
     long long T;
     int pairs, wide, dtype, layout;
     float factor;
-    int tokens_per_wg;
-    int query_parts, key_parts;           // workgroups that share a token's heads (set by rotary_launch)
+    int cus;                              // compute units
+    int tokens;                           // of a workgroup (set by rotary_launch)
 };
 hipError_t rotary_launch(const RotaryParams &p, hipStream_t stream);
 
@@ -68,7 +68,6 @@ struct CacheReadParams {
     long long latent_t, rope_t;           // strides in elements
     long long rows;                       // of the outputs
     int B, maxblk, bs;
-    int batches;                          // of eight rows to a wave: 1 or 4
 };
 hipError_t cache_read_launch(const CacheReadParams &p, hipStream_t stream);
 
@@ -91,6 +90,7 @@ struct PaParams {
     int q_whole;                          // queries come in whole 16-byte pieces
     int splits, split_tiles;              // most splits of a row tile's keys; tiles from which a further split begins
     int grid;                             // workgroups, a multiple of eight
+    int cus;                              // compute units
     float scale_log2;
 };
 hipError_t prompt_attention_launch(const PaParams &p, hipStream_t stream);

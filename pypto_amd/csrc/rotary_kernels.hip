@@ -69,7 +69,7 @@ struct Eight {
             }
         }
     }
-    // (to be thrown out of the caches first: 34 us, where ordinary stores push the rows still to be read out, 37)
+    // (to be thrown out of the caches first: ordinary stores push out the rows that are still to be read, 28 us to 31)
     __device__ __forceinline__ void store(void *base, const long long at) const
     {
         if (DT == PTO_DT_FP32) {
@@ -133,43 +133,40 @@ __global__ __launch_bounds__(256) void rotary_tables_kernel(const RotaryTablesPa
     }
 }
 
-// A workgroup makes the turns of up to four tokens once, in LDS, and takes them through its heads.  A row (a token's head) is a group of LPR
-// lanes of one wave, eight pairs to a lane; a group takes a head through all of the tokens at once, and every lane's loads precede its
-// group's stores: so a row may be turned where it lies whatever its layout.
-// Bound by memory: 64 of 192 channels of 4096 tokens of 128 heads, bf16, 135 MB in 30 us = 4.5 TB/s, where a plain copy of as much takes 27;
-// one row of a group at a time 43 us, results stored as if they were wanted soon 34.
+// A row (a token's head) is a group of LPR lanes of one wave, eight pairs to a lane, and a workgroup's 256 / LPR groups are heads of one token
+// or, where a token has fewer, tokens side by side.  Their turns are made once, in LDS, while the rows are on their way; every lane's
+// loads precede its group's stores, so a row may be turned where it lies whatever its layout.
+// Bound by memory: 64 of 192 channels of 4096 tokens of 128 heads and a shared key, bf16, 135 MB in 27.1 us = 5.0 TB/s, what a plain copy
+// reaches.  Four tokens of a head to a lane, one after the other, 28.7 us; results stored as if they were wanted soon 3 us more; the keys'
+// workgroups in front of all of the queries' 31.4.  One head of a token after the other, 16384 tokens of 8 heads: 15.2 us, side by side 6.5.
 template <int DT, int LPR>
 __global__ __launch_bounds__(256) void rotary_kernel(const RotaryParams p)
 {
-    __shared__ Turn turns[ROT_MAX_TOKENS * ROT_MAX_PAIRS];
+    constexpr int ROWS = 256 / LPR;
+    __shared__ Turn turns[ROWS * 8 * LPR];
     const int tid = threadIdx.x;
-    const int parts = p.query_parts + p.key_parts, part = (int)(blockIdx.x % (unsigned)parts);    // (a token's heads side by side)
-    const long long t0 = (long long)(blockIdx.x / (unsigned)parts) * p.tokens_per_wg;
-    const int tokens = p.T - t0 < p.tokens_per_wg ? (int)(p.T - t0) : p.tokens_per_wg;
+    const int parts = p.side[0].parts + p.side[1].parts, at = (int)(blockIdx.x % (unsigned)parts);    // (a token's heads side by side)
+    const bool key = at >= p.side[0].parts;
+    const RotarySide &s = p.side[key ? 1 : 0];
+    const int part = at - (key ? p.side[0].parts : 0);
+    const long long t0 = (long long)(blockIdx.x / (unsigned)parts) * p.tokens;
+    const int tokens = p.T - t0 < p.tokens ? (int)(p.T - t0) : p.tokens;
 
-    const int lane = tid & (LPR - 1);
-    const bool mine = 8 * lane < p.pairs;                  // (of a group some lanes may have no pairs)
-    const int pair = mine ? 8 * lane : 0;
+    const int lane = tid & (LPR - 1), group = tid / LPR;   // (a key of one head beside many heads leaves most groups idle)
+    const int mine_t = p.tokens > 1 ? group / s.heads : 0, h = part * ROWS + group - mine_t * s.heads;
+    const bool there = mine_t < tokens && h < s.heads;
+    const bool mine = there && 8 * lane < p.pairs;         // (of a group some lanes may have no pairs)
+    const int pair = 8 * lane;
     const bool half = p.layout == PTO_ROPE_HALF;
     const int first = half ? pair : 2 * pair, second = half ? pair + p.pairs : 2 * pair + 8;
     const bool halves = p.layout != PTO_ROPE_INTERLEAVED;  // of what is stored
     const int first_out = halves ? pair : 2 * pair, second_out = halves ? pair + p.pairs : 2 * pair + 8;
-    // this workgroup's heads: of the queries, or behind them of the keys
-    const bool key = part >= p.query_parts;
-    const RotarySide &s = p.side[key ? 1 : 0];
-    const int h = (part - (key ? p.query_parts : 0)) * (256 / LPR) + tid / LPR;
-    const bool there = h < s.heads;
-    const long long from = t0 * s.in_t + (there ? h : 0) * s.in_h, to = t0 * s.out_t + (there ? h : 0) * s.out_h;
+    const long long from = (t0 + mine_t) * s.in_t + h * s.in_h, to = (t0 + mine_t) * s.out_t + h * s.out_h;
 
-    Raw<DT> ra[ROT_MAX_TOKENS], rb[ROT_MAX_TOKENS];
-    if (mine && there) {
-#pragma unroll
-        for (int j = 0; j < ROT_MAX_TOKENS; ++j)
-            if (j < tokens) {
-                const long long at = from + j * s.in_t + s.offset;
-                ra[j].load(s.in, at + first);
-                rb[j].load(s.in, at + second);
-            }
+    Raw<DT> ra, rb;
+    if (mine) {
+        ra.load(s.in, from + s.offset + first);
+        rb.load(s.in, from + s.offset + second);
     }
     for (int i = tid; i < tokens * p.pairs; i += 256) {    // (the rows are on their way)
         const int t = i / p.pairs;
@@ -179,47 +176,45 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryParams p)
     if (!there) return;
     if (s.copies) {                                        // the channels around the part that turns
         const int rest = s.dim - 2 * p.pairs;
-        for (int j = 0; j < tokens; ++j)
-            for (int c = lane; c < rest; c += LPR) {
-                const int ch = c < s.offset ? c : c + 2 * p.pairs;
-                copy_one<DT>(s.in, from + j * s.in_t + ch, s.out, to + j * s.out_t + ch);
-            }
+        for (int c = lane; c < rest; c += LPR) {
+            const int ch = c < s.offset ? c : c + 2 * p.pairs;
+            copy_one<DT>(s.in, from + ch, s.out, to + ch);
+        }
     }
+    if (!mine) return;
+    Eight<DT> x(ra), y(rb), c, d;
+    if (half) {
+        c = x, d = y;
+    } else {                                               // first and second members of the eight pairs
 #pragma unroll
-    for (int j = 0; j < ROT_MAX_TOKENS; ++j) {
-        if (!mine || j >= tokens) continue;
-        Eight<DT> x(ra[j]), y(rb[j]), c, d;
-        if (half) {
-            c = x, d = y;
-        } else {                                           // first and second members of the eight pairs
-#pragma unroll
-            for (int i = 0; i < 4; ++i) c.v[i] = x.v[2 * i], c.v[4 + i] = y.v[2 * i], d.v[i] = x.v[2 * i + 1], d.v[4 + i] = y.v[2 * i + 1];
-        }
-        const Turn *w = turns + j * p.pairs + pair;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float u = c.v[i], v = d.v[i], co = w[i].c, si = w[i].s;
-            c.v[i] = u * co - v * si;
-            d.v[i] = v * co + u * si;
-        }
-        if (!halves) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x.v[2 * i] = c.v[i], x.v[2 * i + 1] = d.v[i], y.v[2 * i] = c.v[4 + i], y.v[2 * i + 1] = d.v[4 + i];
-            c = x, d = y;
-        }
-        const long long at = to + j * s.out_t + s.offset;
-        c.store(s.out, at + first_out);
-        d.store(s.out, at + second_out);
+        for (int i = 0; i < 4; ++i) c.v[i] = x.v[2 * i], c.v[4 + i] = y.v[2 * i], d.v[i] = x.v[2 * i + 1], d.v[4 + i] = y.v[2 * i + 1];
     }
+    const Turn *w = turns + mine_t * p.pairs + pair;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float u = c.v[i], v = d.v[i], co = w[i].c, si = w[i].s;
+        c.v[i] = u * co - v * si;
+        d.v[i] = v * co + u * si;
+    }
+    if (!halves) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x.v[2 * i] = c.v[i], x.v[2 * i + 1] = d.v[i], y.v[2 * i] = c.v[4 + i], y.v[2 * i + 1] = d.v[4 + i];
+        c = x, d = y;
+    }
+    c.store(s.out, to + s.offset + first_out);
+    d.store(s.out, to + s.offset + second_out);
 }
 
 template <int DT, int LPR>
 hipError_t rotary_with(RotaryParams p, hipStream_t stream)
 {
     constexpr int rows = 256 / LPR;
-    p.query_parts = (p.side[0].heads + rows - 1) / rows;
-    p.key_parts = (p.side[1].heads + rows - 1) / rows;
-    const long long grid = (p.T + p.tokens_per_wg - 1) / p.tokens_per_wg * (p.query_parts + p.key_parts);
+    for (RotarySide &s : p.side) s.parts = (s.heads + rows - 1) / rows;
+    // tokens side by side where a workgroup has room for them, as many as leave a workgroup to every compute unit
+    const int most = p.side[0].heads > p.side[1].heads ? p.side[0].heads : p.side[1].heads;
+    const long long room = rows / most, wide = p.T / p.cus, tokens = room < wide ? room : wide;
+    p.tokens = tokens > 1 ? (int)tokens : 1;
+    const long long grid = (p.T + p.tokens - 1) / p.tokens * (p.side[0].parts + p.side[1].parts);
     if (grid > 0x7fffffffll) return hipErrorInvalidConfiguration;
     hipLaunchKernelGGL((rotary_kernel<DT, LPR>), dim3((unsigned)grid), dim3(256), 0, stream, p);
     return hipGetLastError();

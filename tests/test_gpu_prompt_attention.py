@@ -83,6 +83,16 @@ def test_many_heads_and_sequences(d, rope):
     Call([200], [200], 128, 128, d, rope, seed=5).run().check()
 
 
+@pytest.mark.parametrize("d,rope", FORMS)
+@pytest.mark.parametrize("lens_q,lens_k", [([600, 0, 500], [6000, 0, 300]), ([1, 700, 400], [1, 200, 7000])])
+def test_more_divided_rows_than_waves_among_rows_that_are_not(d, rope, lens_q, lens_k):
+    """More rows than the launch that joins the pieces has waves, so a wave has several, of sequences that are divided and of others."""
+    from pypto_amd import _C
+    plan = _C.prompt_attention_plan(len(lens_q), sum(lens_q), sum(lens_k), 16, 1, d, rope, True)
+    assert plan["key_splits"] > 1 and plan["split_keys"] >= 300
+    Call(lens_q, lens_k, 16, 1, d, rope, seed=20).run().check()
+
+
 def test_a_key_head_s_own_rope_part_and_its_one_head_form():
     Call([70, 130], [90, 130], 8, 4, 128, True, seed=6, shared=False).run().check()
     a = Call([70, 130], [90, 130], 8, 4, 128, True, seed=6).run()
