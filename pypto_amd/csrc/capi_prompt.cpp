@@ -99,11 +99,18 @@ int attention_check(const PtoPromptAttentionArgs *a)
 }
 
 struct PromptPlan {
-    int splits, split_tiles;
+    int splits, split_tiles, waves;
     long long workgroups;
     size_t o_bytes, ml_bytes;
 };
 
+// Eight waves to a workgroup or four.  Four leave room for a second workgroup on the compute unit, whose work stands in for one's waits at its
+// beginning and end, and waste less on a short sequence; eight read a tile of keys half as often.  With rope parts two workgroups of four do not
+// fit.  64 channels: four are never slower (3760 causal tokens, 128/16 heads, 321 us with eight, 301 with four; 11 sequences of 72 to 243 tokens
+// over 2100 keys, 128/32 heads, 214 and 185; 11 of 1 to 2 over 600, 128 heads, 83 and 51).  128 channels: four for fewer than 512 rows
+// to a sequence and key head (6 sequences of 66 to 445 tokens over 1000 keys, 32 heads, 53 and 41; 8 of 5 to 11, 16/8 heads, 30 and 22), for
+// more eight (9 prompts of 65 to 1871 tokens, 64/8 heads, 166 and 176; 2 of 1841 and 2988, 32/8 heads, 108 and 114).
+//
 // Dividing a call's keys.  The host knows how many rows, keys and sequences there are, not which sequence has how many, and takes them for
 // dealt out evenly.  In microseconds: a workgroup starts and ends in `fixed`, takes `tile` for 64 keys, and partial results are written
 // and read back by a launch of their own, `merge` and a tenth of a microsecond to a piece.  With s pieces to the longest row tile a launch
@@ -121,23 +128,26 @@ PromptPlan attention_plan(const PtoPromptAttentionArgs *a)
     PromptPlan pl{};
     const long long cus = cu_count() > 0 ? cu_count() : 256;
     const long long rows = a->total_q * (a->heads / a->kv_heads);
-    const long long most_tiles = rows / pto::PA_ROWS + a->b;                                // of a key head
     const long long key_tiles = (a->total_k + pto::PA_KEYS - 1) / pto::PA_KEYS;             // of one sequence, at most
     pl.splits = 1;
+    pl.waves = a->query_rope ? 8 : (a->d == 64 || rows < 512 * a->b ? 4 : 8);
+    const int wg_rows = pl.waves * pto::PA_WAVE_ROWS;
+    const long long slots = pl.waves == 4 ? 2 * cus : cus;                                  // workgroups at a time
+    const long long most_tiles = rows / wg_rows + a->b;                                     // of a key head
     pl.split_tiles = 1 << 24;
     pl.workgroups = most_tiles * a->kv_heads;
 
     const double seq_rows = (double)rows / a->b;
-    const double items = (seq_rows <= pto::PA_ROWS ? (double)a->b : (double)rows / pto::PA_ROWS + (a->b > 1 ? 0.5 * a->b : 0.0)) * a->kv_heads;
+    const double items = (seq_rows <= wg_rows ? (double)a->b : (double)rows / wg_rows + (a->b > 1 ? 0.5 * a->b : 0.0)) * a->kv_heads;
     const double longest = std::ceil((double)a->total_k / a->b / pto::PA_KEYS);
     const double mean = a->causal && a->total_k >= a->total_q ? ((double)a->total_k - 0.5 * a->total_q) / a->b / pto::PA_KEYS : longest;
-    if (items < 2.0 * cus && longest > 1.0) {
+    if (items < 2.0 * slots && longest > 1.0) {
         const double fixed = 9.0, tile = a->d == 64 ? 1.1 : (a->query_rope ? 2.05 : 1.65);
         const double partial = (double)a->total_q * a->heads * (a->d + 2) * sizeof(float);
         const double merge = 4.0 + 3.0 * (double)a->total_q * a->heads / (32.0 * cus);
         auto pieces_of = [&](const long long len) { return (key_tiles + len - 1) / len; };
         auto cost = [&](const double s) {
-            const double len = std::ceil(longest / s), rounds = std::ceil(std::ceil(items) * s / cus);
+            const double len = std::ceil(longest / s), rounds = std::ceil(std::ceil(items) * s / slots);
             return fixed + tile * len + (rounds - 1.0) * (fixed + tile * mean / s) + (s > 1.0 ? merge + s * (0.1 + partial * 0.5e-6) : 0.0);
         };
         double best = cost(1.0), s_best = 1.0;
@@ -146,16 +156,16 @@ PromptPlan attention_plan(const PtoPromptAttentionArgs *a)
         if (best > 0.9 * cost(1.0)) s_best = 1.0;
         long long len = (long long)std::ceil(longest / s_best);
         if (s_best == 1.0) {
-            const bool uneven = a->b > 1 && items <= 1.5 * cus;
+            const bool uneven = a->b > 1 && items <= 1.5 * slots;
             len = uneven && tile * longest >= 8.0 * fixed ? (len + 1) / 2 : key_tiles;
         }
         while (pieces_of(len) > pto::PA_MAX_SPLITS || (len < key_tiles && partial * (double)pieces_of(len) > (double)PA_MOST_PARTIALS)) len += (len + 3) / 4;
         if (pieces_of(len) > 1) {
             pl.splits = (int)pieces_of(len);
             pl.split_tiles = (int)len;
-            const long long by_tiles = most_tiles * pl.splits, by_keys = ((rows + pto::PA_ROWS - 1) / pto::PA_ROWS) * (key_tiles / len + a->b + 1);
+            const long long by_tiles = most_tiles * pl.splits, by_keys = ((rows + wg_rows - 1) / wg_rows) * (key_tiles / len + a->b + 1);
             pl.workgroups = (by_tiles < by_keys ? by_tiles : by_keys) * a->kv_heads;
-            if (pl.workgroups > 4 * cus) pl.workgroups = 4 * cus;
+            if (pl.workgroups > 4 * slots) pl.workgroups = 4 * slots;
         }
     }
     pl.workgroups = (pl.workgroups + 7) / 8 * 8;
@@ -298,7 +308,7 @@ int pto_prompt_attention_plan(const PtoPromptAttentionArgs *a, PtoPromptPlan *pl
     const int rc = attention_check(a);
     if (rc != PTO_OK) return rc;
     const PromptPlan pl = attention_plan(a);
-    plan->rows_per_workgroup = pto::PA_ROWS;
+    plan->rows_per_workgroup = pl.waves * pto::PA_WAVE_ROWS;
     plan->key_splits = pl.splits;
     plan->split_keys = (int64_t)pl.split_tiles * pto::PA_KEYS;
     plan->workgroups = pl.workgroups;
@@ -359,6 +369,7 @@ int pto_prompt_attention_launch(const PtoPromptAttentionArgs *a, void *hip_strea
                 a->query_rope_stride_t % 8 == 0 && a->query_rope_stride_h % 8 == 0;
     p.splits = pl.splits;
     p.split_tiles = pl.split_tiles;
+    p.waves = pl.waves;
     p.grid = (int)pl.workgroups;
     p.cus = cu_count();
     p.scale_log2 = a->softmax_scale * 1.4426950408889634f;

@@ -18,8 +18,8 @@
 // product of 8192^3 reaches 1330.  Of what is above it 6 % are the halves of tiles that the mask cuts off, 10 % workgroups' beginnings and
 // ends, the rest the waits of phases for the longer half.  On the way: one phase, every wave products and softmax in turn 732 us; two
 // phases, two stages of tiles, requests among the products 675; three stages, requests before the softmax 670 at fewer clocks; queries and
-// results by whole cache lines 637.  Not kept: four waves and two workgroups to a compute unit (1 % slower), and workgroups that stay and
-// draw their work from counters (1 % slower here, 3 % faster for nine ragged sequences, 7 % slower where keys are divided).
+// results by whole cache lines 637.  Not kept: workgroups that stay and draw their work from counters (1 % slower here, 3 % faster for nine
+// ragged sequences, 7 % slower where keys are divided).
 #include <cmath>
 #include <type_traits>
 
@@ -117,23 +117,24 @@ __device__ __forceinline__ int pa_visible(const int t, const int lq, const int l
 // whole cache line.
 constexpr int PA_BLOCK = 1040;
 
-template <typename E, int D, int R>
-__global__ __launch_bounds__(64 * PA_WAVES, 2) void prompt_attention_kernel(const PaParams p)
+template <typename E, int D, int R, int W>
+__global__ __launch_bounds__(64 * W, 2) void prompt_attention_kernel(const PaParams p)
 {
-    constexpr int W = PA_WAVES, ROWS = PA_ROWS;
+    constexpr int ROWS = 32 * W;
+    constexpr bool PHASED = W == 8;                        // two waves of a SIMD in this workgroup; otherwise of two workgroups
     constexpr int KP = D * 2;                              // bytes of a key row, and of a value row
     constexpr int REQ = D == 128 ? PA_BLOCK : 1024;        // bytes from one request's rows to the next one's
     constexpr int K_REQS = PA_KEYS * KP / 1024, R_REQS = PA_KEYS * R * 2 / 1024;
     constexpr int K_BYTES = K_REQS * REQ, R_BYTES = R_REQS * 1024;
     constexpr int K_STAGE = K_BYTES + R_BYTES;             // [keys | rope keys] of a tile
-    constexpr int STAGES = 3, AHEAD = 5;
+    constexpr int STAGES = PHASED ? 3 : 2, AHEAD = 5;
     constexpr int POOL = STAGES * (K_STAGE + K_BYTES) > W * 32 * 256 ? STAGES * (K_STAGE + K_BYTES) : W * 32 * 256;   // (results: 256 bytes to a row)
     constexpr int KS = D / 16, RS = R / 16, CT = D / 32;
     constexpr int NK = K_REQS / W, NR = R_REQS / W;   // requests of a wave per tile: keys (as many values), rope keys
     static_assert(K_REQS % W == 0 && R_REQS % W == 0, "whole requests for every wave");
     typedef typename E::frag frag;
 
-    __shared__ __attribute__((aligned(1024))) uint8_t pool[POOL];   // keys of three tiles, then their values
+    __shared__ __attribute__((aligned(1024))) uint8_t pool[POOL];   // keys of the stages' tiles, then their values
 
     const int tid = threadIdx.x;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -407,28 +408,30 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void prompt_attention_kernel(cons
             l_run += sum[0] + sum[1];
         };
 
-        // Two waves share a SIMD, and while one multiplies the other does the softmax of its tile: the second half of the waves is one phase
+        // Two waves share a SIMD, and while one multiplies the other does the softmax of its tile.  Four waves to a workgroup: the other is of
+        // another workgroup, and they find their turns themselves; a barrier ends a tile's products, behind it nobody reads the keys of tile t or
+        // the values of tile t - 1, and those of tiles t + 2 and t + 1 are asked for.  Eight waves: the second half is one phase
         // behind, and a barrier ends every phase.  First half: phase 2t products of tile t (and t - 1), phase 2t + 1 its softmax.  A wave asks
         // for its part of the keys of tile t + 2 and the values of tile t + 1 where it has time, at the beginning of its softmax of tile t (in
         // phase 2t + 1 or 2t + 2: the last readers of those buffers, of the keys of tile t - 1 and the values of tile t - 2, were done with
         // phase 2t - 1), and waits for them at the end of its products of tile t + 1 (phase 2t + 2 or 2t + 3; the first reader's phase is
         // 2t + 4).  Asked for among the products they held up the first half's by 550 of 2050 clocks.
-        const bool late = w >= W / 2;
+        const bool late = PHASED && w >= W / 2;
         const std::integral_constant<bool, true> yes;
         const std::integral_constant<bool, false> no;
         if (t_begin < t_end) {
-            int s0 = 0, s1 = 1, s2 = 2;                        // stages of tiles t, t + 1 and t + 2 (or t - 1)
+            int s0 = 0, s1 = 1, s2 = PHASED ? 2 : 1;           // stages of tiles t, t + 1 and t - 1
             auto end_products = [&]() __attribute__((always_inline)) {
                 __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
                 pa_barrier();
             };
             auto request_next = [&]() __attribute__((always_inline)) {
-                if (k_tile < t_end) request_keys(s2);
+                if (k_tile < t_end) request_keys(PHASED ? s2 : s0);
                 if (v_tile < t_end) request_values(s1);
             };
             auto turn = [&]() __attribute__((always_inline)) {
                 const int s = s0;
-                s0 = s1, s1 = s2, s2 = s;
+                s0 = s1, s1 = PHASED ? s2 : s, s2 = s;
             };
             // tiles that this wave's rows see end here; in later ones it asks for its part of the tile and keeps step
             int own_end = (wave_most + PA_KEYS - 1) / PA_KEYS;
@@ -456,7 +459,7 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void prompt_attention_kernel(cons
                 end_products();
                 request_next();
                 softmax(t);
-                pa_barrier();
+                if (PHASED) pa_barrier();
                 turn();
                 for (++t; t < own_end; ++t) {
                     __builtin_amdgcn_s_setprio(1);
@@ -465,7 +468,7 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void prompt_attention_kernel(cons
                     end_products();
                     request_next();
                     softmax(t);
-                    pa_barrier();
+                    if (PHASED) pa_barrier();
                     turn();
                 }
                 products(no, yes, s0, s2);
@@ -473,10 +476,10 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void prompt_attention_kernel(cons
             for (; t < t_end; ++t) {
                 end_products();
                 request_next();
-                pa_barrier();
+                if (PHASED) pa_barrier();
                 turn();
             }
-            if (!late) pa_barrier();                 // (as many as the other half)
+            if (PHASED && !late) pa_barrier();                 // (as many as the other half)
         }
 
         // Results through LDS (each wave in memory of its own, which no wave reads any more), 256 bytes of a row at a time, so that a store writes
@@ -607,6 +610,7 @@ __global__ __launch_bounds__(256) void prompt_merge_kernel(const PaParams p, con
             for (int d = 1; d < 64; d *= 2) total += __shfl_xor(total, d);
 
             f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
             for (int i0 = 0; i0 < splits; i0 += 4 * AT_ONCE) {
                 if (i0 > 0) load(i0);
 #pragma unroll
@@ -633,7 +637,12 @@ __global__ __launch_bounds__(256) void prompt_merge_kernel(const PaParams p, con
 template <typename E, int D, int R>
 hipError_t launch_of(const PaParams &p, hipStream_t stream)
 {
-    hipLaunchKernelGGL((prompt_attention_kernel<E, D, R>), dim3((unsigned)p.grid), dim3(64 * PA_WAVES), 0, stream, p);
+    if constexpr (R == 0) {
+        if (p.waves == 4) hipLaunchKernelGGL((prompt_attention_kernel<E, D, R, 4>), dim3((unsigned)p.grid), dim3(64 * 4), 0, stream, p);
+    }
+    if constexpr (D == 128) {
+        if (p.waves == 8) hipLaunchKernelGGL((prompt_attention_kernel<E, D, R, 8>), dim3((unsigned)p.grid), dim3(64 * 8), 0, stream, p);
+    }
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.splits <= 1) return e;
     const long long rows = p.total_q * p.kv_heads * p.group, waves = 64ll * p.cus, each = (rows + waves - 1) / waves;

@@ -74,8 +74,7 @@ hipError_t cache_read_launch(const CacheReadParams &p, hipStream_t stream);
 // ---- prompt attention (prompt_attention.hip)
 
 constexpr int PA_KEYS = 64;               // keys of a tile
-constexpr int PA_WAVES = 8;               // of a workgroup, 32 rows each
-constexpr int PA_ROWS = 32 * PA_WAVES;
+constexpr int PA_WAVE_ROWS = 32;
 constexpr int PA_MAX_SPLITS = 128;
 
 struct PaParams {
@@ -89,6 +88,7 @@ struct PaParams {
     int B, kv_heads, group, d, rope, fp16, causal;
     int q_whole;                          // queries come in whole 16-byte pieces
     int splits, split_tiles;              // most splits of a row tile's keys; tiles from which a further split begins
+    int waves;                            // of a workgroup, PA_WAVE_ROWS rows each: 8, or 4 where there are no rope parts
     int grid;                             // workgroups, a multiple of eight
     int cus;                              // compute units
     float scale_log2;

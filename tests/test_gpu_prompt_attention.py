@@ -84,6 +84,19 @@ def test_many_heads_and_sequences(d, rope):
 
 
 @pytest.mark.parametrize("d,rope", FORMS)
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lens_q,lens_k,heads,kv", [([700, 300], [700, 333], 4, 4), ([735, 300], [735, 333], 4, 4), ([65, 1, 0, 80], [400, 1, 7, 80], 15, 1),
+                                                    ([127], [129], 8, 2), ([128], [128], 8, 2), ([129], [1027], 8, 2)])
+def test_workgroups_of_either_size(d, rope, causal, lens_q, lens_k, heads, kv):
+    """Around the number of rows from which workgroups of 128 channels are twice as large."""
+    from pypto_amd import _C
+    plan = _C.prompt_attention_plan(len(lens_q), sum(lens_q), sum(lens_k), heads, kv, d, rope, causal)
+    many = sum(lens_q) * heads // kv >= 512 * len(lens_q)
+    assert plan["rows_per_workgroup"] == (256 if rope or (d == 128 and many) else 128)
+    Call(lens_q, lens_k, heads, kv, d, rope, causal=causal, seed=21, spare=2).run().check()
+
+
+@pytest.mark.parametrize("d,rope", FORMS)
 @pytest.mark.parametrize("lens_q,lens_k", [([600, 0, 500], [6000, 0, 300]), ([1, 700, 400], [1, 200, 7000])])
 def test_more_divided_rows_than_waves_among_rows_that_are_not(d, rope, lens_q, lens_k):
     """More rows than the launch that joins the pieces has waves, so a wave has several, of sequences that are divided and of others."""
