@@ -555,38 +555,37 @@ __global__ __launch_bounds__(64 * W, 2) void prompt_attention_kernel(const PaPar
 // a row, a lane works out the weight of a piece, then eight pieces' outputs are on their way at a time.  Rows of a sequence whose keys were
 // not divided are stepped over together (54000 rows of 2 such sequences: 3 us; with a wave to a row, each looking its sequence up, 9).
 template <typename E, int D>
-__global__ __launch_bounds__(256) void prompt_merge_kernel(const PaParams p, const int each)
+__global__ __launch_bounds__(256, 8) void prompt_merge_kernel(const PaParams p, const int each)
 {
     constexpr int LANES = D / 4, AT_ONCE = 64 / LANES;     // lanes to a piece, four channels each; pieces to a load
     const int l = threadIdx.x & 63;
     const int heads = p.kv_heads * p.group;
-    const long long first = ((long long)blockIdx.x * 4 + (threadIdx.x >> 6)) * each, all = p.total_q * heads;
+    const long long first = ((long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * each, all = p.total_q * heads;
     const long long end = first + each < all ? first + each : all;
     if (first >= end) return;
-    int b = sequence_of(p.cu_q, p.B, first / heads);
+    int tq = (int)(first / heads), head = (int)(first - (long long)tq * heads);
+    int b = __builtin_amdgcn_readfirstlane(sequence_of(p.cu_q, p.B, tq));
     for (long long r = first; b < p.B; ++b) {
         const Span sq = span_of(p.cu_q, b, (int)p.total_q), sk = span_of(p.cu_k, b, (int)p.total_k);
         const int splits = pa_splits_of((sk.len + PA_KEYS - 1) / PA_KEYS, p.split_tiles, p.splits);
-        const long long begins = (long long)sq.begin * heads, behind = (long long)(sq.begin + sq.len) * heads;
-        r = r > begins ? r : begins;
+        if (tq < sq.begin) tq = sq.begin, head = 0, r = (long long)tq * heads;
         if (r >= end) return;
         if (splits <= 1) {                                 // written by the attention kernel
-            r = r > behind ? r : behind;
+            if (tq < sq.begin + sq.len) tq = sq.begin + sq.len, head = 0, r = (long long)tq * heads;
             continue;
         }
-        for (; r < end && r < behind; ++r) {
-            const int tq = (int)(r / heads), head = (int)(r - (long long)tq * heads);
+        for (; r < end && tq < sq.begin + sq.len; ++r, tq += head + 1 == heads, head = head + 1 == heads ? 0 : head + 1) {
             const int sees = pa_visible(tq - sq.begin, sq.len, sk.len, p.causal);
             const f32x2 *const ml = reinterpret_cast<const f32x2 *>(p.part_ml) + r * p.splits;
             const int part = l / LANES, ch = 4 * (l % LANES);
-            const float *po = p.part_o + r * p.splits * D + ch;
+            const float *po = p.part_o + r * p.splits * D;
             f32x4 x[4];
             auto load = [&](const int i0) __attribute__((always_inline)) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int i = i0 + j * AT_ONCE + part;
                     x[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-                    if (i < splits) x[j] = *reinterpret_cast<const f32x4 *>(po + (long long)i * D);
+                    if (i < splits) x[j] = *reinterpret_cast<const f32x4 *>(po + (uint32_t)(i * D + ch));
                 }
             };
             f32x2 mine[PA_MAX_SPLITS / 64];
