@@ -105,11 +105,14 @@ struct PromptPlan {
 };
 
 // Eight waves to a workgroup or four.  Four leave room for a second workgroup on the compute unit, whose work stands in for one's waits at its
-// beginning and end, and waste less on a short sequence; eight read a tile of keys half as often.  With rope parts two workgroups of four do not
-// fit.  64 channels: four are never slower (3760 causal tokens, 128/16 heads, 321 us with eight, 301 with four; 11 sequences of 72 to 243 tokens
-// over 2100 keys, 128/32 heads, 214 and 185; 11 of 1 to 2 over 600, 128 heads, 83 and 51).  128 channels: four for fewer than 512 rows
-// to a sequence and key head (6 sequences of 66 to 445 tokens over 1000 keys, 32 heads, 53 and 41; 8 of 5 to 11, 16/8 heads, 30 and 22), for
-// more eight (9 prompts of 65 to 1871 tokens, 64/8 heads, 166 and 176; 2 of 1841 and 2988, 32/8 heads, 108 and 114).
+// beginning and end, and waste less on a short sequence; eight read a tile of keys half as often.  64 channels: four are never slower (3760
+// causal tokens, 128/16 heads, 321 us with eight, 301 with four; 11 sequences of 72 to 243 tokens over 2100 keys, 128/32 heads, 214 and
+// 185; 11 of 1 to 2 over 600, 128 heads, 83 and 51).  128 channels: four for fewer than 512 rows to a sequence and key head (6 sequences
+// of 66 to 445 tokens over 1000 keys, 32 heads, 53 and 41; with rope parts 9 of 33 to 206 tokens, 128 heads, 68 and 61, 3 of 3 to 17
+// over 2500 keys, 64/16 heads, 38 and 28), and for so few tiles that eight would fill half of the chip or less, unless there are many
+// keys (412 tokens, 16/2 heads, 15.8 and 13.7; 2 of 369, 16/1 heads and rope parts, 17.7 and 15.4; but 5 of 74 to 535 over 6284 to 11824 keys,
+// 8/4 heads and rope parts, 116 and 122).  For more eight (9 prompts of 65 to 1871 tokens, 64/8 heads, 166 and 176; 2 of 1841 and 2988, 32/8
+// heads, 108 and 114).
 //
 // Dividing a call's keys.  The host knows how many rows, keys and sequences there are, not which sequence has how many, and takes them for
 // dealt out evenly.  In microseconds: a workgroup starts and ends in `fixed`, takes `tile` for 64 keys, and partial results are written
@@ -130,7 +133,8 @@ PromptPlan attention_plan(const PtoPromptAttentionArgs *a)
     const long long rows = a->total_q * (a->heads / a->kv_heads);
     const long long key_tiles = (a->total_k + pto::PA_KEYS - 1) / pto::PA_KEYS;             // of one sequence, at most
     pl.splits = 1;
-    pl.waves = a->query_rope ? 8 : (a->d == 64 || rows < 512 * a->b ? 4 : 8);
+    const bool few = 2 * (rows / 256 + a->b) * a->kv_heads <= cus && a->total_k <= 4096 * a->b;
+    pl.waves = a->d == 64 || rows < 512 * a->b || few ? 4 : 8;
     const int wg_rows = pl.waves * pto::PA_WAVE_ROWS;
     const long long slots = pl.waves == 4 ? 2 * cus : cus;                                  // workgroups at a time
     const long long most_tiles = rows / wg_rows + a->b;                                     // of a key head

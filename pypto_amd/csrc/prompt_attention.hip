@@ -114,7 +114,8 @@ __device__ __forceinline__ int pa_visible(const int t, const int lq, const int l
 // the lower two rows.  Then neither 16 lanes that read one piece of 16 key rows nor 16 lanes that read 32 value channels of four
 // rows meet in a bank, and (128 channels) the pieces that a lane reads one after the other are constants away from one of two addresses.  A
 // DMA request writes 1024 bytes in the order of its lanes, so the order of the pieces is in what each lane asks for; eight lanes ask for a
-// whole cache line.
+// whole cache line.  Where two workgroups with rope parts share a compute unit's 160 KiB there is no room between blocks: rows of 256 bytes, piece
+// c of row r at c ^ r % 16 (keys) or c ^ 4 * (r % 4) (values), and an exclusive or to each read.
 constexpr int PA_BLOCK = 1040;
 
 template <typename E, int D, int R, int W>
@@ -123,7 +124,8 @@ __global__ __launch_bounds__(64 * W, 2) void prompt_attention_kernel(const PaPar
     constexpr int ROWS = 32 * W;
     constexpr bool PHASED = W == 8;                        // two waves of a SIMD in this workgroup; otherwise of two workgroups
     constexpr int KP = D * 2;                              // bytes of a key row, and of a value row
-    constexpr int REQ = D == 128 ? PA_BLOCK : 1024;        // bytes from one request's rows to the next one's
+    constexpr bool BLOCKS = D == 128 && !(R > 0 && W == 4), ROW_256 = D == 128 && !BLOCKS;    // how a tile lies in LDS
+    constexpr int REQ = BLOCKS ? PA_BLOCK : 1024;          // bytes from one request's rows to the next one's
     constexpr int K_REQS = PA_KEYS * KP / 1024, R_REQS = PA_KEYS * R * 2 / 1024;
     constexpr int K_BYTES = K_REQS * REQ, R_BYTES = R_REQS * 1024;
     constexpr int K_STAGE = K_BYTES + R_BYTES;             // [keys | rope keys] of a tile
@@ -204,9 +206,9 @@ __global__ __launch_bounds__(64 * W, 2) void prompt_attention_kernel(const PaPar
         const uint8_t *const v_base = reinterpret_cast<const uint8_t *>(p.v + k0 * p.v_t + kvh * p.v_h);
         const uint8_t *const r_base = R > 0 ? reinterpret_cast<const uint8_t *>(p.kr + k0 * p.kr_t + kvh * p.kr_h) : nullptr;
         constexpr int PER = 1024 / KP;                         // rows of a request
-        const int row_of = D == 128 ? (l >> 3) & 3 : l >> 3;   // this lane's row of a request, and its pieces: of keys, values, rope keys
-        const int k_piece = D == 128 ? 8 * (l >> 5) + ((l & 7) ^ (4 * (row_of >> 1))) : (l & 7) ^ (((PER * w + row_of) >> 1) & 7);
-        const int v_piece = D == 128 ? k_piece : (l & 7) ^ (4 * ((row_of >> 1) & 1));
+        const int row_of = BLOCKS ? (l >> 3) & 3 : l / (KP / 16);   // this lane's row of a request, and its pieces: of keys, values, rope keys
+        const int k_piece = BLOCKS ? 8 * (l >> 5) + ((l & 7) ^ (4 * (row_of >> 1))) : ROW_256 ? (l & 15) ^ ((PER * w + row_of) & 15) : (l & 7) ^ (((PER * w + row_of) >> 1) & 7);
+        const int v_piece = BLOCKS ? k_piece : ROW_256 ? (l & 15) ^ (4 * (row_of & 3)) : (l & 7) ^ (4 * ((row_of >> 1) & 1));
         const int r_piece = (l & 7) ^ (((8 * w + (l >> 3)) >> 1) & 7);
         static_assert(W % 2 == 0, "a wave's requests, W * 8 rows apart, have their pieces in the same places");
         const uint32_t k_off = (uint32_t)row_of * (uint32_t)(p.k_t * 2) + 16 * k_piece, v_off = (uint32_t)row_of * (uint32_t)(p.v_t * 2) + 16 * v_piece;
@@ -306,21 +308,25 @@ __global__ __launch_bounds__(64 * W, 2) void prompt_attention_kernel(const PaPar
 
         // LDS addresses of the operand reads in stage 0: key row n, pieces 2 * ks + half; values: keys 4 * half + (l % 16) / 4 (+ 8), channels
         // 16 * ((l / 16) & 1) + 4 * (l % 4)
-        constexpr int KA = D == 128 ? 2 : KS;
-        uint32_t k_lane[KA], r_lane[R > 0 ? RS : 1], v_lane[2];
+        constexpr int KA = BLOCKS ? 2 : ROW_256 ? 1 : KS, VA = ROW_256 ? 1 : 2;
+        uint32_t k_lane[KA], r_lane[R > 0 ? RS : 1], v_lane[VA];
 #pragma unroll
         for (int i = 0; i < KA; ++i)
-            k_lane[i] = lds0 + (D == 128 ? (n >> 2) * REQ + (n & 3) * 128 + 16 * half + 64 * (i ^ ((n >> 1) & 1)) : n * KP + 16 * ((2 * i + half) ^ ((n >> 1) & 7)));
+            k_lane[i] = lds0 + (BLOCKS    ? (n >> 2) * REQ + (n & 3) * 128 + 16 * half + 64 * (i ^ ((n >> 1) & 1))
+                                : ROW_256 ? n * KP + 16 * (half ^ (n & 15))
+                                          : n * KP + 16 * ((2 * i + half) ^ ((n >> 1) & 7)));
 #pragma unroll
         for (int i = 0; i < RS; ++i) r_lane[i] = lds0 + K_BYTES + n * (R * 2) + 16 * ((2 * i + half) ^ ((n >> 1) & 7));
         {
             const int row = (l & 15) >> 2, low = 2 * ((l >> 4) & 1) + ((l & 3) >> 1);
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < VA; ++i)
                 v_lane[i] = lds0 + STAGES * K_STAGE + 8 * (l & 1) +
-                            (D == 128 ? half * REQ + row * 128 + 64 * (i ^ (row >> 1)) + 16 * low : (4 * half + row) * KP + 16 * ((4 * i + low) ^ (4 * (row >> 1))));
+                            (BLOCKS    ? half * REQ + row * 128 + 64 * (i ^ (row >> 1)) + 16 * low
+                             : ROW_256 ? (4 * half + row) * KP + 64 * row + 16 * low
+                                       : (4 * half + row) * KP + 16 * ((4 * i + low) ^ (4 * (row >> 1))));
         }
-        constexpr int V_EIGHT = D == 128 ? 2 * REQ : 8 * KP;   // to the value row eight keys on
+        constexpr int V_EIGHT = BLOCKS ? 2 * REQ : 8 * KP;   // to the value row eight keys on
 
         f32x16 s[2];                                           // scores of the tile in hand
         frag pf[4];                                            // probabilities of the tile before it
@@ -328,7 +334,7 @@ __global__ __launch_bounds__(64 * W, 2) void prompt_attention_kernel(const PaPar
         // values, in another; operands are read AHEAD products before their use.
         auto products = [&](auto with_scores, auto with_values, const int k_stage, const int v_stage) __attribute__((always_inline)) {
             constexpr int NQ = decltype(with_scores)::value ? 2 * (KS + RS) : 0, NP = decltype(with_values)::value ? 4 * CT : 0, N = NQ + NP;
-            uint32_t kb[KA], rb[R > 0 ? RS : 1], vb[2];        // (what the compiler cannot take apart: the rest of an address is an instruction's constant)
+            uint32_t kb[KA], rb[R > 0 ? RS : 1], vb[VA];        // (what the compiler cannot take apart: the rest of an address is an instruction's constant)
             if (NQ > 0) {
 #pragma unroll
                 for (int i = 0; i < KA; ++i) kb[i] = opaque(k_lane[i] + k_stage * K_STAGE);
@@ -337,7 +343,7 @@ __global__ __launch_bounds__(64 * W, 2) void prompt_attention_kernel(const PaPar
             }
             if (NP > 0) {
 #pragma unroll
-                for (int i = 0; i < 2; ++i) vb[i] = opaque(v_lane[i] + v_stage * K_BYTES);
+                for (int i = 0; i < VA; ++i) vb[i] = opaque(v_lane[i] + v_stage * K_BYTES);
             }
             frag a[N];
             auto is_value = [](const int j) { return (j + 1) * NP / N > j * NP / N; };
@@ -345,13 +351,15 @@ __global__ __launch_bounds__(64 * W, 2) void prompt_attention_kernel(const PaPar
                 const int pv = j * NP / N, qk = j - pv;        // products of either kind before this one
                 if (is_value(j)) {
                     const int ks = pv / CT, c = pv % CT;
-                    const uint32_t at = vb[c & 1] + (D == 128 ? ks * 4 * REQ + (c >> 1) * 512 : 16 * ks * KP);
+                    const uint32_t at = ROW_256 ? (vb[0] ^ (64 * c)) + 16 * ks * KP : vb[c & (VA - 1)] + (BLOCKS ? ks * 4 * REQ + (c >> 1) * 512 : 16 * ks * KP);
                     const s16x4 lo = lds_tr16(at), hi = lds_tr16(at + V_EIGHT);
                     a[j] = __builtin_bit_cast(frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
                 } else {
                     const int h = qk & 1, i = qk >> 1;
-                    a[j] = lds_frag<frag>(i >= KS ? rb[(i - KS) % (R > 0 ? RS : 1)] + h * 32 * (R * 2)
-                                                  : D == 128 ? kb[(i >> 1) & 1] + h * 8 * REQ + (i >> 2) * 512 + (i & 1) * 32 : kb[i % KA] + h * 32 * KP);
+                    a[j] = lds_frag<frag>(i >= KS   ? rb[(i - KS) % (R > 0 ? RS : 1)] + h * 32 * (R * 2)
+                                          : BLOCKS  ? kb[(i >> 1) & (KA - 1)] + h * 8 * REQ + (i >> 2) * 512 + (i & 1) * 32
+                                          : ROW_256 ? (kb[0] ^ (32 * i)) + h * 32 * KP
+                                                    : kb[i % KA] + h * 32 * KP);
                 }
             };
             const f32x16 zero = {};
@@ -636,9 +644,7 @@ __global__ __launch_bounds__(256, 8) void prompt_merge_kernel(const PaParams p, 
 template <typename E, int D, int R>
 hipError_t launch_of(const PaParams &p, hipStream_t stream)
 {
-    if constexpr (R == 0) {
-        if (p.waves == 4) hipLaunchKernelGGL((prompt_attention_kernel<E, D, R, 4>), dim3((unsigned)p.grid), dim3(64 * 4), 0, stream, p);
-    }
+    if (p.waves == 4) hipLaunchKernelGGL((prompt_attention_kernel<E, D, R, 4>), dim3((unsigned)p.grid), dim3(64 * 4), 0, stream, p);
     if constexpr (D == 128) {
         if (p.waves == 8) hipLaunchKernelGGL((prompt_attention_kernel<E, D, R, 8>), dim3((unsigned)p.grid), dim3(64 * 8), 0, stream, p);
     }

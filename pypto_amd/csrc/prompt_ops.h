@@ -88,7 +88,7 @@ struct PaParams {
     int B, kv_heads, group, d, rope, fp16, causal;
     int q_whole;                          // queries come in whole 16-byte pieces
     int splits, split_tiles;              // most splits of a row tile's keys; tiles from which a further split begins
-    int waves;                            // of a workgroup, PA_WAVE_ROWS rows each: 8, or 4 where there are no rope parts
+    int waves;                            // of a workgroup, PA_WAVE_ROWS rows each: 8, or 4
     int grid;                             // workgroups, a multiple of eight
     int cus;                              // compute units
     float scale_log2;

@@ -85,14 +85,14 @@ def test_many_heads_and_sequences(d, rope):
 
 @pytest.mark.parametrize("d,rope", FORMS)
 @pytest.mark.parametrize("causal", [True, False])
-@pytest.mark.parametrize("lens_q,lens_k,heads,kv", [([700, 300], [700, 333], 4, 4), ([735, 300], [735, 333], 4, 4), ([65, 1, 0, 80], [400, 1, 7, 80], 15, 1),
-                                                    ([127], [129], 8, 2), ([128], [128], 8, 2), ([129], [1027], 8, 2)])
-def test_workgroups_of_either_size(d, rope, causal, lens_q, lens_k, heads, kv):
-    """Around the number of rows from which workgroups of 128 channels are twice as large."""
+@pytest.mark.parametrize("lens_q,lens_k,heads,kv,rows", [
+    ([700, 300], [700, 333], 4, 4, 128), ([735, 300], [735, 333], 32, 32, 256), ([65, 1, 0, 80], [400, 1, 7, 80], 15, 1, 128),
+    ([600], [700], 64, 32, 256), ([500], [1027], 40, 40, 128), ([513], [1027], 64, 64, 256), ([127], [129], 8, 2, 128)])
+def test_workgroups_of_either_size(d, rope, causal, lens_q, lens_k, heads, kv, rows):
+    """Around the numbers of rows from which workgroups of 128 channels are twice as large."""
     from pypto_amd import _C
     plan = _C.prompt_attention_plan(len(lens_q), sum(lens_q), sum(lens_k), heads, kv, d, rope, causal)
-    many = sum(lens_q) * heads // kv >= 512 * len(lens_q)
-    assert plan["rows_per_workgroup"] == (256 if rope or (d == 128 and many) else 128)
+    assert plan["rows_per_workgroup"] == (rows if d == 128 else 128)
     Call(lens_q, lens_k, heads, kv, d, rope, causal=causal, seed=21, spare=2).run().check()
 
 
