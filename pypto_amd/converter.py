@@ -94,15 +94,21 @@ def same_rows(a: torch.Tensor, b: torch.Tensor) -> bool:
 
 
 def side_by_side(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether two tensors are different columns of rows that lie equally far apart (slices of one tensor)."""
-    if min(a.dim(), b.dim()) < 2 or min(a.shape[0], b.shape[0]) < 2:
-        return False
-    pitch = a.stride(0) * a.element_size()
-    if pitch != b.stride(0) * b.element_size() or pitch <= 0:
-        return False
-    (lo, hi), (lo2, hi2) = extent(a[0]), extent(b[0])
-    at = (lo2 - lo) % pitch                                # where b's columns begin, seen from a's
-    return at >= hi - lo and at + (hi2 - lo2) <= pitch
+    """Whether two tensors are different columns of rows that lie equally far apart, or different channels of such heads (slices of one
+    tensor)."""
+    x, y = a, b
+    for d in range(min(a.dim(), b.dim()) - 1):
+        pitch = x.stride(0) * a.element_size()
+        if min(x.shape[0], y.shape[0]) < 2 or pitch <= 0 or y.stride(0) * b.element_size() != pitch:
+            return False
+        if d and (a.stride(0) % x.stride(0) or b.stride(0) % y.stride(0)):
+            return False
+        x, y = x[0], y[0]
+        (lo, hi), (lo2, hi2) = extent(x), extent(y)
+        at = (lo2 - lo) % pitch                            # where b's columns begin, seen from a's
+        if at >= hi - lo and at + (hi2 - lo2) <= pitch:
+            return True
+    return False
 
 
 def refuse_overlap(out: torch.Tensor, other: torch.Tensor, what: str) -> None:

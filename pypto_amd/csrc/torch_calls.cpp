@@ -395,13 +395,14 @@ bool clash(const at::Tensor &out, const at::Tensor &in, const bool where_same = 
         for (int64_t d = from; d < t.dim(); ++d) n += (t.size(d) - 1) * t.stride(d);
         return n * static_cast<int64_t>(t.element_size());
     };
-    if (out.dim() >= 2 && in.dim() >= 2 && out.size(0) > 1 && in.size(0) > 1) {
-        // different columns of the same rows (slices of one tensor) do not meet
-        const int64_t pitch = out.stride(0) * static_cast<int64_t>(out.element_size());
-        if (pitch > 0 && pitch == in.stride(0) * static_cast<int64_t>(in.element_size())) {
-            const int64_t at = (((b - a) % pitch) + pitch) % pitch;
-            if (at >= bytes(out, 1) && at + bytes(in, 1) <= pitch) return false;
-        }
+    // different columns of the same rows, or channels of the same heads (slices of one tensor) do not meet
+    for (int64_t d = 0; d + 1 < out.dim() && d + 1 < in.dim(); ++d) {
+        if (out.size(d) < 2 || in.size(d) < 2) break;
+        const int64_t pitch = out.stride(d) * static_cast<int64_t>(out.element_size());
+        if (pitch <= 0 || pitch != in.stride(d) * static_cast<int64_t>(in.element_size())) break;
+        if (d > 0 && (out.stride(0) % out.stride(d) != 0 || in.stride(0) % in.stride(d) != 0)) break;
+        const int64_t at = (((b - a) % pitch) + pitch) % pitch;
+        if (at >= bytes(out, d + 1) && at + bytes(in, d + 1) <= pitch) return false;
     }
     return a < b + bytes(in, 0) && b < a + bytes(out, 0);
 }
@@ -470,10 +471,7 @@ PyObject *rotary_embedding_call(PyObject *, PyObject *const *args, Py_ssize_t n)
             seen[k] = &in, seen[2 + k] = &out;
             if (clash(out, in, false)) return declined();
         }
-        if (sides == 2) {
-            const bool in_place = seen[0]->const_data_ptr() == seen[2]->const_data_ptr() && seen[1]->const_data_ptr() == seen[3]->const_data_ptr();
-            if (!in_place && (clash(*seen[2], *seen[1]) || clash(*seen[3], *seen[0]) || clash(*seen[2], *seen[3]))) return declined();
-        }
+        if (sides == 2 && (clash(*seen[2], *seen[1]) || clash(*seen[3], *seen[0]) || clash(*seen[2], *seen[3]))) return declined();
         for (int k = 0; k < sides; ++k) {
             PtoRotaryTensor &r = k == 0 ? a.query : a.key;
             r.out = c.out<void>(*seen[2 + k]), r.in = c.ptr<void>(*seen[k]);
@@ -588,12 +586,14 @@ PyObject *prompt_attention_call(PyObject *, PyObject *const *args, Py_ssize_t n)
             if (!c.ok || !dims(qr, 3) || qr.size(0) != a.total_q || qr.size(1) != a.heads || kr.size(0) != a.total_k ||
                 (heads_of(kr) != 1 && heads_of(kr) != a.kv_heads) || clash(out, qr) || clash(out, kr))
                 return declined();
-            a.query_rope = c.ptr<void>(qr), a.query_rope_stride_t = row_stride(qr), a.query_rope_stride_h = head_stride(qr);
-            a.key_rope = c.ptr<void>(kr), a.key_rope_stride_t = row_stride(kr), a.key_rope_stride_h = head_stride(kr);
+            alignas(16) static char none_there[16];                   // (an empty tensor may have no memory)
+            a.query_rope = qr.numel() > 0 ? c.ptr<void>(qr) : none_there, a.query_rope_stride_t = row_stride(qr), a.query_rope_stride_h = head_stride(qr);
+            a.key_rope = kr.numel() > 0 ? c.ptr<void>(kr) : none_there, a.key_rope_stride_t = row_stride(kr), a.key_rope_stride_h = head_stride(kr);
         }
         if (!c.none(9)) {
             const at::Tensor &lse = c.shaped(9, FP32, {a.total_q, a.heads});
             if (!c.ok || clash(lse, out) || clash(lse, q) || clash(lse, k) || clash(lse, v)) return declined();
+            if (!c.none(7) && (clash(lse, c.tensor(7, true)) || clash(lse, c.tensor(8, true)))) return declined();
             a.lse = c.out<float>(lse);
         }
         a.query = c.ptr<void>(q), a.key = c.ptr<void>(k), a.value = c.ptr<void>(v), a.out = c.out<void>(out);

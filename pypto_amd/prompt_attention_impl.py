@@ -33,7 +33,8 @@ def prompt_attention(query, key, value, cu_seqlens_q, cu_seqlens_k, attention_ou
     query_rope (total_q, heads, 64) and key_rope (total_k, 64) or (total_k, kv_heads, 64), or None both (with d = 128);
     cu_seqlens_q, cu_seqlens_k (b + 1,) int32, ascending: where each sequence's queries and keys begin, and behind the last one;
     attention_out (total_q, heads, d), softmax_lse (total_q, heads) fp32 or None: written in place, the latter with the natural
-    logarithm of the sum of the exponentials of a row's scores.
+    logarithm of the sum of the exponentials of a row's scores.  key, value and key_rope begin at multiples of 16 bytes and their strides are
+    multiples of 8 elements.
 
     causal: the last query of a sequence sees all of its keys, each one before it one key less; otherwise every query sees all keys of
     its sequence.  Rows that see no key are zeros (softmax_lse -inf); rows of no sequence stay as they were.  What lies behind a

@@ -228,6 +228,44 @@ def test_empty_calls():
         Call(lens_q, lens_k, 4, 2, 64, seed=17).run().check()
 
 
+@pytest.mark.parametrize("lens_q,lens_k", [([0], [0]), ([0, 0], [5, 0]), ([4], [0]), ([0], [9])])
+def test_empty_calls_with_rope_parts(lens_q, lens_k):
+    """(Empty tensors have no address.)"""
+    Call(lens_q, lens_k, 4, 2, 128, True, seed=17).run().check()
+
+
+def test_statistics_in_the_memory_of_an_input_are_refused():
+    c = Call([20], [20], 4, 4, 128, True, seed=22, shared=False)
+    for name in ("q", "qr", "out"):
+        t = getattr(c, name).contiguous()
+        setattr(c, name, t)
+        c.lse = t.view(-1).view(torch.float32)[:80].view(20, 4)
+        with pytest.raises(ValueError, match="overlap"):
+            c.run()
+
+
+@pytest.mark.parametrize("rope", [False, True])
+@pytest.mark.parametrize("form", ["sliced", "odd_output", "sign", "many_keys"])
+def test_the_larger_workgroups_in_every_form(form, rope):
+    """Queries and outputs that promise their element's alignment only, a negative scale, keys divided over workgroups."""
+    from pypto_amd import _C
+    lens = [513, 600] if form == "many_keys" else [600]
+    keys, heads = ([5000, 4900], 16) if form == "many_keys" else ([700], 48)
+    plan = _C.prompt_attention_plan(len(lens), sum(lens), sum(keys), heads, heads, 128, rope, True)
+    assert plan["rows_per_workgroup"] == 256 and (plan["key_splits"] > 1) == (form == "many_keys")
+    c = Call(lens, keys, heads, heads, 128, rope, HALF, seed=23, scale=-0.09 if form == "sign" else None)
+    if form == "sliced":
+        wide = torch.zeros(600, heads, 200, dtype=HALF, device=DEV)
+        wide[:, :, 3:131] = c.q
+        c.q = wide[:, :, 3:131]
+        if rope:
+            wide[:, :, 131:195] = c.qr
+            c.qr = wide[:, :, 131:195]
+    elif form == "odd_output":
+        c.out = torch.full((600, heads, 131), 7.0, dtype=HALF, device=DEV)[:, :, 1:129]
+    c.run().check()
+
+
 def test_pieces_of_keys_joined_by_their_statistics():
     """Two calls over parts of the keys, joined by softmax_lse, are the call over all of them."""
     c = Call([50], [300], 4, 2, 128, causal=False, seed=18).run()

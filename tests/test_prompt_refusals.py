@@ -77,6 +77,22 @@ def test_rotation_s_scalars_overlaps_and_device():
     refused(ValueError, "overlap", pypto_amd.rotary_embedding, changed(changed(args, 4, wide[:, :4]), 5, wide[:, 3:4, :64]))
 
 
+def test_rotation_of_one_tensor_as_queries_and_keys():
+    """In place or not, no memory may be queries and keys at once; channels of the same heads that do not meet may."""
+    pos, freq = torch.zeros(5, dtype=torch.int64), pypto_amd.rotary_frequencies(64)
+    x = torch.zeros(5, 4, 160, dtype=BF)
+    refused(ValueError, "overlap", pypto_amd.rotary_embedding, [x, x, pos, freq, x, x])
+    refused(ValueError, "overlap", pypto_amd.rotary_embedding, [x[:, :3], x[:, 2:], pos, freq, x[:, :3], x[:, 2:]])
+    refused(ValueError, "overlap", pypto_amd.rotary_embedding, [x[..., :96], x[..., 64:], pos, freq, x[..., :96], x[..., 64:]])
+    q, k = x[..., :80], x[..., 80:]
+    refused(RuntimeError, "GPU", pypto_amd.rotary_embedding, [q, k, pos, freq, q, k])
+    refused(RuntimeError, "GPU", pypto_amd.rotary_embedding, [x[:, :3], x[:, 3:], pos, freq, x[:, :3], x[:, 3:]])
+    odd = torch.zeros(1600, dtype=BF).as_strided((5, 3, 80), (200, 160, 1))          # heads run into the next row's
+    other = torch.zeros(1600, dtype=BF)
+    refused(ValueError, "overlap|share", pypto_amd.rotary_embedding,
+            [odd, other.as_strided((5, 3, 80), (200, 160, 1)), pos, freq, odd, odd[:, :, :80]])
+
+
 def test_frequencies():
     plain = pypto_amd.rotary_frequencies(64)
     assert plain.dtype == torch.float64 and float(plain[0]) == 1.0 and float(plain[16]) == pytest.approx(0.01, rel=1e-14)
