@@ -312,3 +312,29 @@ def test_another_stream_and_replays_of_a_captured_call():
             call(e)
             torch.cuda.synchronize()
             assert torch.equal(c.out, e.out) and torch.equal(c.lse, e.lse)
+
+
+def test_replays_with_other_lengths_and_on_two_streams_at_once():
+    """A captured launch follows the tables of beginnings as they are when it is replayed; two graphs run side by side."""
+    calls = [Call([1, 200, 3], [4000, 200, 900], 8, 2, 128, True, seed=24 + i) for i in range(2)]
+    cu = [[starts(c.lens_q), starts(c.lens_k)] for c in calls]
+    graphs, streams = [], [torch.cuda.Stream() for _ in calls]
+    for c, (cu_q, cu_k) in zip(calls, cu):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            pypto_amd.prompt_attention(c.q, c.k, c.v, cu_q, cu_k, c.out, c.scale, query_rope=c.qr, key_rope=c.kr, softmax_lse=c.lse)
+        graphs.append(graph)
+    for lens_q, lens_k in (([1, 200, 3], [4000, 200, 900]), ([150, 4, 50], [100, 3900, 1100]), ([0, 0, 204], [5000, 99, 1])):
+        for c, (cu_q, cu_k) in zip(calls, cu):
+            c.lens_q, c.lens_k = lens_q, lens_k
+            cu_q.copy_(starts(lens_q))
+            cu_k.copy_(starts(lens_k))
+            c.out.fill_(7.0)
+            c.lse.fill_(7.0)
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for c in calls:
+            c.check()
