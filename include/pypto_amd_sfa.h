@@ -515,8 +515,10 @@ int pto_rotary_launch(const PtoRotaryArgs *args, void *hip_stream);
 
 /*
  * Quantises latents as they are written into the cache of the sparse attention: of every 128 channels
- * steps = 127 * (1 / max|v|), code = rint(v * steps), scale = 1 / steps in fp32, each operation rounded (the MLA prolog
- * divides 127 by the maximum at once: a code may be one step away from the prolog's in rare entries).
+ * steps = 127 * (1 / max|v|), code = rint(v * steps), scale = 1 / steps in fp32, each operation rounded.  With prolog_steps
+ * steps = 127 / max|v| in one rounding, as the MLA prolog divides: the codes and scales are then those that it writes for such latents.
+ * Without it (normally distributed bf16 latents) one scale in four or five differs from them in its last bits, and 4 codes in 10000, in
+ * one row of six, are one step away.
  *
  *   latent       [t, 512], rope [t, 64]   dtype (PTO_DT_*)
  *   cache_index  [t]  int64, physical row of each token; rows outside [0, cache_rows) are skipped.  No row may be named twice:
@@ -542,6 +544,8 @@ typedef struct PtoCacheWriteArgs {
     int64_t latent_stride, rope_stride, values_stride;
     int32_t dtype;
     int32_t packed;
+    int32_t prolog_steps;
+    int32_t reserved;
 } PtoCacheWriteArgs;
 
 int pto_cache_write_launch(const PtoCacheWriteArgs *args, void *hip_stream);
@@ -645,11 +649,11 @@ const char *pto_version(void);
 
 /*
  * Revision of the argument structs above.  The structs carry no size field and have grown between revisions
- * (revision 2 added absorb_exact and a reserved word to PtoMlaPrologQuantArgs, revision 1 was library 0.1.0): a
- * caller built against another revision would hand over structs of another size.  Compare once after loading:
+ * (revision 3 added prolog_steps and a reserved word to PtoCacheWriteArgs, revision 2 absorb_exact and a reserved word to
+ * PtoMlaPrologQuantArgs, revision 1 was library 0.1.0): a caller built against another revision would hand over structs of another size.  Compare once after loading:
  * pto_abi_revision() == PTO_ABI_REVISION, else do not call the launch functions of this library.
  */
-#define PTO_ABI_REVISION 2
+#define PTO_ABI_REVISION 3
 int pto_abi_revision(void);
 
 #ifdef __cplusplus

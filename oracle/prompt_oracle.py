@@ -33,13 +33,13 @@ def turn(x, positions, frequencies, layout, offset=0, factor=1.0):
     return out
 
 
-def quantise(latent):
+def quantise(latent, prolog_steps=False):
     """latent [t, 512] -> codes int8 [t, 512], scales fp32 [t, 4], values fp32 [t, 512] (to be rounded to bf16), in numpy's fp32,
-    groups of no number and of next to nothing among them."""
+    groups of no number and of next to nothing among them.  prolog_steps: 127 / max rounded once."""
     y = latent.float().cpu().numpy().reshape(-1, 4, 128)
     most = np.abs(y).max(axis=2, keepdims=True)                      # (carries what is no number)
     with np.errstate(all="ignore"):
-        steps = (np.float32(127.0) * (np.float32(1) / most).astype(np.float32)).astype(np.float32)
+        steps = ((np.float32(127.0) / most) if prolog_steps else np.float32(127.0) * (np.float32(1) / most).astype(np.float32)).astype(np.float32)
         number, zero = np.isfinite(most), ~np.isfinite(steps)
         codes = np.where(number & ~zero, np.rint((y * steps).astype(np.float32)), 0).astype(np.float32)
         scales = np.where(number, np.where(zero, np.float32(0), (np.float32(1) / steps).astype(np.float32)), np.float32("nan"))

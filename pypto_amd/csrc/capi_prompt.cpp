@@ -261,6 +261,7 @@ int pto_cache_write_launch(const PtoCacheWriteArgs *a, void *hip_stream)
     p.values_t = a->values_stride;
     p.T = a->t;
     p.dtype = a->dtype;
+    p.one_rounding = a->prolog_steps != 0;
     const hipError_t e = pto::cache_write_launch(p, static_cast<hipStream_t>(hip_stream));
     if (e != hipSuccess) return fail(PTO_E_LAUNCH, "cache_write: launch failed: %s", hipGetErrorString(e));
     return PTO_OK;

@@ -56,6 +56,7 @@ struct CacheWriteParams {
     long long values_t;
     long long T;
     int dtype;
+    int one_rounding;                     // 127 / max in one rounding
 };
 hipError_t cache_write_launch(const CacheWriteParams &p, hipStream_t stream);
 

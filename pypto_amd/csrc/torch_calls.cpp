@@ -494,13 +494,14 @@ bool cache_args(Call &c, const int i, const at::Tensor *(&parts)[3], int64_t &ro
     return c.ok;
 }
 
-// latent, key_rope, cache_index, nope, rope, scales (or packed, None, None), values (or None)
+// latent, key_rope, cache_index, nope, rope, scales (or packed, None, None), values (or None), prolog_steps
 PyObject *cache_write_call(PyObject *, PyObject *const *args, Py_ssize_t n)
 {
-    if (n != 7) return declined();
+    if (n != 8 || (args[7] != Py_True && args[7] != Py_False)) return declined();
     return guarded([&]() -> PyObject * {
         Call c{args};
         PtoCacheWriteArgs a{};
+        a.prolog_steps = args[7] == Py_True;
         const at::Tensor &latent = c.tensor(0, true);
         if (!c.ok) return declined();
         a.dtype = dtype_code(latent, c.ok);

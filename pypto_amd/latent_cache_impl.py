@@ -4,7 +4,9 @@ The cache is what the attention operators take: three arrays (``sparse_flash_att
 one packed array of 656-byte rows (``sparse_attention_antiquant_d``).  The MLA prolog writes the three arrays as the last step of its
 projections; these operators write either form from latents that are already there (a prompt's, from plain projections), in
 fp32: of every 128 channels ``steps = 127 * (1 / max|v|)``, ``code = rint(v * steps)``, ``scale = 1 / steps``, the value stored being
-``bf16(code * scale)``.  (The prolog rounds ``127 / max|v|`` once: a code may be one step away from its in rare entries.)
+``bf16(code * scale)``.  With ``prolog_steps`` ``steps = 127 / max|v|`` in one rounding, as the prolog divides: rows are then bit for bit
+those that it writes for the same latents, which a cache that both write, or whose pages are compared, wants.  (Between the two one scale
+in four or five differs in its last bits, and of bf16 latents 4 codes in 10000, in one row of six, by one step.)
 
 Reading gathers positions of sequences through their block tables, de-quantised as the attention does it and packed one sequence behind
 the other: the context that a prompt's next chunk makes its keys and values from.
@@ -49,10 +51,10 @@ def _rows(t, name, width, dtypes, rows=None):
     return t
 
 
-def _write(op, latent, key_rope, cache_index, parts, names, latent_out):
+def _write(op, latent, key_rope, cache_index, parts, names, latent_out, prolog_steps):
     C = _native.load()
     pad = list(parts) + [None] * (3 - len(parts))
-    if C.cache_write_call(latent, key_rope, cache_index, *pad, latent_out):
+    if C.cache_write_call(latent, key_rope, cache_index, *pad, latent_out, prolog_steps):
         return None
     lat = _rows(as_rows(latent, "latent"), "latent", KV_LORA_RANK, DTYPES)
     rope = _rows(as_rows(key_rope, "key_rope"), "key_rope", ROPE_DIM, (lat.dtype,), lat.shape[0])
@@ -77,26 +79,27 @@ def _write(op, latent, key_rope, cache_index, parts, names, latent_out):
             refuse_overlap(values, c, f"latent_out and {n}")
         tensors.append(values)
     _on_gpu(op, tensors)
-    if not C.cache_write_call(lat, rope, idx, *(cache + [None] * (3 - len(cache))), values):
+    if not C.cache_write_call(lat, rope, idx, *(cache + [None] * (3 - len(cache))), values, bool(prolog_steps)):
         raise RuntimeError(f"{op}: these arguments are not supported")
     return None
 
 
-def latent_cache_write(latent, key_rope, cache_index, kv_cache, kr_cache, k_scale_cache, latent_out=None):
+def latent_cache_write(latent, key_rope, cache_index, kv_cache, kr_cache, k_scale_cache, latent_out=None, prolog_steps=False):
     """Quantises rows into the three-array cache.
 
     latent (t, 512), key_rope (t, 64) bf16, fp16 or fp32, both alike; cache_index (t,) int64, the physical row of each token (rows outside the
     cache are skipped; no row may be named twice); kv_cache int8 with rows of 512, kr_cache bf16 of 64, k_scale_cache fp32 of 4, in the
     attention's two or the MLA prolog's four dimensions, written in place.  latent_out (t, 512) bf16 or None receives what the written rows
-    stand for (it may be ``latent`` itself).
+    stand for (it may be ``latent`` itself).  prolog_steps: codes and scales are those that the MLA prolog writes.
     """
     return _write("latent_cache_write", latent, key_rope, cache_index, (kv_cache, kr_cache, k_scale_cache),
-                  ("kv_cache", "kr_cache", "k_scale_cache"), latent_out)
+                  ("kv_cache", "kr_cache", "k_scale_cache"), latent_out, prolog_steps)
 
 
-def latent_cache_write_packed(latent, key_rope, cache_index, nope_cache, latent_out=None):
+def latent_cache_write_packed(latent, key_rope, cache_index, nope_cache, latent_out=None, prolog_steps=False):
     """The same into the packed cache: nope_cache int8 with rows of 656 bytes, written in place."""
-    return _write("latent_cache_write_packed", latent, key_rope, cache_index, (nope_cache,), ("nope_cache",), latent_out)
+    return _write("latent_cache_write_packed", latent, key_rope, cache_index, (nope_cache,), ("nope_cache",), latent_out,
+                  prolog_steps)
 
 
 def _read(op, parts, names, block_table, cu_seqlens, latent_out, key_rope_out, block_size, first):

@@ -155,6 +155,12 @@ def test_read_s_first_positions_and_device():
     refused(RuntimeError, "GPU", pypto_amd.latent_cache_read_packed, [torch.zeros(256, 656, dtype=torch.int8)] + read()[3:], first=torch.zeros(2, dtype=torch.int32))
 
 
+def test_write_with_the_prolog_s_steps_refuses_what_the_other_does():
+    refused(RuntimeError, "GPU", pypto_amd.latent_cache_write, write(), prolog_steps=True)
+    refused(TypeError, "cache_index", pypto_amd.latent_cache_write, changed(write(), 2, torch.zeros(3, dtype=torch.int32)), prolog_steps=True)
+    refused(RuntimeError, "GPU", pypto_amd.latent_cache_write_packed, write()[:3] + [torch.zeros(256, 656, dtype=torch.int8)], prolog_steps=1)
+
+
 # ---------------------------------------------------------------- prompt attention
 
 def attention():
