@@ -2,7 +2,8 @@
 //
 // Channel pair i of a token at position n turns by the angle n * freq[i].  The angle needs 64 bits (position 131071 in fp32
 // leaves an angle 2^-7 of its bits after the point); it is reduced to the nearest quarter turn there, and what is left, at most
-// pi/4, goes through the sine's and cosine's series in fp32, whose first left-out terms are below 2e-9.
+// pi/4, goes through the sine's and cosine's Taylor series in fp32, whose first left-out terms, x^11 / 11! and x^12 / 12!, are at most
+// 1.8e-9 and 1.2e-10.  (The cosine without its tenth power is 2.5e-8 off there, 0.4 of an fp32 step.)
 #include "common.h"
 #include "prompt_ops.h"
 #include "pypto_amd_sfa.h"
@@ -22,7 +23,7 @@ __device__ __forceinline__ Turn turn_of(const double position, const double freq
     const double left = fma(-k, 6.123233995736766036e-17, fma(-k, 1.5707963267948965580, angle));
     const float x = (float)left, z = x * x;
     const float s = x + x * z * (-1.6666667e-1f + z * (8.3333333e-3f + z * (-1.9841270e-4f + z * 2.7557319e-6f)));
-    const float c = 1.0f + z * (-0.5f + z * (4.1666667e-2f + z * (-1.3888889e-3f + z * 2.4801587e-5f)));
+    const float c = 1.0f + z * (-0.5f + z * (4.1666667e-2f + z * (-1.3888889e-3f + z * (2.4801587e-5f + z * -2.7557319e-7f))));
     const int quarter = (int)(k - 4.0 * floor(k * 0.25));
     const float cc = (quarter & 1) ? s : c, ss = (quarter & 1) ? c : s;
     return {factor * ((quarter == 1 || quarter == 2) ? -cc : cc), factor * ((quarter & 2) ? -ss : ss)};
