@@ -462,7 +462,7 @@ int pto_mla_indexer_prolog_quant_launch(const PtoMlaIndexerPrologQuantArgs *args
  *   frequencies  [pairs]       fp64, radians per position
  *   cos, sin     [t, 2*pairs]  dtype (PTO_DT_*), columns i and i + pairs alike
  *
- * Angles are taken in 64 bits.  Constraints: pairs a multiple of 4, up to 128.
+ * Angles are taken in 64 bits, up to 2^63 to either side.  Constraints: pairs a multiple of 4, up to 128.
  */
 typedef struct PtoRotaryTablesArgs {
     const void *positions;

@@ -15,18 +15,45 @@ struct Turn {
     float c, s;
 };
 
-__device__ __forceinline__ Turn turn_of(const double position, const double freq, const float factor)
+// The rounding of an angle's quotient may miss the nearest quarter turn where it is more than this, by a thousand of them at 2^63: what is
+// left is then reduced again.
+constexpr double TURNS_FAR = 1.0e12;
+
+// far: set if this angle is to be asked for again, with AGAIN.
+template <bool AGAIN>
+__device__ __forceinline__ Turn turn_by(const double position, const double freq, const float factor, bool &far)
 {
     const double angle = position * freq;
-    const double k = rint(angle * 0.63661977236758134308);                  // 2 / pi
+    double k = rint(angle * 0.63661977236758134308);                        // 2 / pi
     // pi / 2 as the sum of two doubles
-    const double left = fma(-k, 6.123233995736766036e-17, fma(-k, 1.5707963267948965580, angle));
+    auto without = [](const double x, const double n) { return fma(-n, 6.123233995736766036e-17, fma(-n, 1.5707963267948965580, x)); };
+    double left = without(angle, k);
+    if (AGAIN) {
+        const double more = rint(left * 0.63661977236758134308);
+        left = without(left, more);
+        k = (k - 4.0 * floor(k * 0.25)) + more;
+    } else {
+        far |= fabs(k) > TURNS_FAR;
+    }
     const float x = (float)left, z = x * x;
     const float s = x + x * z * (-1.6666667e-1f + z * (8.3333333e-3f + z * (-1.9841270e-4f + z * 2.7557319e-6f)));
     const float c = 1.0f + z * (-0.5f + z * (4.1666667e-2f + z * (-1.3888889e-3f + z * (2.4801587e-5f + z * -2.7557319e-7f))));
     const int quarter = (int)(k - 4.0 * floor(k * 0.25));
     const float cc = (quarter & 1) ? s : c, ss = (quarter & 1) ? c : s;
     return {factor * ((quarter == 1 || quarter == 2) ? -cc : cc), factor * ((quarter & 2) ? -ss : ss)};
+}
+
+// N neighbouring pairs' turns; the angles that are far are looked for once.
+template <int N>
+__device__ __forceinline__ void turns_of(const double position, const double *freq, const float factor, Turn (&out)[N])
+{
+    bool far = false;
+#pragma unroll
+    for (int j = 0; j < N; ++j) out[j] = turn_by<false>(position, freq[j], factor, far);
+    if (far) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) out[j] = turn_by<true>(position, freq[j], factor, far);
+    }
 }
 
 __device__ __forceinline__ double position_of(const void *positions, const int wide, const long long t)
@@ -110,11 +137,10 @@ __global__ __launch_bounds__(256) void rotary_tables_kernel(const RotaryTablesPa
     const int pair = 4 * (int)(i - t * quads);
     const double n = position_of(p.positions, p.wide, t);
     float c[4], s[4];
+    Turn turn[4];
+    turns_of(n, p.freq + pair, p.factor, turn);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const Turn a = turn_of(n, p.freq[pair + j], p.factor);
-        c[j] = a.c, s[j] = a.s;
-    }
+    for (int j = 0; j < 4; ++j) c[j] = turn[j].c, s[j] = turn[j].s;
     const long long at = t * 2 * p.pairs + pair;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -171,7 +197,9 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryParams p)
     }
     for (int i = tid; i < tokens * p.pairs; i += 256) {    // (the rows are on their way)
         const int t = i / p.pairs;
-        turns[i] = turn_of(position_of(p.positions, p.wide, t0 + t), p.freq[i - t * p.pairs], p.factor);
+        Turn turn[1];
+        turns_of(position_of(p.positions, p.wide, t0 + t), p.freq + (i - t * p.pairs), p.factor, turn);
+        turns[i] = turn[0];
     }
     __syncthreads();
     if (!there) return;

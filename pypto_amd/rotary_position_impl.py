@@ -9,7 +9,8 @@ projections: ``rotary_embedding`` rotates them, or a part of every head, in the 
 * ``"deinterleaved"``  channel 2i turns with channel 2i + 1, and the results go to i and i + pairs (the MLA prolog's).
 
 ``rotary_frequencies`` gives the radians per position of every pair, stretched for contexts longer than the trained one if asked
-for.  It is made once, on the host; angles are ``position * frequency`` in 64 bits, so far positions keep their bits.
+for.  It is made once, on the host; angles are ``position * frequency`` in 64 bits, so far positions keep their bits (angles up to 2^63 are
+reduced exactly enough for fp32).
 
 Calling convention as for the other operators: ``from_torch`` wrappers or bare torch tensors, outputs pre-allocated and written in
 place, ``None`` returned, asynchronous on the current stream.  Bare tensors may be strided (a slice of a projection's output): the

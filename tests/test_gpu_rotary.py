@@ -183,3 +183,25 @@ def test_the_series_leave_out_nothing_that_fp32_shows(which):
     for off in (even_cos, even_sin):
         assert float(off.abs().max()) <= 7.7e-8 + 2.0 ** 21 * 2.0 ** -53
         assert abs(float(off[near_border].mean())) <= 6 * 7.7e-8 * n ** -0.5 + 1e-9
+
+
+@pytest.mark.parametrize("which", ["tables", "rotation"])
+def test_positions_at_the_ends_of_64_bits(which):
+    """Angles are positions times frequencies in 64 bits, and their cosines and sines are those of that number, however far it is."""
+    freq = pypto_amd.rotary_frequencies(64, device=DEV)
+    pos = torch.tensor([2 ** 63 - 1, -2 ** 63, 2 ** 62 + 12345678901, -(10 ** 18), 10 ** 17 + 1, 2 ** 53 + 1, -(10 ** 15), 2 ** 50, 10 ** 14, 0], device=DEV)
+    pos = torch.cat([pos, torch.randint(-2 ** 62, 2 ** 62, (500,), generator=torch.Generator().manual_seed(1)).to(DEV)])
+    t = len(pos)
+    if which == "tables":
+        cos, sin = (torch.zeros(t, 64, device=DEV) for _ in range(2))
+        pypto_amd.rotary_tables(pos, freq, cos, sin)
+        cos, sin = cos[:, :32], sin[:, :32]
+    else:
+        one = torch.zeros(t, 1, 64, device=DEV)
+        one[..., :32] = 1
+        pypto_amd.rotary_embedding(one, None, pos, freq, one, None)
+        cos, sin = one[:, 0, :32], one[:, 0, 32:]
+    angle = pos.cpu().double()[:, None] * freq.cpu()
+    # the series' 2^-23; the reduction subtracts multiples of pi/2 (known to 2^-107) below 2^63, in steps below 2^12 times 2^-53
+    assert float((cos.cpu().double() - angle.cos()).abs().max()) <= 2.0 ** -22
+    assert float((sin.cpu().double() - angle.sin()).abs().max()) <= 2.0 ** -22
