@@ -448,7 +448,8 @@ int pto_mla_indexer_prolog_quant_launch(const PtoMlaIndexerPrologQuantArgs *args
 /*
  * ---- Around a prompt: rotary positions, writing and reading the latent cache, attention over whole sequences.
  * These have no counterpart among the reference's operators of this path.  Strides are in elements; a tensor's last
- * dimension is contiguous.  An empty call (no token, no row) does nothing.
+ * dimension is contiguous.  An empty call (no token, no row) does nothing.  Memory that is written is nothing else of the call, neither
+ * another output nor an input, positions, tables and indices among them, but where it is said; these entries do not look for that.
  */
 
 #define PTO_ROPE_HALF 0           /* pairs (i, i + pairs)                                              */

@@ -407,6 +407,14 @@ bool clash(const at::Tensor &out, const at::Tensor &in, const bool where_same = 
     return a < b + bytes(in, 0) && b < a + bytes(out, 0);
 }
 
+// whether a written tensor meets any of these
+bool clash_any(const at::Tensor &out, std::initializer_list<const at::Tensor *> others)
+{
+    for (const at::Tensor *t : others)
+        if (clash(out, *t)) return true;
+    return false;
+}
+
 template <typename Args, typename Launch>
 PyObject *enqueue_without_workspace(const c10::Device &device, const Args &a, Launch launch)
 {
@@ -416,10 +424,11 @@ PyObject *enqueue_without_workspace(const c10::Device &device, const Args &a, La
     Py_RETURN_TRUE;
 }
 
-// positions [t] int64 or int32, frequencies [pairs] fp64
-bool turns_of(Call &c, const int at, const void *&positions, const double *&frequencies, int64_t &t, int64_t &pairs, int32_t &wide)
+// positions [t] int64 or int32, frequencies [pairs] fp64; from: the two tensors
+bool turns_of(Call &c, const int at, const at::Tensor *(&from)[2], const void *&positions, const double *&frequencies, int64_t &t, int64_t &pairs, int32_t &wide)
 {
     const at::Tensor &pos = c.tensor(at), &freq = c.of(at + 1, at::kDouble);
+    from[0] = &pos, from[1] = &freq;
     if (!c.ok || !dims(pos, 1) || !dims(freq, 1) || (pos.scalar_type() != I64 && pos.scalar_type() != I32)) return false;
     positions = c.ptr<void>(pos), frequencies = c.ptr<double>(freq);
     t = pos.size(0), pairs = freq.size(0), wide = pos.scalar_type() == I64;
@@ -434,10 +443,11 @@ PyObject *rotary_tables_call(PyObject *, PyObject *const *args, Py_ssize_t n)
         Call c{args};
         PtoRotaryTablesArgs a{};
         a.factor = c.real(4);
-        if (!turns_of(c, 0, a.positions, a.frequencies, a.t, a.pairs, a.positions_int64)) return declined();
+        const at::Tensor *from[2];
+        if (!turns_of(c, 0, from, a.positions, a.frequencies, a.t, a.pairs, a.positions_int64)) return declined();
         const at::Tensor &cos = c.tensor(2), &sin = c.tensor(3);
         if (!c.ok || !dims(cos, 2) || cos.size(0) != a.t || cos.size(1) != 2 * a.pairs || sin.sizes() != cos.sizes() || sin.scalar_type() != cos.scalar_type() ||
-            clash(cos, sin))
+            clash_any(cos, {&sin, from[0], from[1]}) || clash_any(sin, {from[0], from[1]}))
             return declined();
         a.dtype = dtype_code(cos, c.ok);
         a.cos = c.out<void>(cos), a.sin = c.out<void>(sin);
@@ -454,8 +464,8 @@ PyObject *rotary_embedding_call(PyObject *, PyObject *const *args, Py_ssize_t n)
         Call c{args};
         PtoRotaryArgs a{};
         a.layout = static_cast<int32_t>(c.integer(6)), a.factor = c.real(9);
-        if (!turns_of(c, 2, a.positions, a.frequencies, a.t, a.pairs, a.positions_int64) || c.none(1) != c.none(5)) return declined();
-        const at::Tensor *seen[4];
+        const at::Tensor *seen[4], *from[2];
+        if (!turns_of(c, 2, from, a.positions, a.frequencies, a.t, a.pairs, a.positions_int64) || c.none(1) != c.none(5)) return declined();
         const int sides = c.none(1) ? 1 : 2;
         for (int k = 0; k < sides; ++k) {
             PtoRotaryTensor &r = k == 0 ? a.query : a.key;
@@ -469,7 +479,7 @@ PyObject *rotary_embedding_call(PyObject *, PyObject *const *args, Py_ssize_t n)
             r.heads = heads_of(in), r.dim = in.size(-1), r.offset = c.integer(7 + k);
             r.in_stride_t = row_stride(in), r.in_stride_h = head_stride(in), r.out_stride_t = row_stride(out), r.out_stride_h = head_stride(out);
             seen[k] = &in, seen[2 + k] = &out;
-            if (clash(out, in, false)) return declined();
+            if (clash(out, in, false) || clash_any(out, {from[0], from[1]})) return declined();
         }
         if (sides == 2 && (clash(*seen[2], *seen[1]) || clash(*seen[3], *seen[0]) || clash(*seen[2], *seen[3]))) return declined();
         for (int k = 0; k < sides; ++k) {
@@ -514,10 +524,12 @@ PyObject *cache_write_call(PyObject *, PyObject *const *args, Py_ssize_t n)
             return declined();
         a.t = latent.size(0), a.latent_stride = row_stride(latent), a.rope_stride = row_stride(rope);
         for (const at::Tensor *p : parts)
-            if (p && (clash(*p, latent) || clash(*p, rope))) return declined();
+            if (p && clash_any(*p, {&latent, &rope, &index})) return declined();
+        if (!a.packed && (clash_any(*parts[0], {parts[1], parts[2]}) || clash(*parts[1], *parts[2]))) return declined();
         if (!c.none(6)) {
             const at::Tensor &values = c.rows_of(6, BF16, 512);
-            if (!c.ok || values.sizes() != latent.sizes() || !writable(values) || clash(values, latent, type != BF16) || clash(values, rope)) return declined();
+            if (!c.ok || values.sizes() != latent.sizes() || !writable(values) || clash(values, latent, type != BF16) || clash_any(values, {&rope, &index}))
+                return declined();
             for (const at::Tensor *p : parts)
                 if (p && clash(*p, values)) return declined();
             a.values = c.out<void>(values), a.values_stride = row_stride(values);
@@ -546,7 +558,12 @@ PyObject *cache_read_call(PyObject *, PyObject *const *args, Py_ssize_t n)
         a.b = bt.size(0), a.max_blocknum_perbatch = bt.size(1), a.rows = latent.size(0);
         for (const at::Tensor *p : parts)
             if (p && (clash(latent, *p) || clash(rope, *p))) return declined();
-        if (!c.none(5)) a.first = c.ptr<int32_t>(c.shaped(5, I32, {a.b}));
+        if (clash_any(latent, {&bt, &cu}) || clash_any(rope, {&bt, &cu})) return declined();
+        if (!c.none(5)) {
+            const at::Tensor &first = c.shaped(5, I32, {a.b});
+            if (!c.ok || clash(latent, first) || clash(rope, first)) return declined();
+            a.first = c.ptr<int32_t>(first);
+        }
         a.nope = c.ptr<void>(*parts[0]);
         if (!a.packed) a.rope_cache = c.ptr<void>(*parts[1]), a.scales = c.ptr<void>(*parts[2]);
         a.block_table = c.ptr<int32_t>(bt), a.cu_seqlens = c.ptr<int32_t>(cu);
@@ -575,7 +592,7 @@ PyObject *prompt_attention_call(PyObject *, PyObject *const *args, Py_ssize_t n)
         a.d = q.size(2);
         c.rows_of(0, type);
         const at::Tensor &k = c.rows_of(1, type, a.d), &v = c.rows_of(2, type, a.d), &out = c.rows_of(5, type, a.d);
-        if (!c.ok || !dims(k, 3) || k.sizes() != v.sizes() || out.sizes() != q.sizes() || !writable(out) || clash(out, q) || clash(out, k) || clash(out, v) ||
+        if (!c.ok || !dims(k, 3) || k.sizes() != v.sizes() || out.sizes() != q.sizes() || !writable(out) || clash_any(out, {&q, &k, &v, &cu_q, &cu_k}) ||
             c.none(7) != c.none(8))
             return declined();
         a.fp16 = type == FP16;
@@ -593,7 +610,7 @@ PyObject *prompt_attention_call(PyObject *, PyObject *const *args, Py_ssize_t n)
         }
         if (!c.none(9)) {
             const at::Tensor &lse = c.shaped(9, FP32, {a.total_q, a.heads});
-            if (!c.ok || clash(lse, out) || clash(lse, q) || clash(lse, k) || clash(lse, v)) return declined();
+            if (!c.ok || clash_any(lse, {&out, &q, &k, &v, &cu_q, &cu_k})) return declined();
             if (!c.none(7) && (clash(lse, c.tensor(7, true)) || clash(lse, c.tensor(8, true)))) return declined();
             a.lse = c.out<float>(lse);
         }

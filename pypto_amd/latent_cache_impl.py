@@ -67,6 +67,9 @@ def _write(op, latent, key_rope, cache_index, parts, names, latent_out, prolog_s
     for c, n in zip(cache, names):
         refuse_overlap(c, lat, f"{n} and latent")
         refuse_overlap(c, rope, f"{n} and key_rope")
+        refuse_overlap(c, idx, f"{n} and cache_index")
+    for i, j in ((0, 1), (0, 2), (1, 2)) if len(cache) == 3 else ():
+        refuse_overlap(cache[i], cache[j], f"{names[i]} and {names[j]}")
     tensors = [lat, rope, idx] + cache
     values = None
     if latent_out is not None:
@@ -75,6 +78,7 @@ def _write(op, latent, key_rope, cache_index, parts, names, latent_out, prolog_s
         if lat.dtype != values.dtype or not same_rows(values, lat):
             refuse_overlap(values, lat, "latent_out and latent")
         refuse_overlap(values, rope, "latent_out and key_rope")
+        refuse_overlap(values, idx, "latent_out and cache_index")
         for c, n in zip(cache, names):
             refuse_overlap(values, c, f"latent_out and {n}")
         tensors.append(values)
@@ -129,6 +133,8 @@ def _read(op, parts, names, block_table, cu_seqlens, latent_out, key_rope_out, b
         check_writable(t, n)
         for c, m in zip(cache, names):
             refuse_overlap(t, c, f"{n} and {m}")
+        for i, m in ints:
+            refuse_overlap(t, i, f"{n} and {m}")
     refuse_overlap(latent, rope, "latent_out and key_rope_out")
     _on_gpu(op, cache + [t for t, _ in ints] + [latent, rope])
     if not C.cache_read_call(*(cache + [None] * (3 - len(cache))), bt, cu, start, latent, rope, int(block_size)):

@@ -69,7 +69,7 @@ def prompt_attention(query, key, value, cu_seqlens_q, cu_seqlens_k, attention_ou
         raise ValueError(f"heads must be a multiple of kv_heads, got {heads} and {kv_heads}")
     if (query_rope is None) != (key_rope is None):
         raise ValueError("query_rope and key_rope come together")
-    inputs = [(q, "query"), (k, "key"), (v, "value")]
+    inputs = [(q, "query"), (k, "key"), (v, "value"), (cu_q, "cu_seqlens_q"), (cu_k, "cu_seqlens_k")]
     qr = kr = lse = None
     if query_rope is not None:
         qr, kr = as_rows(query_rope, "query_rope"), as_rows(key_rope, "key_rope")
@@ -97,7 +97,7 @@ def prompt_attention(query, key, value, cu_seqlens_q, cu_seqlens_k, attention_ou
         refuse_overlap(out, t, f"attention_out and {n}")
     if not math.isfinite(float(softmax_scale)):
         raise ValueError("softmax_scale is not finite")
-    _on_gpu("prompt_attention", [t for t, _ in inputs] + [cu_q, cu_k, out] + ([lse] if lse is not None else []))
+    _on_gpu("prompt_attention", [t for t, _ in inputs] + [out] + ([lse] if lse is not None else []))
     if not C.prompt_attention_call(q, k, v, cu_q, cu_k, out, float(softmax_scale), qr, kr, lse, bool(causal)):
         raise RuntimeError("prompt_attention: these arguments are not supported")
     return None

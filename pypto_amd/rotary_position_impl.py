@@ -109,6 +109,9 @@ def rotary_tables(positions, frequencies, cos_out, sin_out, factor=1.0):
         if tuple(t.shape) != (pos.shape[0], 2 * freq.shape[0]):
             raise ValueError(f"{name}: expected shape {(pos.shape[0], 2 * freq.shape[0])}, got {tuple(t.shape)}")
     refuse_overlap(cos, sin, "cos_out and sin_out")
+    for t, name in ((cos, "cos_out"), (sin, "sin_out")):
+        refuse_overlap(t, pos, f"{name} and positions")
+        refuse_overlap(t, freq, f"{name} and frequencies")
     _on_gpu("rotary_tables", (pos, freq, cos, sin))
     if not C.rotary_tables_call(pos, freq, cos, sin, float(factor)):
         raise RuntimeError("rotary_tables: these arguments are not supported")
@@ -145,6 +148,8 @@ def rotary_embedding(query, key, positions, frequencies, query_out, key_out, lay
         check_writable(out, f"{name}_out")
         if not same_rows(x, out):
             refuse_overlap(out, x, f"{name} and {name}_out")
+        refuse_overlap(out, pos, f"{name}_out and positions")
+        refuse_overlap(out, freq, f"{name}_out and frequencies")
     if len(sides) == 2:
         (_, q, qo, _), (_, k, ko, _) = sides
         refuse_overlap(qo, k, "query_out and key")

@@ -82,3 +82,42 @@ def test_a_prompt_in_two_chunks_and_the_sparse_attention_over_its_cache(packed):
     through = torch.einsum("thl,hcl->thc", sparse[:, 0].float(), w_uv.float())
     assert total == sum(o.shape[0] for o in outs)
     assert relative(through, torch.stack([o[-1] for o in outs])) <= 0.03
+
+
+def test_outputs_in_the_memory_of_positions_tables_and_indices_are_refused():
+    """Nothing is launched, whichever output and index meet."""
+    z = lambda *s, dtype=BF: torch.zeros(s, dtype=dtype, device=DEV)  # noqa: E731
+    within = lambda t, dtype, *s: t.reshape(-1).view(dtype)[:torch.Size(s).numel()].view(s)  # noqa: E731
+    I32, I64, F64, I8 = torch.int32, torch.int64, torch.float64, torch.int8
+
+    def refused(op, args, at, value, **kw):
+        with pytest.raises(ValueError, match="overlap"):
+            op(*(value if i == at else x for i, x in enumerate(args)), **kw)
+
+    freq = pypto_amd.rotary_frequencies(64, device=DEV)
+    tables = [z(5, dtype=I64), freq, z(5, 64), z(5, 64)]
+    turn = [z(5, 4, 80), z(5, 1, 64), z(5, dtype=I64), freq, z(5, 4, 80), z(5, 1, 64)]
+    write = [z(3, 512), z(3, 64), z(3, dtype=I64), z(256, 512, dtype=I8), z(256, 64), z(256, 4, dtype=torch.float32), z(3, 512)]
+    read = write[3:6] + [z(2, 3, dtype=I32), z(3, dtype=I32), z(9, 512), z(9, 64), 128]
+    attend = [z(6, 4, 128), z(9, 2, 128), z(9, 2, 128), torch.tensor([0, 6], dtype=I32, device=DEV), torch.tensor([0, 9], dtype=I32, device=DEV), z(6, 4, 128), 0.1]
+    for out in (2, 3):
+        refused(pypto_amd.rotary_tables, tables, 0, within(tables[out], I64, 5))
+        refused(pypto_amd.rotary_tables, tables, 1, within(tables[out], F64, 32))
+    for out in (4, 5):
+        refused(pypto_amd.rotary_embedding, turn, 2, within(turn[out], I64, 5))
+        refused(pypto_amd.rotary_embedding, turn, 3, within(turn[out], F64, 32))
+    for out in (3, 4, 5, 6):
+        refused(pypto_amd.latent_cache_write, write, 2, within(write[out], I64, 3))
+    refused(pypto_amd.latent_cache_write, write, 4, within(write[3], BF, 256, 64))
+    refused(pypto_amd.latent_cache_write, write, 5, within(write[3], torch.float32, 256, 4))
+    refused(pypto_amd.latent_cache_write, write, 5, within(write[4], torch.float32, 256, 4))
+    for out in (5, 6):
+        refused(pypto_amd.latent_cache_read, read, 3, within(read[out], I32, 2, 3))
+        refused(pypto_amd.latent_cache_read, read, 4, within(read[out], I32, 3))
+        refused(pypto_amd.latent_cache_read, read, 9, None, first=within(read[out], I32, 2))
+    lse = z(6, 4, dtype=torch.float32)
+    for at in (3, 4):
+        refused(pypto_amd.prompt_attention, attend, at, within(attend[5], I32, 2))
+        refused(pypto_amd.prompt_attention, attend, at, within(lse, I32, 2), softmax_lse=lse)
+    for t in tables[2:] + turn[4:] + write[3:] + read[5:7] + [attend[5], lse]:
+        assert not bool(t.any())

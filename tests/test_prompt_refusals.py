@@ -261,3 +261,65 @@ def test_c_entries_say_what_they_refuse():
     assert lib.pto_prompt_attention_workspace_bytes(ctypes.byref(a), ctypes.byref(n)) == 0 and n.value % 4 == 0
     a.total_q = 0
     assert lib.pto_prompt_attention_launch(ctypes.byref(a), None) == 0                 # an empty call does nothing
+
+
+# ---------------------------------------------------------------- outputs in the memory of what says where and how much
+
+def inside(t, dtype, *shape):
+    """A tensor in the first bytes of another one."""
+    n = math.prod(shape)
+    return t.reshape(-1).view(dtype)[:n].view(shape)
+
+
+@pytest.mark.parametrize("at", [2, 3])
+def test_tables_over_positions_or_frequencies(at):
+    args = tables()
+    refused(ValueError, "positions overlap", pypto_amd.rotary_tables, changed(args, 0, inside(args[at], torch.int64, 5)))
+    refused(ValueError, "frequencies overlap", pypto_amd.rotary_tables, changed(args, 1, inside(args[at], torch.float64, 32)))
+
+
+@pytest.mark.parametrize("at", [4, 5])
+def test_rotation_over_positions_or_frequencies(at):
+    args = rotation()
+    refused(ValueError, "positions overlap", pypto_amd.rotary_embedding, changed(args, 2, inside(args[at], torch.int64, 5)))
+    refused(ValueError, "frequencies overlap", pypto_amd.rotary_embedding, changed(args, 3, inside(args[at], torch.float64, 32)))
+    args[at - 4] = args[at]                                        # (in place too)
+    refused(ValueError, "positions overlap", pypto_amd.rotary_embedding, changed(args, 2, inside(args[at], torch.int64, 5)))
+
+
+@pytest.mark.parametrize("at", [3, 4, 5, 6])
+def test_write_over_the_cache_index(at):
+    args = write()
+    refused(ValueError, "cache_index overlap", pypto_amd.latent_cache_write, changed(args, 2, inside(args[at], torch.int64, 3)))
+    if at in (3, 6):
+        packed = [torch.zeros(256, 656, dtype=torch.int8), args[6]]
+        refused(ValueError, "cache_index overlap", pypto_amd.latent_cache_write_packed, args[:2] + [inside(packed[at // 6], torch.int64, 3)] + packed)
+
+
+def test_write_to_arrays_of_a_cache_in_one_memory():
+    one = torch.zeros(256 * (512 + 128 + 16), dtype=torch.int8)
+    cut = lambda at, width, dtype: one[at:at + 256 * width].view(dtype).view(256, -1)  # noqa: E731
+    parts = [cut(0, 512, torch.int8), cut(256 * 512, 128, BF), cut(256 * 640, 16, F32)]
+    args = write()
+    refused(RuntimeError, "GPU", pypto_amd.latent_cache_write, args[:3] + parts)           # side by side they do not meet
+    for i, (at, width, dtype) in enumerate(((1024, 512, torch.int8), (256 * 512 - 128, 128, BF), (256 * 640 - 16, 16, F32))):
+        refused(ValueError, "overlap", pypto_amd.latent_cache_write, changed(args[:3] + parts, 3 + i, cut(at, width, dtype)))
+
+
+@pytest.mark.parametrize("at", [5, 6])
+def test_read_over_the_tables(at):
+    args = read()
+    refused(ValueError, "block_table overlap", pypto_amd.latent_cache_read, changed(args, 3, inside(args[at], torch.int32, 2, 3)))
+    refused(ValueError, "cu_seqlens overlap", pypto_amd.latent_cache_read, changed(args, 4, inside(args[at], torch.int32, 3)))
+    refused(ValueError, "first overlap", pypto_amd.latent_cache_read, args, first=inside(args[at], torch.int32, 2))
+    refused(ValueError, "first overlap", pypto_amd.latent_cache_read_packed, [torch.zeros(256, 656, dtype=torch.int8)] + args[3:],
+            first=inside(args[at], torch.int32, 2))
+
+
+def test_attention_over_the_beginnings_of_sequences():
+    args = attention()
+    lse = torch.zeros(6, 4)
+    refused(ValueError, "cu_seqlens_q overlap", pypto_amd.prompt_attention, changed(args, 3, inside(args[5], torch.int32, 2)))
+    refused(ValueError, "cu_seqlens_k overlap", pypto_amd.prompt_attention, changed(args, 4, inside(args[5], torch.int32, 2)))
+    refused(ValueError, "cu_seqlens_q overlap", pypto_amd.prompt_attention, changed(args, 3, inside(lse, torch.int32, 2)), softmax_lse=lse)
+    refused(ValueError, "cu_seqlens_k overlap", pypto_amd.prompt_attention, changed(args, 4, inside(lse, torch.int32, 2)), softmax_lse=lse)
