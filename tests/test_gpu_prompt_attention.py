@@ -338,3 +338,53 @@ def test_replays_with_other_lengths_and_on_two_streams_at_once():
         torch.cuda.synchronize()
         for c in calls:
             c.check()
+
+
+def plan_and_items(c, heads, kv, d, rope):
+    """The call's plan, and how many (key head, row tile, piece of its keys) there are for its workgroups."""
+    from pypto_amd import _C
+    plan = _C.prompt_attention_plan(len(c.lens_q), sum(c.lens_q), sum(c.lens_k), heads, kv, d, rope, c.causal)
+    pieces = [min(max(-(-k // plan["split_keys"]), 1), plan["key_splits"]) for k in c.lens_k]
+    return plan, kv * sum(-(-q * (heads // kv) // plan["rows_per_workgroup"]) * n for q, n in zip(c.lens_q, pieces))
+
+
+@pytest.mark.parametrize("d,rope,rows,heads,kv,causal,lens_q,lens_k", [
+    (64, False, 128, 32, 16, True, [1236, 460, 345, 641], [9255, 1733, 564, 5608]),
+    (128, False, 128, 64, 32, False, [52, 578, 26, 102], [1365, 11556, 126, 1256]),
+    (128, True, 128, 32, 32, True, [2, 2, 2, 2, 1, 2, 2, 2, 2, 2, 2, 1, 1, 2, 1, 1, 1, 2, 1],
+     [2876, 2377, 2364, 2929, 1586, 2645, 2547, 646, 163, 2416, 2907, 646, 1798, 214, 1816, 2506, 569, 215, 1391]),
+    (128, False, 256, 128, 16, False, [91, 34, 532], [2089, 1245, 5243]),
+    (128, True, 256, 128, 16, True, [100, 612], [912, 4692])])
+def test_workgroups_that_take_a_second_item(d, rope, rows, heads, kv, causal, lens_q, lens_k):
+    """More items of a divided launch than workgroups: one that has written its results begins anew, over the LDS that they came through."""
+    c = Call(lens_q, lens_k, heads, kv, d, rope, causal=causal, seed=30)
+    plan, items = plan_and_items(c, heads, kv, d, rope)
+    assert plan["key_splits"] > 1 and plan["rows_per_workgroup"] == rows and items > 1.05 * plan["workgroups"]
+    c.run().check()
+    first = c.out.clone(), c.lse.clone()
+    c.out.fill_(3.0)
+    c.run()
+    assert torch.equal(c.out, first[0]) and torch.equal(c.lse, first[1])
+
+
+@pytest.mark.parametrize("d,rope,tiles", [(128, False, 33), (128, True, 30), (64, False, 50)])
+def test_second_items_beyond_the_first_64_sequences(d, rope, tiles):
+    """Sequences are looked through 64 at a time, from the first on for every item."""
+    lens_k = [64 * tiles + 5] * 65
+    for i in range(4):
+        lens_k[7 * i + 3] = 60
+    c = Call([1] * 65, lens_k, 11, 11, d, rope, seed=31)
+    plan, items = plan_and_items(c, 11, 11, d, rope)
+    assert plan["key_splits"] > 1 and items > plan["workgroups"]
+    c.run().check()
+
+
+@pytest.mark.parametrize("d,rope", FORMS)
+@pytest.mark.parametrize("causal", [True, False])
+def test_divided_keys_of_more_than_64_sequences(d, rope, causal):
+    lens_k = [(i * i * 37) % 5000 + 2000 * (i % 3) for i in range(150)]
+    lens_q = [(i * 5) % 4 for i in range(150)]
+    c = Call(lens_q, lens_k, 8, 4, d, rope, causal=causal, seed=32, spare=2)
+    plan, _ = plan_and_items(c, 8, 4, d, rope)
+    assert plan["key_splits"] > 1 and min(lens_k) < plan["split_keys"] < max(lens_k)
+    c.run().check()
