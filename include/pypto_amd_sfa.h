@@ -592,7 +592,8 @@ int pto_cache_read_launch(const PtoCacheReadArgs *args, void *hip_stream);
  * Head h uses key head h / (heads / kv_heads).  s = softmax_scale * (q . k + q_rope . k_rope).  causal: the last query of a
  * sequence sees all of its keys, each one before it one key less; otherwise every query sees all keys.  Rows that see no key are
  * zeros, their lse -infinity; query rows of no sequence stay as they were.  Keys and values of rows past a sequence's last are
- * not looked at.  The values of a sequence's keys that a row does not see have to be finite.
+ * not looked at.  The values of a sequence's keys that a row does not see have to be finite.  Scores (before the scale and after it) are
+ * summed in fp32: what stays below 1e38 in magnitude is exact to its roundings; with a scale of zero, what stays below 1e31.
  * Beginnings outside the tensors are moved into them.
  *
  * Constraints: d 64 or 128, rope parts with d 128 only; heads a multiple of kv_heads; strides of 64 key rows below 4 GiB.

@@ -12,11 +12,14 @@
 // The rope part of queries and keys is a separate product over 64 more channels, whose keys all heads may share: nothing is
 // concatenated in memory.
 //
-// Bound by the matrix cores, and under them by power: 256 rows and 64 keys of 128 + 64 channels are 1280 clocks of products on each of
-// the four SIMDs, and a tile takes them two phases of 1480 (products of one half of the waves beside 1080 clocks of softmax and 530 of requests of
-// the other), at 1.6 of 2.4 GHz.  4096 causal tokens of 128 heads, bf16: 637 us, 1080 TFLOP/s of the products that the mask asks for; a
-// product of 8192^3 reaches 1330.  Of what is above it 6 % are the halves of tiles that the mask cuts off, 10 % workgroups' beginnings and
-// ends, the rest the waits of phases for the longer half.  On the way: one phase, every wave products and softmax in turn 732 us; two
+// Bound by the longer of a tile's two phases, which is the softmax and the requests.  32 rows and 64 keys of 128 + 64 channels are 1280 clocks of
+// products to a wave, 2560 on a SIMD, whose two waves take turns; a tile takes 3250, two phases of 1625: 1080 clocks of softmax and 530 of
+// requests of one half of the waves beside 1490 (the products and their operands' way) of the other.  Without rope parts 2900 for 2048 of
+// products, phases of the same softmax and requests beside 1170.  4096 causal tokens of 128 heads, bf16: 637 to 690 us, 1080 to 1000 TFLOP/s of the
+// products that the mask asks for; a product of 8192^3 reaches 1330.  Where its time goes (clocks read by two waves of each workgroup): 15 %
+// of the compute units' time is without a workgroup, between two and at the launch's end, 11 % are workgroups' beginnings (11900 clocks) and ends (4250 of 127000),
+// and of the 74 % in the loop products are 0.79: 0.58 in all, where the counters say 0.54, since of a sequence's last tiles some waves multiply
+// nothing.  The shader clock is at 1.8 of 2.4 GHz meanwhile.  On the way: one phase, every wave products and softmax in turn 732 us; two
 // phases, two stages of tiles, requests among the products 675; three stages, requests before the softmax 670 at fewer clocks; queries and
 // results by whole cache lines 637.  Not kept: workgroups that stay and draw their work from counters (1 % slower here, 3 % faster for nine
 // ragged sequences, 7 % slower where keys are divided).
@@ -450,7 +453,7 @@ __global__ __launch_bounds__(64 * W, 2) void prompt_attention_kernel(const PaPar
             asm volatile("" ::: "memory");
             read_queries();
             // Scores are scaled inside the exponent.  That wants a positive scale: the sign of a negative one moves into Q^T, and a zero one
-            // becomes the smallest normal number, under which every finite score scales to the same probabilities.
+            // becomes the smallest normal number, under which scores up to 1e31 scale to the same probabilities (2^-23 apart).
             if (scale < 0.f) {
                 scale = -scale;
 #pragma unroll
