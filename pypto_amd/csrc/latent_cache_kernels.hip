@@ -2,7 +2,8 @@
 //
 // A row is 512 int8 codes, one fp32 scale to 128 of them, and 64 bf16 rope channels.  Of a group v of 128 channels
 //   steps = 127 * (1 / max |v|), code = rint(v * steps), scale = 1 / steps, value = bf16(code * scale),
-// each an IEEE fp32 operation; the values are those that the attention multiplies.  A caller whose rows are to be those that the MLA
+// each an IEEE fp32 operation; the values are those that the attention multiplies.  (In this order torch evaluates 127 / max, so codes
+// equal those of the rule written in torch.)  A caller whose rows are to be those that the MLA
 // prolog writes asks for its steps, 127 / max in one rounding.  (20000 rows of normally distributed latents: 22 % of the scales differ
 // between the two, by a bit or two, and of 10000 codes 3.9 in bf16, 0.9 in fp16, 0.01 in fp32, by one step; in bf16 one row in six holds
 // such a code.  Codes of exact quotients are missed by 5.8 and 4.5 of 10000 in bf16.)  Both directions move bytes and nothing else bounds

@@ -205,3 +205,20 @@ def test_positions_at_the_ends_of_64_bits(which):
     # the series' 2^-23; the reduction subtracts multiples of pi/2 (known to 2^-107) below 2^63, in steps below 2^12 times 2^-53
     assert float((cos.cpu().double() - angle.cos()).abs().max()) <= 2.0 ** -22
     assert float((sin.cpu().double() - angle.sin()).abs().max()) <= 2.0 ** -22
+
+
+@pytest.mark.parametrize("in_place", [True, False])
+def test_offsets_past_32_bits(in_place):
+    """Tokens 128 KiB apart: the last ones lie more than 8 GiB behind the first."""
+    t = 70000
+    freq = pypto_amd.rotary_frequencies(64, device=DEV)
+    pos = positions_of(t, 131071, seed=12)
+    x = torch.empty(t, 1, 65536, dtype=BF, device=DEV)[:, :, 100:164]
+    x.copy_(normal((t, 1, 64), BF, 13))
+    was = x.contiguous()
+    out = x if in_place else torch.zeros_like(was)
+    pypto_amd.rotary_embedding(x, None, pos, freq, out, None, layout="interleaved")
+    near(out.contiguous(), was, pos, freq, "interleaved", 0, 1.0)
+    if not in_place:
+        pypto_amd.rotary_embedding(was, None, pos, freq, x, None, layout="interleaved")      # (written that far away, too)
+        assert torch.equal(x, out)
