@@ -643,6 +643,135 @@ typedef struct PtoPromptPlan {
 int pto_prompt_attention_plan(const PtoPromptAttentionArgs *args, PtoPromptPlan *plan);
 int pto_prompt_attention_launch(const PtoPromptAttentionArgs *args, void *hip_stream);
 
+/*
+ * The same with a window (prompt.causal has to be set): of the keys up to its own a query sees the last `window` and the first `sinks`.
+ * Keys are counted within the sequence, so keys between those that no query sees may as well be left out of it, if the first
+ * `sinks` and at least the last (queries - 1 + window) are there.
+ *
+ * Constraints: window in [1, 2^30], sinks in [0, 2^30].
+ */
+typedef struct PtoPromptWindowArgs {
+    PtoPromptAttentionArgs prompt;
+    int64_t window;
+    int64_t sinks;
+} PtoPromptWindowArgs;
+
+int pto_prompt_window_workspace_bytes(const PtoPromptWindowArgs *args, size_t *bytes);
+int pto_prompt_window_launch(const PtoPromptWindowArgs *args, void *hip_stream);
+
+/*
+ * Pages of the cache for sequences that grow and shrink: sequence i's pages hold lens_before[i] tokens and shall hold lens_after[i],
+ * each page block_size, up to max_blocknum_perbatch of them.
+ *
+ *   lens_before, lens_after [b] int32;  block_table [b, max_blocknum_perbatch] int32, written where sequences grow
+ *   free_pages [room] int32: a stack of free pages, the first free_count[0] of them;  free_left [1] int32 receives how many there are
+ *                afterwards (it may be free_count itself)
+ *
+ * First the pages behind lens_after go onto the stack, in the order of the sequences and of their blocks (entries below zero are no pages and do
+ * not; what the stack has no room for is dropped); their entries in the table stay.  Then sequences that grow take pages from its top in the
+ * same order; where none are left their entries become -1, which the other operators take for no page.  Lengths below zero count as zero.
+ */
+typedef struct PtoCachePagesArgs {
+    const int32_t *lens_before;
+    const int32_t *lens_after;
+    int32_t *block_table;
+    int32_t *free_pages;
+    const int32_t *free_count;
+    int32_t *free_left;
+    int64_t b;
+    int64_t max_blocknum_perbatch;
+    int64_t block_size;
+    int64_t room;
+} PtoCachePagesArgs;
+
+int pto_cache_pages_launch(const PtoCachePagesArgs *args, void *hip_stream);
+
+/*
+ * What a step's operators take, from lengths: sequence i has query_lens[i] new tokens, the last of its seq_lens[i].
+ *
+ *   query_lens, seq_lens [b] int32;  block_table [b, max_blocknum_perbatch] int32
+ *   cu_seqlens_q [b + 1] int32, cu_seqlens_k [b + 1] int32 or NULL: sums of query_lens and of seq_lens (no more than 2^31 - 1)
+ *   positions, cache_index [t] int64: a token's position, and its row of the cache, -1 where the table holds no page for it
+ *   parents [t] int32 and tree_mask [t, mask_words] int64, or NULL both: a sequence's new tokens are a tree; a token's parent by its
+ *                number within the sequence's new tokens, lower than its own (anything else: none).  Row r of a sequence is then at
+ *                position seq_len - query_len + its depth, and bit j % 64 of word j / 64 of its mask says whether it is node j or
+ *                hangs on it, for nodes below 64 * mask_words.  cache_index is by the token's number, not by its depth.
+ *
+ * Tokens of no sequence get position 0, cache row -1 and an empty mask.  Lengths below zero count as zero.  mask_words up to 16.
+ */
+typedef struct PtoCacheSlotsArgs {
+    const int32_t *query_lens;
+    const int32_t *seq_lens;
+    const int32_t *block_table;
+    int32_t *cu_seqlens_q;
+    int32_t *cu_seqlens_k;
+    int64_t *positions;
+    int64_t *cache_index;
+    const int32_t *parents;
+    int64_t *tree_mask;
+    int64_t b;
+    int64_t t;
+    int64_t max_blocknum_perbatch;
+    int64_t block_size;
+    int64_t mask_words;
+} PtoCacheSlotsArgs;
+
+int pto_cache_slots_launch(const PtoCacheSlotsArgs *args, void *hip_stream);
+
+/*
+ * Attention over the cached latents of whole sequences, in the absorbed form: s = softmax_scale * (q_nope . k + q_rope . k_rope), the
+ * values being the 512 latent channels, bf16(code * scale).
+ *
+ *   query_nope [total_q, heads, 512], query_rope [total_q, heads, 64] bf16
+ *   nope, rope_cache, scales   the three arrays of PtoSfaQuantArgs, or packed: nope alone, the other two NULL
+ *   block_table [b, max_blocknum_perbatch] int32;  cu_seqlens_q [b + 1] int32, ascending;  seq_lens [b] int32: keys of a sequence, its
+ *                query tokens' among them, which are the last
+ *   tree_mask [total_q, mask_words] int64 or NULL
+ *   out [total_q, heads, 512] bf16;  lse [total_q, heads] fp32 or NULL: the natural logarithm of the sum of exp of a row's scores
+ *
+ * Without a mask a token sees the keys up to its own; with a window > 0 of these the last `window` and the first `sinks`.  With a mask it sees
+ * the keys before the sequence's query tokens and, of theirs, key j where bit j % 64 of word j / 64 of its mask is set.  Rows that see no key are
+ * zeros, their lse -infinity; rows of no sequence stay as they were.  Keys that a row does not see may hold anything, infinite scales too.
+ * Positions without a page (an entry below zero, or a page outside the cache) read as zeros, as latents and as rope; keys that the table is too
+ * short for do not exist.  Beginnings outside the queries are moved into them.
+ *
+ * Constraints: total_q * heads below 2^31 - 65536; mask_words up to 16, not together with a window.  Alignment: queries 16 bytes, their strides
+ * multiples of 8 elements; cache arrays 16 bytes; the others their element's.  The workspace holds partial results: launches that may run at the
+ * same time must not share it.
+ */
+typedef struct PtoLatentAttentionArgs {
+    const void *query_nope;
+    const void *query_rope;
+    const void *nope;
+    const void *rope_cache;
+    const void *scales;
+    const int32_t *block_table;
+    const int32_t *cu_seqlens_q;
+    const int32_t *seq_lens;
+    const int64_t *tree_mask;
+    void *out;
+    float *lse;
+    void *workspace;
+    size_t workspace_bytes;
+    int64_t b;
+    int64_t total_q;
+    int64_t heads;
+    int64_t cache_rows;
+    int64_t block_size;
+    int64_t max_blocknum_perbatch;
+    int64_t query_nope_stride_t, query_nope_stride_h;
+    int64_t query_rope_stride_t, query_rope_stride_h;
+    int64_t out_stride_t, out_stride_h;
+    int64_t window;
+    int64_t sinks;
+    int64_t mask_words;
+    float softmax_scale;
+    int32_t packed;
+} PtoLatentAttentionArgs;
+
+int pto_latent_attention_workspace_bytes(const PtoLatentAttentionArgs *args, size_t *bytes);
+int pto_latent_attention_launch(const PtoLatentAttentionArgs *args, void *hip_stream);
+
 /* Thread-local description of the last error on this thread ("" if none). */
 const char *pto_last_error(void);
 

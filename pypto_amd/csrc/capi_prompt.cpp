@@ -99,7 +99,7 @@ int attention_check(const PtoPromptAttentionArgs *a)
 }
 
 struct PromptPlan {
-    int splits, split_tiles, waves;
+    int splits, split_tiles, waves, most_tiles;
     long long workgroups;
     size_t o_bytes, ml_bytes;
 };
@@ -126,16 +126,24 @@ struct PromptPlan {
 // could be more than four for each compute unit, the workgroups of a divided launch take the pieces there are in turn.
 constexpr size_t PA_MOST_PARTIALS = (size_t)256 << 20;
 
-PromptPlan attention_plan(const PtoPromptAttentionArgs *a)
+// A window bounds the tiles of any row tile: those of the first keys, those that the windows of its tokens reach over, and one more where these
+// begin inside a tile.  The plan then takes a sequence for no longer.
+PromptPlan attention_plan(const PtoPromptAttentionArgs *a, const int64_t window, const int64_t sinks)
 {
     PromptPlan pl{};
     const long long cus = cu_count() > 0 ? cu_count() : 256;
     const long long rows = a->total_q * (a->heads / a->kv_heads);
-    const long long key_tiles = (a->total_k + pto::PA_KEYS - 1) / pto::PA_KEYS;             // of one sequence, at most
+    long long key_tiles = (a->total_k + pto::PA_KEYS - 1) / pto::PA_KEYS;                   // of one sequence, at most
     pl.splits = 1;
     const bool few = 2 * (rows / 256 + a->b) * a->kv_heads <= cus && a->total_k <= 4096 * a->b;
     pl.waves = a->d == 64 || rows < 512 * a->b || few ? 4 : 8;
     const int wg_rows = pl.waves * pto::PA_WAVE_ROWS;
+    pl.most_tiles = 1 << 30;
+    if (window > 0) {
+        const long long reach = window + (wg_rows - 2) / (a->heads / a->kv_heads) + 1;
+        pl.most_tiles = (int)((sinks + pto::PA_KEYS - 1) / pto::PA_KEYS + (reach + pto::PA_KEYS - 1) / pto::PA_KEYS + 1);
+        key_tiles = key_tiles < pl.most_tiles ? key_tiles : pl.most_tiles;
+    }
     const long long slots = pl.waves == 4 ? 2 * cus : cus;                                  // workgroups at a time
     const long long most_tiles = rows / wg_rows + a->b;                                     // of a key head
     pl.split_tiles = 1 << 24;
@@ -143,8 +151,8 @@ PromptPlan attention_plan(const PtoPromptAttentionArgs *a)
 
     const double seq_rows = (double)rows / a->b;
     const double items = (seq_rows <= wg_rows ? (double)a->b : (double)rows / wg_rows + (a->b > 1 ? 0.5 * a->b : 0.0)) * a->kv_heads;
-    const double longest = std::ceil((double)a->total_k / a->b / pto::PA_KEYS);
-    const double mean = a->causal && a->total_k >= a->total_q ? ((double)a->total_k - 0.5 * a->total_q) / a->b / pto::PA_KEYS : longest;
+    const double longest = std::fmin(std::ceil((double)a->total_k / a->b / pto::PA_KEYS), pl.most_tiles);
+    const double mean = a->causal && a->total_k >= a->total_q ? std::fmin(((double)a->total_k - 0.5 * a->total_q) / a->b / pto::PA_KEYS, longest) : longest;
     if (items < 2.0 * slots && longest > 1.0) {
         const double fixed = 9.0, tile = a->d == 64 ? 1.1 : (a->query_rope ? 2.05 : 1.65);
         const double partial = (double)a->total_q * a->heads * (a->d + 2) * sizeof(float);
@@ -167,7 +175,7 @@ PromptPlan attention_plan(const PtoPromptAttentionArgs *a)
         if (pieces_of(len) > 1) {
             pl.splits = (int)pieces_of(len);
             pl.split_tiles = (int)len;
-            const long long by_tiles = most_tiles * pl.splits, by_keys = ((rows + wg_rows - 1) / wg_rows) * (key_tiles / len + a->b + 1);
+            const long long by_tiles = most_tiles * pl.splits, by_keys = window > 0 ? by_tiles : ((rows + wg_rows - 1) / wg_rows) * (key_tiles / len + a->b + 1);
             pl.workgroups = (by_tiles < by_keys ? by_tiles : by_keys) * a->kv_heads;
             if (pl.workgroups > 4 * slots) pl.workgroups = 4 * slots;
         }
@@ -178,6 +186,80 @@ PromptPlan attention_plan(const PtoPromptAttentionArgs *a)
         pl.ml_bytes = (size_t)a->total_q * a->heads * pl.splits * 2 * sizeof(float);
     }
     return pl;
+}
+
+int attention_launch(const PtoPromptAttentionArgs *a, const int64_t window, const int64_t sinks, void *hip_stream)
+{
+    if (a->total_q == 0) return PTO_OK;
+    if (!a->query || !a->out || !a->cu_seqlens_q || !a->cu_seqlens_k || (a->total_k > 0 && (!a->key || !a->value)))
+        return fail(PTO_E_INVALID_ARG, "prompt_attention: a tensor pointer is NULL");
+    if (!aligned(a->key, 16) || !aligned(a->value, 16) || !aligned(a->key_rope, 16) || a->key_stride_t % 8 != 0 || a->key_stride_h % 8 != 0 ||
+        a->value_stride_t % 8 != 0 || a->value_stride_h % 8 != 0 || a->key_rope_stride_t % 8 != 0 || a->key_rope_stride_h % 8 != 0)
+        return fail(PTO_E_INVALID_ARG, "prompt_attention: keys and values must be 16-byte aligned, their strides multiples of 8 elements");
+    if (!aligned(a->query, 2) || !aligned(a->query_rope, 2) || !aligned(a->out, 2) || !aligned(a->lse, 4) || !aligned(a->cu_seqlens_q, 4) ||
+        !aligned(a->cu_seqlens_k, 4))
+        return fail(PTO_E_INVALID_ARG, "prompt_attention: pointers must be aligned to their element size");
+    constexpr int64_t most = (1ll << 32) / (2 * pto::PA_KEYS) - 256;
+    if (a->key_stride_t < 0 || a->key_stride_t > most || a->value_stride_t < 0 || a->value_stride_t > most || a->key_rope_stride_t < 0 || a->key_rope_stride_t > most)
+        return fail(PTO_E_INVALID_ARG, "prompt_attention: key and value token strides must be in [0, %lld]", (long long)most);
+    if (cu_count() <= 0) return fail(PTO_E_NO_DEVICE, "prompt_attention: no usable device is current");
+    const PromptPlan pl = attention_plan(a, window, sinks);
+    const size_t need = pl.o_bytes + pl.ml_bytes;
+    if (need > 0 && (!a->workspace || a->workspace_bytes < need))
+        return fail(PTO_E_WORKSPACE, "prompt_attention: workspace of %zu bytes required, %zu given", need, a->workspace ? a->workspace_bytes : (size_t)0);
+    if (!aligned(a->workspace, 16)) return fail(PTO_E_INVALID_ARG, "prompt_attention: the workspace must be 16-byte aligned");
+    if (pl.workgroups > 0x7ffffff0ll)
+        return fail(PTO_E_INVALID_ARG, "prompt_attention: the call exceeds the largest launch");
+
+    pto::PaParams p{};
+    p.q = static_cast<const uint16_t *>(a->query);
+    p.qr = static_cast<const uint16_t *>(a->query_rope);
+    p.k = static_cast<const uint16_t *>(a->key);
+    p.kr = static_cast<const uint16_t *>(a->key_rope);
+    p.v = static_cast<const uint16_t *>(a->value);
+    p.out = static_cast<uint16_t *>(a->out);
+    p.lse = a->lse;
+    p.part_o = static_cast<float *>(a->workspace);
+    p.part_ml = reinterpret_cast<float *>(static_cast<char *>(a->workspace) + pl.o_bytes);
+    p.cu_q = a->cu_seqlens_q;
+    p.cu_k = a->cu_seqlens_k;
+    p.q_t = a->query_stride_t, p.q_h = a->query_stride_h;
+    p.qr_t = a->query_rope_stride_t, p.qr_h = a->query_rope_stride_h;
+    p.k_t = a->key_stride_t, p.k_h = a->key_stride_h;
+    p.kr_t = a->key_rope_stride_t, p.kr_h = a->key_rope_stride_h;
+    p.v_t = a->value_stride_t, p.v_h = a->value_stride_h;
+    p.o_t = a->out_stride_t, p.o_h = a->out_stride_h;
+    p.total_q = a->total_q, p.total_k = a->total_k;
+    p.B = (int)a->b;
+    p.kv_heads = (int)a->kv_heads;
+    p.group = (int)(a->heads / a->kv_heads);
+    p.d = (int)a->d;
+    p.rope = a->query_rope != nullptr;
+    p.fp16 = a->fp16 != 0;
+    p.causal = a->causal != 0;
+    p.q_whole = aligned(a->query, 16) && aligned(a->query_rope, 16) && a->query_stride_t % 8 == 0 && a->query_stride_h % 8 == 0 &&
+                a->query_rope_stride_t % 8 == 0 && a->query_rope_stride_h % 8 == 0;
+    p.window = (int)window;
+    p.sinks = (int)sinks;
+    p.most_tiles = pl.most_tiles;
+    p.splits = pl.splits;
+    p.split_tiles = pl.split_tiles;
+    p.waves = pl.waves;
+    p.grid = (int)pl.workgroups;
+    p.cus = cu_count();
+    p.scale_log2 = a->softmax_scale * 1.4426950408889634f;
+    const hipError_t e = pto::prompt_attention_launch(p, static_cast<hipStream_t>(hip_stream));
+    if (e != hipSuccess) return fail(PTO_E_LAUNCH, "prompt_attention: launch failed: %s", hipGetErrorString(e));
+    return PTO_OK;
+}
+
+int window_check(const PtoPromptWindowArgs *a)
+{
+    if (!a) return fail(PTO_E_INVALID_ARG, "prompt_window_attention: args is NULL");
+    if (a->window < 1 || a->window > MOST_TOKENS || a->sinks < 0 || a->sinks > MOST_TOKENS)
+        return fail(PTO_E_INVALID_ARG, "prompt_window_attention: window must be in [1, 2^30], sinks in [0, 2^30]");
+    if (!a->prompt.causal) return fail(PTO_E_INVALID_ARG, "prompt_window_attention: a window is causal");
+    return attention_check(&a->prompt);
 }
 
 }  // namespace
@@ -302,7 +384,7 @@ int pto_prompt_attention_workspace_bytes(const PtoPromptAttentionArgs *a, size_t
     if (!bytes) return fail(PTO_E_INVALID_ARG, "prompt_attention: bytes is NULL");
     const int rc = attention_check(a);
     if (rc != PTO_OK) return rc;
-    const PromptPlan pl = attention_plan(a);
+    const PromptPlan pl = attention_plan(a, 0, 0);
     *bytes = pl.o_bytes + pl.ml_bytes;
     return PTO_OK;
 }
@@ -312,7 +394,7 @@ int pto_prompt_attention_plan(const PtoPromptAttentionArgs *a, PtoPromptPlan *pl
     if (!plan) return fail(PTO_E_INVALID_ARG, "prompt_attention: plan is NULL");
     const int rc = attention_check(a);
     if (rc != PTO_OK) return rc;
-    const PromptPlan pl = attention_plan(a);
+    const PromptPlan pl = attention_plan(a, 0, 0);
     plan->rows_per_workgroup = pl.waves * pto::PA_WAVE_ROWS;
     plan->key_splits = pl.splits;
     plan->split_keys = (int64_t)pl.split_tiles * pto::PA_KEYS;
@@ -323,64 +405,23 @@ int pto_prompt_attention_plan(const PtoPromptAttentionArgs *a, PtoPromptPlan *pl
 int pto_prompt_attention_launch(const PtoPromptAttentionArgs *a, void *hip_stream)
 {
     const int rc = attention_check(a);
-    if (rc != PTO_OK || a->total_q == 0) return rc;
-    if (!a->query || !a->out || !a->cu_seqlens_q || !a->cu_seqlens_k || (a->total_k > 0 && (!a->key || !a->value)))
-        return fail(PTO_E_INVALID_ARG, "prompt_attention: a tensor pointer is NULL");
-    if (!aligned(a->key, 16) || !aligned(a->value, 16) || !aligned(a->key_rope, 16) || a->key_stride_t % 8 != 0 || a->key_stride_h % 8 != 0 ||
-        a->value_stride_t % 8 != 0 || a->value_stride_h % 8 != 0 || a->key_rope_stride_t % 8 != 0 || a->key_rope_stride_h % 8 != 0)
-        return fail(PTO_E_INVALID_ARG, "prompt_attention: keys and values must be 16-byte aligned, their strides multiples of 8 elements");
-    if (!aligned(a->query, 2) || !aligned(a->query_rope, 2) || !aligned(a->out, 2) || !aligned(a->lse, 4) || !aligned(a->cu_seqlens_q, 4) ||
-        !aligned(a->cu_seqlens_k, 4))
-        return fail(PTO_E_INVALID_ARG, "prompt_attention: pointers must be aligned to their element size");
-    constexpr int64_t most = (1ll << 32) / (2 * pto::PA_KEYS) - 256;
-    if (a->key_stride_t < 0 || a->key_stride_t > most || a->value_stride_t < 0 || a->value_stride_t > most || a->key_rope_stride_t < 0 || a->key_rope_stride_t > most)
-        return fail(PTO_E_INVALID_ARG, "prompt_attention: key and value token strides must be in [0, %lld]", (long long)most);
-    if (cu_count() <= 0) return fail(PTO_E_NO_DEVICE, "prompt_attention: no usable device is current");
-    const PromptPlan pl = attention_plan(a);
-    const size_t need = pl.o_bytes + pl.ml_bytes;
-    if (need > 0 && (!a->workspace || a->workspace_bytes < need))
-        return fail(PTO_E_WORKSPACE, "prompt_attention: workspace of %zu bytes required, %zu given", need, a->workspace ? a->workspace_bytes : (size_t)0);
-    if (!aligned(a->workspace, 16)) return fail(PTO_E_INVALID_ARG, "prompt_attention: the workspace must be 16-byte aligned");
-    if (pl.workgroups > 0x7ffffff0ll)
-        return fail(PTO_E_INVALID_ARG, "prompt_attention: the call exceeds the largest launch");
+    return rc != PTO_OK ? rc : attention_launch(a, 0, 0, hip_stream);
+}
 
-    pto::PaParams p{};
-    p.q = static_cast<const uint16_t *>(a->query);
-    p.qr = static_cast<const uint16_t *>(a->query_rope);
-    p.k = static_cast<const uint16_t *>(a->key);
-    p.kr = static_cast<const uint16_t *>(a->key_rope);
-    p.v = static_cast<const uint16_t *>(a->value);
-    p.out = static_cast<uint16_t *>(a->out);
-    p.lse = a->lse;
-    p.part_o = static_cast<float *>(a->workspace);
-    p.part_ml = reinterpret_cast<float *>(static_cast<char *>(a->workspace) + pl.o_bytes);
-    p.cu_q = a->cu_seqlens_q;
-    p.cu_k = a->cu_seqlens_k;
-    p.q_t = a->query_stride_t, p.q_h = a->query_stride_h;
-    p.qr_t = a->query_rope_stride_t, p.qr_h = a->query_rope_stride_h;
-    p.k_t = a->key_stride_t, p.k_h = a->key_stride_h;
-    p.kr_t = a->key_rope_stride_t, p.kr_h = a->key_rope_stride_h;
-    p.v_t = a->value_stride_t, p.v_h = a->value_stride_h;
-    p.o_t = a->out_stride_t, p.o_h = a->out_stride_h;
-    p.total_q = a->total_q, p.total_k = a->total_k;
-    p.B = (int)a->b;
-    p.kv_heads = (int)a->kv_heads;
-    p.group = (int)(a->heads / a->kv_heads);
-    p.d = (int)a->d;
-    p.rope = a->query_rope != nullptr;
-    p.fp16 = a->fp16 != 0;
-    p.causal = a->causal != 0;
-    p.q_whole = aligned(a->query, 16) && aligned(a->query_rope, 16) && a->query_stride_t % 8 == 0 && a->query_stride_h % 8 == 0 &&
-                a->query_rope_stride_t % 8 == 0 && a->query_rope_stride_h % 8 == 0;
-    p.splits = pl.splits;
-    p.split_tiles = pl.split_tiles;
-    p.waves = pl.waves;
-    p.grid = (int)pl.workgroups;
-    p.cus = cu_count();
-    p.scale_log2 = a->softmax_scale * 1.4426950408889634f;
-    const hipError_t e = pto::prompt_attention_launch(p, static_cast<hipStream_t>(hip_stream));
-    if (e != hipSuccess) return fail(PTO_E_LAUNCH, "prompt_attention: launch failed: %s", hipGetErrorString(e));
+int pto_prompt_window_workspace_bytes(const PtoPromptWindowArgs *a, size_t *bytes)
+{
+    if (!bytes) return fail(PTO_E_INVALID_ARG, "prompt_window_attention: bytes is NULL");
+    const int rc = window_check(a);
+    if (rc != PTO_OK) return rc;
+    const PromptPlan pl = attention_plan(&a->prompt, a->window, a->sinks);
+    *bytes = pl.o_bytes + pl.ml_bytes;
     return PTO_OK;
+}
+
+int pto_prompt_window_launch(const PtoPromptWindowArgs *a, void *hip_stream)
+{
+    const int rc = window_check(a);
+    return rc != PTO_OK ? rc : attention_launch(&a->prompt, a->window, a->sinks, hip_stream);
 }
 
 }  // extern "C"

@@ -1,0 +1,223 @@
+// C ABI of a serving step's operators: pages and slots of the cache, attention over the cached latents.
+// Declarations: include/pypto_amd_sfa.h.
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+
+#include "capi_error.h"
+#include "common.h"
+#include "pypto_amd_sfa.h"
+#include "serving_ops.h"
+
+namespace {
+
+using pto::cu_count;
+using pto::fail;
+
+constexpr int64_t MOST_TOKENS = 1ll << 30;
+constexpr int PACKED_PITCH = 656;
+
+bool aligned(const void *p, const uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+
+int table_check(const char *op, const int64_t b, const int64_t maxblk, const int64_t bs)
+{
+    if (b < 1 || b > (1ll << 24)) return fail(PTO_E_INVALID_ARG, "%s: b out of range", op);
+    if (bs < 1 || bs > (1ll << 30) || maxblk < 1 || maxblk > (1ll << 30))
+        return fail(PTO_E_INVALID_ARG, "%s: block_size and max_blocknum_perbatch must be in [1, 2^30]", op);
+    if (b * maxblk > 0x7fffffffll) return fail(PTO_E_INVALID_ARG, "%s: a block table holds at most 2^31 - 1 entries", op);
+    return PTO_OK;
+}
+
+int latent_check(const PtoLatentAttentionArgs *a)
+{
+    if (!a) return fail(PTO_E_INVALID_ARG, "latent_attention: args is NULL");
+    const int rc = table_check("latent_attention", a->b, a->max_blocknum_perbatch, a->block_size);
+    if (rc != PTO_OK) return rc;
+    if (a->total_q < 0 || a->total_q > MOST_TOKENS || a->heads < 1 || a->heads > 65536 || a->total_q * a->heads > 0x7fff0000ll)
+        return fail(PTO_E_INVALID_ARG, "latent_attention: total_q or heads out of range");
+    if (a->max_blocknum_perbatch * a->block_size > 0x7ffffff0ll)
+        return fail(PTO_E_INVALID_ARG, "latent_attention: a sequence of the block table holds at most 2^31 - 16 keys");
+    if (a->window < 0 || a->window > MOST_TOKENS || a->sinks < 0 || a->sinks > MOST_TOKENS)
+        return fail(PTO_E_INVALID_ARG, "latent_attention: window and sinks must be in [0, 2^30]");
+    if (a->sinks > 0 && a->window == 0) return fail(PTO_E_INVALID_ARG, "latent_attention: sinks go with a window");
+    if (a->tree_mask && a->window > 0) return fail(PTO_E_INVALID_ARG, "latent_attention: a tree mask and a window exclude one another");
+    if (a->tree_mask && (a->mask_words < 1 || a->mask_words > pto::SLOTS_MAX_WORDS))
+        return fail(PTO_E_INVALID_ARG, "latent_attention: mask_words must be in [1, %d]", pto::SLOTS_MAX_WORDS);
+    if (!std::isfinite(a->softmax_scale) || !std::isfinite(a->softmax_scale * 1.4426950408889634f))
+        return fail(PTO_E_INVALID_ARG, "latent_attention: softmax_scale is not finite");
+    return PTO_OK;
+}
+
+struct LatentPlan {
+    int groups, by_tile, entries;
+    size_t o_bytes, ml_bytes, join_bytes;
+};
+
+// The device divides the work, since lengths are there.  Here only as many workgroups as there can be pieces of LA_LEAST tiles, one to a
+// compute unit at most (a workgroup's LDS is most of one's), and memory for two pieces of each.
+LatentPlan latent_plan(const PtoLatentAttentionArgs *a)
+{
+    LatentPlan pl{};
+    const long long cus = cu_count() > 0 ? cu_count() : 256;
+    const long long row_tiles = a->total_q * a->heads / pto::LA_ROWS + (a->b < a->total_q ? a->b : a->total_q);    // at most
+    long long tiles = (a->max_blocknum_perbatch * a->block_size + pto::LA_KEYS - 1) / pto::LA_KEYS;
+    if (a->window > 0) {
+        const long long w = (a->window + a->sinks + pto::LA_ROWS) / pto::LA_KEYS + 4;
+        tiles = w < tiles ? w : tiles;
+    }
+    const double pieces = (double)row_tiles * (double)(tiles + pto::LA_OPEN) / (pto::LA_LEAST + pto::LA_OPEN);
+    const long long groups = pieces < (double)cus ? (long long)pieces + 1 : cus;
+    pl.groups = (int)((groups + 7) / 8 * 8);
+    pl.by_tile = row_tiles <= pl.groups;
+    pl.entries = (int)(pl.by_tile ? (row_tiles > 0 ? row_tiles : 1) : pl.groups);
+    pl.o_bytes = (size_t)2 * pl.groups * pto::LA_ROWS * 512 * sizeof(float);
+    pl.ml_bytes = (size_t)2 * pl.groups * pto::LA_ROWS * 2 * sizeof(float);
+    pl.join_bytes = (size_t)pl.entries * 4 * sizeof(int32_t);
+    return pl;
+}
+
+}  // namespace
+
+extern "C" {
+
+int pto_cache_pages_launch(const PtoCachePagesArgs *a, void *hip_stream)
+{
+    if (!a) return fail(PTO_E_INVALID_ARG, "cache_pages: args is NULL");
+    const int rc = table_check("cache_pages", a->b, a->max_blocknum_perbatch, a->block_size);
+    if (rc != PTO_OK) return rc;
+    if (a->room < 0 || a->room > 0x7fffffffll) return fail(PTO_E_INVALID_ARG, "cache_pages: room out of range");
+    if (!a->lens_before || !a->lens_after || !a->block_table || !a->free_count || !a->free_left || (a->room > 0 && !a->free_pages))
+        return fail(PTO_E_INVALID_ARG, "cache_pages: a tensor pointer is NULL");
+    if (!aligned(a->lens_before, 4) || !aligned(a->lens_after, 4) || !aligned(a->block_table, 4) || !aligned(a->free_pages, 4) || !aligned(a->free_count, 4) ||
+        !aligned(a->free_left, 4))
+        return fail(PTO_E_INVALID_ARG, "cache_pages: pointers must be aligned to their element size");
+    if (cu_count() <= 0) return fail(PTO_E_NO_DEVICE, "cache_pages: no usable device is current");
+    pto::CachePagesParams p{};
+    p.before = a->lens_before;
+    p.after = a->lens_after;
+    p.bt = a->block_table;
+    p.stack = a->free_pages;
+    p.count = a->free_count;
+    p.left = a->free_left;
+    p.room = a->room;
+    p.B = (int)a->b;
+    p.maxblk = (int)a->max_blocknum_perbatch;
+    p.bs = (int)a->block_size;
+    const hipError_t e = pto::cache_pages_launch(p, static_cast<hipStream_t>(hip_stream));
+    if (e != hipSuccess) return fail(PTO_E_LAUNCH, "cache_pages: launch failed: %s", hipGetErrorString(e));
+    return PTO_OK;
+}
+
+int pto_cache_slots_launch(const PtoCacheSlotsArgs *a, void *hip_stream)
+{
+    if (!a) return fail(PTO_E_INVALID_ARG, "cache_slots: args is NULL");
+    const int rc = table_check("cache_slots", a->b, a->max_blocknum_perbatch, a->block_size);
+    if (rc != PTO_OK) return rc;
+    if (a->t < 0 || a->t > MOST_TOKENS) return fail(PTO_E_INVALID_ARG, "cache_slots: t out of range");
+    if (!a->parents != !a->tree_mask && a->t > 0) return fail(PTO_E_INVALID_ARG, "cache_slots: parents and tree_mask come together");
+    if (a->tree_mask && (a->mask_words < 1 || a->mask_words > pto::SLOTS_MAX_WORDS))
+        return fail(PTO_E_INVALID_ARG, "cache_slots: mask_words must be in [1, %d]", pto::SLOTS_MAX_WORDS);
+    if (!a->query_lens || !a->seq_lens || !a->block_table || !a->cu_seqlens_q || (a->t > 0 && (!a->positions || !a->cache_index)))
+        return fail(PTO_E_INVALID_ARG, "cache_slots: a tensor pointer is NULL");
+    if (!aligned(a->query_lens, 4) || !aligned(a->seq_lens, 4) || !aligned(a->block_table, 4) || !aligned(a->cu_seqlens_q, 4) || !aligned(a->cu_seqlens_k, 4) ||
+        !aligned(a->positions, 8) || !aligned(a->cache_index, 8) || !aligned(a->parents, 4) || !aligned(a->tree_mask, 8))
+        return fail(PTO_E_INVALID_ARG, "cache_slots: pointers must be aligned to their element size");
+    if (cu_count() <= 0) return fail(PTO_E_NO_DEVICE, "cache_slots: no usable device is current");
+    pto::CacheSlotsParams p{};
+    p.new_lens = a->query_lens;
+    p.all_lens = a->seq_lens;
+    p.bt = a->block_table;
+    p.cu_q = a->cu_seqlens_q;
+    p.cu_k = a->cu_seqlens_k;
+    p.positions = reinterpret_cast<long long *>(a->positions);
+    p.slots = reinterpret_cast<long long *>(a->cache_index);
+    p.parents = a->parents;
+    p.mask = reinterpret_cast<unsigned long long *>(a->tree_mask);
+    p.T = a->t;
+    p.B = (int)a->b;
+    p.maxblk = (int)a->max_blocknum_perbatch;
+    p.bs = (int)a->block_size;
+    p.words = (int)a->mask_words;
+    p.cus = cu_count();
+    const hipError_t e = pto::cache_slots_launch(p, static_cast<hipStream_t>(hip_stream));
+    if (e != hipSuccess) return fail(PTO_E_LAUNCH, "cache_slots: launch failed: %s", hipGetErrorString(e));
+    return PTO_OK;
+}
+
+int pto_latent_attention_workspace_bytes(const PtoLatentAttentionArgs *a, size_t *bytes)
+{
+    if (!bytes) return fail(PTO_E_INVALID_ARG, "latent_attention: bytes is NULL");
+    const int rc = latent_check(a);
+    if (rc != PTO_OK) return rc;
+    const LatentPlan pl = latent_plan(a);
+    *bytes = pl.o_bytes + pl.ml_bytes + pl.join_bytes;
+    return PTO_OK;
+}
+
+int pto_latent_attention_launch(const PtoLatentAttentionArgs *a, void *hip_stream)
+{
+    const int rc = latent_check(a);
+    if (rc != PTO_OK || a->total_q == 0) return rc;
+    const bool packed = a->packed != 0;
+    if (a->cache_rows < 1 || a->cache_rows > 0x7fffffffll) return fail(PTO_E_INVALID_ARG, "latent_attention: cache_rows out of range");
+    if (!a->nope || (packed ? a->rope_cache || a->scales : !a->rope_cache || !a->scales))
+        return fail(PTO_E_INVALID_ARG, "latent_attention: a cache is three arrays, or one packed array and two NULL pointers");
+    if (!a->query_nope || !a->query_rope || !a->out || !a->block_table || !a->cu_seqlens_q || !a->seq_lens)
+        return fail(PTO_E_INVALID_ARG, "latent_attention: a tensor pointer is NULL");
+    if (!aligned(a->nope, 16) || !aligned(a->rope_cache, 16) || !aligned(a->scales, 16))
+        return fail(PTO_E_INVALID_ARG, "latent_attention: cache pointers must be 16-byte aligned");
+    if (!aligned(a->query_nope, 16) || !aligned(a->query_rope, 16) || a->query_nope_stride_t % 8 != 0 || a->query_nope_stride_h % 8 != 0 ||
+        a->query_rope_stride_t % 8 != 0 || a->query_rope_stride_h % 8 != 0)
+        return fail(PTO_E_INVALID_ARG, "latent_attention: queries must be 16-byte aligned, their strides multiples of 8 elements");
+    if (!aligned(a->out, 2) || !aligned(a->lse, 4) || !aligned(a->block_table, 4) || !aligned(a->cu_seqlens_q, 4) || !aligned(a->seq_lens, 4) ||
+        !aligned(a->tree_mask, 8))
+        return fail(PTO_E_INVALID_ARG, "latent_attention: pointers must be aligned to their element size");
+    if (cu_count() <= 0) return fail(PTO_E_NO_DEVICE, "latent_attention: no usable device is current");
+    const LatentPlan pl = latent_plan(a);
+    const size_t need = pl.o_bytes + pl.ml_bytes + pl.join_bytes;
+    if (!a->workspace || a->workspace_bytes < need)
+        return fail(PTO_E_WORKSPACE, "latent_attention: workspace of %zu bytes required, %zu given", need, a->workspace ? a->workspace_bytes : (size_t)0);
+    if (!aligned(a->workspace, 16)) return fail(PTO_E_INVALID_ARG, "latent_attention: the workspace must be 16-byte aligned");
+
+    pto::LaParams p{};
+    p.q = static_cast<const uint16_t *>(a->query_nope);
+    p.qr = static_cast<const uint16_t *>(a->query_rope);
+    p.q_t = a->query_nope_stride_t, p.q_h = a->query_nope_stride_h;
+    p.qr_t = a->query_rope_stride_t, p.qr_h = a->query_rope_stride_h;
+    p.o_t = a->out_stride_t, p.o_h = a->out_stride_h;
+    p.cache.nope = static_cast<uint8_t *>(const_cast<void *>(a->nope));
+    p.cache.rope = packed ? p.cache.nope + 512 : static_cast<uint8_t *>(const_cast<void *>(a->rope_cache));
+    p.cache.scale = packed ? p.cache.nope + 640 : static_cast<uint8_t *>(const_cast<void *>(a->scales));
+    p.cache.nope_pitch = packed ? PACKED_PITCH : 512;
+    p.cache.rope_pitch = packed ? PACKED_PITCH : 128;
+    p.cache.scale_pitch = packed ? PACKED_PITCH : 16;
+    p.cache.rows = a->cache_rows;
+    p.bt = a->block_table;
+    p.cu_q = a->cu_seqlens_q;
+    p.lens = a->seq_lens;
+    p.mask = reinterpret_cast<const unsigned long long *>(a->tree_mask);
+    p.out = static_cast<uint16_t *>(a->out);
+    p.lse = a->lse;
+    p.part_o = static_cast<float *>(a->workspace);
+    p.part_ml = reinterpret_cast<float *>(static_cast<char *>(a->workspace) + pl.o_bytes);
+    p.joins = reinterpret_cast<int32_t *>(static_cast<char *>(a->workspace) + pl.o_bytes + pl.ml_bytes);
+    p.total_q = a->total_q;
+    p.B = (int)a->b;
+    p.maxblk = (int)a->max_blocknum_perbatch;
+    p.bs = (int)a->block_size;
+    p.heads = (int)a->heads;
+    p.words = a->tree_mask ? (int)a->mask_words : 0;
+    p.window = (int)a->window;
+    p.sinks = (int)a->sinks;
+    p.groups = pl.groups;
+    p.by_tile = pl.by_tile;
+    p.entries = pl.entries;
+    p.of_heads = pto::divisor_of((uint32_t)a->heads);
+    p.of_bs = pto::divisor_of((uint32_t)a->block_size);
+    p.scale_log2 = a->softmax_scale * 1.4426950408889634f;
+    const hipError_t e = pto::latent_attention_launch(p, static_cast<hipStream_t>(hip_stream));
+    if (e != hipSuccess) return fail(PTO_E_LAUNCH, "latent_attention: launch failed: %s", hipGetErrorString(e));
+    return PTO_OK;
+}
+
+}  // extern "C"

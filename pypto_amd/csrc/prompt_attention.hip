@@ -121,7 +121,9 @@ __device__ __forceinline__ int pa_visible(const int t, const int lq, const int l
 // c of row r at c ^ r % 16 (keys) or c ^ 4 * (r % 4) (values), and an exclusive or to each read.
 constexpr int PA_BLOCK = 1040;
 
-template <typename E, int D, int R, int W>
+// WINDOW: a row sees the last p.window of the keys up to its own, and the first p.sinks.  Tiles that no row of the workgroup sees, between
+// the first keys and the windows, are stepped over: t counts the tiles that are left.
+template <typename E, int D, int R, int W, bool WINDOW>
 __global__ __launch_bounds__(64 * W, 2) void prompt_attention_kernel(const PaParams p)
 {
     constexpr int ROWS = 32 * W;
@@ -155,7 +157,7 @@ __global__ __launch_bounds__(64 * W, 2) void prompt_attention_kernel(const PaPar
         const int l = tid & 63, mine = base + l < p.B ? base + l : p.B - 1;
         c.sq = span_of(p.cu_q, mine, (int)p.total_q), c.sk = span_of(p.cu_k, mine, (int)p.total_k);
         c.tiles = base + l < p.B ? (c.sq.len * p.group + ROWS - 1) / ROWS : 0;
-        c.splits = pa_splits_of((c.sk.len + PA_KEYS - 1) / PA_KEYS, p.split_tiles, p.splits);
+        c.splits = pa_splits_of(WINDOW ? pa_tiles_of(c.sk.len, p.most_tiles) : (c.sk.len + PA_KEYS - 1) / PA_KEYS, p.split_tiles, p.splits);
         c.upto = wave_sums(c.tiles * c.splits);
         return c;
     };
@@ -197,7 +199,16 @@ __global__ __launch_bounds__(64 * W, 2) void prompt_attention_kernel(const PaPar
         const int wave_most = tile * ROWS + 32 * w < rows ? pa_visible(__builtin_amdgcn_readlane(tok, 31), lq, lk, p.causal) : 0;
         const int wave_least = pa_visible(__builtin_amdgcn_readlane(tok, 0), lq, lk, p.causal);
 
-        const int key_tiles = (wg_sees + PA_KEYS - 1) / PA_KEYS;
+        // where windows begin: of this lane's row, of the workgroup's first and the wave's last; tiles of the first keys in front of them, tiles
+        // stepped over
+        auto from_of = [&](const int n) { return WINDOW && n > p.window ? n - p.window : 0; };
+        const int from = from_of(sees), wave_from = WINDOW ? from_of(wave_most) : 0;
+        const int low = WINDOW ? from_of(pa_visible(tile * ROWS / p.group, lq, lk, 1)) / PA_KEYS : 0;
+        const int sink_tiles = WINDOW ? ((p.sinks + PA_KEYS - 1) / PA_KEYS < low ? (p.sinks + PA_KEYS - 1) / PA_KEYS : low) : 0;
+        const int skip = low - sink_tiles;
+        auto tile_at = [&](const int t) { return WINDOW && t >= sink_tiles ? t + skip : t; };
+
+        const int key_tiles = (wg_sees + PA_KEYS - 1) / PA_KEYS - skip;
         const int split_len = (key_tiles + splits - 1) / splits;
         const int t_begin = split * split_len;
         const int t_end = t_begin + split_len < key_tiles ? t_begin + split_len : key_tiles;
@@ -217,8 +228,8 @@ __global__ __launch_bounds__(64 * W, 2) void prompt_attention_kernel(const PaPar
         const uint32_t k_off = (uint32_t)row_of * (uint32_t)(p.k_t * 2) + 16 * k_piece, v_off = (uint32_t)row_of * (uint32_t)(p.v_t * 2) + 16 * v_piece;
         const uint32_t r_off = (uint32_t)(l >> 3) * (uint32_t)(p.kr_t * 2) + 16 * r_piece;
         // the next tile's first row of this wave, of keys, rope keys and values, and which tiles these are
-        const uint8_t *k_next = k_base + ((long long)t_begin * PA_KEYS + PER * w) * p.k_t * 2, *v_next = v_base + ((long long)t_begin * PA_KEYS + PER * w) * p.v_t * 2;
-        const uint8_t *r_next = R > 0 ? r_base + ((long long)t_begin * PA_KEYS + 8 * w) * p.kr_t * 2 : nullptr;
+        const uint8_t *k_next = k_base + ((long long)tile_at(t_begin) * PA_KEYS + PER * w) * p.k_t * 2, *v_next = v_base + ((long long)tile_at(t_begin) * PA_KEYS + PER * w) * p.v_t * 2;
+        const uint8_t *r_next = R > 0 ? r_base + ((long long)tile_at(t_begin) * PA_KEYS + 8 * w) * p.kr_t * 2 : nullptr;
         int k_tile = t_begin, v_tile = t_begin;
         // one request of a tile all of whose keys there are: NK of its keys, NR of its rope keys, NK of its values
         auto request_whole = [&](const int i, const int k_stage, const int v_stage) __attribute__((always_inline)) {
@@ -232,18 +243,23 @@ __global__ __launch_bounds__(64 * W, 2) void prompt_attention_kernel(const PaPar
             const int r = (i * W + w) * each + row_in, from = r < left ? r : left - 1;
             dma16_base(at - (long long)each * w * pitch * 2, (uint32_t)from * (uint32_t)(pitch * 2) + 16 * piece, dst + (i * W + w) * bytes);
         };
-        auto whole = [&](const int tile_of) { return lk - tile_of * PA_KEYS >= PA_KEYS; };
+        auto whole = [&](const int t) { return lk - tile_at(t) * PA_KEYS >= PA_KEYS; };
         auto next_keys = [&]() __attribute__((always_inline)) {
             k_next += PA_KEYS * 2 * p.k_t;
             if (R > 0) r_next += PA_KEYS * 2 * p.kr_t;
             ++k_tile;
+            if (WINDOW && k_tile == sink_tiles) {
+                k_next += (long long)skip * (PA_KEYS * 2) * p.k_t;
+                if (R > 0) r_next += (long long)skip * (PA_KEYS * 2) * p.kr_t;
+            }
         };
         auto next_values = [&]() __attribute__((always_inline)) {
             v_next += PA_KEYS * 2 * p.v_t;
             ++v_tile;
+            if (WINDOW && v_tile == sink_tiles) v_next += (long long)skip * (PA_KEYS * 2) * p.v_t;
         };
         auto request_keys = [&](const int stage) __attribute__((always_inline)) {
-            const int left = lk - k_tile * PA_KEYS;
+            const int left = lk - tile_at(k_tile) * PA_KEYS;
             if (whole(k_tile)) {
 #pragma unroll
                 for (int i = 0; i < NK + NR; ++i) request_whole(i, stage, 0);
@@ -261,7 +277,7 @@ __global__ __launch_bounds__(64 * W, 2) void prompt_attention_kernel(const PaPar
                 for (int i = 0; i < NK; ++i) request_whole(NK + NR + i, 0, stage);
             } else {
 #pragma unroll
-                for (int i = 0; i < NK; ++i) request_last(v_next, p.v_t, v_piece, row_of, lds0 + STAGES * K_STAGE + stage * K_BYTES, lk - v_tile * PA_KEYS, i, PER, REQ);
+                for (int i = 0; i < NK; ++i) request_last(v_next, p.v_t, v_piece, row_of, lds0 + STAGES * K_STAGE + stage * K_BYTES, lk - tile_at(v_tile) * PA_KEYS, i, PER, REQ);
             }
             next_values();
         };
@@ -379,8 +395,17 @@ __global__ __launch_bounds__(64 * W, 2) void prompt_attention_kernel(const PaPar
             }
         };
         // The softmax of tile t: scores to probabilities.
-        auto softmax = [&](const int t) __attribute__((always_inline)) {
-            if ((t + 1) * PA_KEYS > wave_least) {
+        auto softmax = [&](const int count) __attribute__((always_inline)) {
+            const int t = tile_at(count);
+            if (WINDOW && ((t + 1) * PA_KEYS > wave_least || (t * PA_KEYS < wave_from && (t + 1) * PA_KEYS > p.sinks))) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int key = t * PA_KEYS + 32 * h + 8 * (i >> 2) + 4 * half + (i & 3);
+                        if (key >= sees || (key < from && key >= p.sinks)) s[h][i] = -INFINITY;
+                    }
+            } else if (!WINDOW && (t + 1) * PA_KEYS > wave_least) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -445,7 +470,7 @@ __global__ __launch_bounds__(64 * W, 2) void prompt_attention_kernel(const PaPar
                 s0 = s1, s1 = PHASED ? s2 : s, s2 = s;
             };
             // tiles that this wave's rows see end here; in later ones it asks for its part of the tile and keeps step
-            int own_end = (wave_most + PA_KEYS - 1) / PA_KEYS;
+            int own_end = (wave_most + PA_KEYS - 1) / PA_KEYS - skip;
             own_end = own_end < t_end ? own_end : t_end;
             request_keys(s0);
             if (p.q_whole) request_queries();
@@ -578,7 +603,7 @@ __global__ __launch_bounds__(256, 8) void prompt_merge_kernel(const PaParams p, 
     int b = __builtin_amdgcn_readfirstlane(sequence_of(p.cu_q, p.B, tq));
     for (long long r = first; b < p.B; ++b) {
         const Span sq = span_of(p.cu_q, b, (int)p.total_q), sk = span_of(p.cu_k, b, (int)p.total_k);
-        const int splits = pa_splits_of((sk.len + PA_KEYS - 1) / PA_KEYS, p.split_tiles, p.splits);
+        const int splits = pa_splits_of(pa_tiles_of(sk.len, p.most_tiles), p.split_tiles, p.splits);
         if (tq < sq.begin) tq = sq.begin, head = 0, r = (long long)tq * heads;
         if (r >= end) return;
         if (splits <= 1) {                                 // written by the attention kernel
@@ -644,12 +669,12 @@ __global__ __launch_bounds__(256, 8) void prompt_merge_kernel(const PaParams p, 
     }
 }
 
-template <typename E, int D, int R>
+template <typename E, int D, int R, bool WINDOW>
 hipError_t launch_of(const PaParams &p, hipStream_t stream)
 {
-    if (p.waves == 4) hipLaunchKernelGGL((prompt_attention_kernel<E, D, R, 4>), dim3((unsigned)p.grid), dim3(64 * 4), 0, stream, p);
+    if (p.waves == 4) hipLaunchKernelGGL((prompt_attention_kernel<E, D, R, 4, WINDOW>), dim3((unsigned)p.grid), dim3(64 * 4), 0, stream, p);
     if constexpr (D == 128) {
-        if (p.waves == 8) hipLaunchKernelGGL((prompt_attention_kernel<E, D, R, 8>), dim3((unsigned)p.grid), dim3(64 * 8), 0, stream, p);
+        if (p.waves == 8) hipLaunchKernelGGL((prompt_attention_kernel<E, D, R, 8, WINDOW>), dim3((unsigned)p.grid), dim3(64 * 8), 0, stream, p);
     }
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.splits <= 1) return e;
@@ -658,18 +683,19 @@ hipError_t launch_of(const PaParams &p, hipStream_t stream)
     return hipGetLastError();
 }
 
-template <typename E>
+template <typename E, bool WINDOW>
 hipError_t launch_type(const PaParams &p, hipStream_t stream)
 {
-    if (p.d == 64) return launch_of<E, 64, 0>(p, stream);
-    return p.rope ? launch_of<E, 128, PA_ROPE>(p, stream) : launch_of<E, 128, 0>(p, stream);
+    if (p.d == 64) return launch_of<E, 64, 0, WINDOW>(p, stream);
+    return p.rope ? launch_of<E, 128, PA_ROPE, WINDOW>(p, stream) : launch_of<E, 128, 0, WINDOW>(p, stream);
 }
 
 }  // namespace
 
 hipError_t prompt_attention_launch(const PaParams &p, hipStream_t stream)
 {
-    return p.fp16 ? launch_type<F16>(p, stream) : launch_type<BF16>(p, stream);
+    if (p.window > 0) return p.fp16 ? launch_type<F16, true>(p, stream) : launch_type<BF16, true>(p, stream);
+    return p.fp16 ? launch_type<F16, false>(p, stream) : launch_type<BF16, false>(p, stream);
 }
 
 }  // namespace pto

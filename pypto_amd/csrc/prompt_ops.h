@@ -87,6 +87,8 @@ struct PaParams {
     long long q_t, q_h, qr_t, qr_h, k_t, k_h, kr_t, kr_h, v_t, v_h, o_t, o_h;   // strides in elements
     long long total_q, total_k;
     int B, kv_heads, group, d, rope, fp16, causal;
+    int window, sinks;                    // keys up to its own that a row sees, and first ones (window 0: all up to its own)
+    int most_tiles;                       // most tiles of keys that a row tile of such a window sees
     int q_whole;                          // queries come in whole 16-byte pieces
     int splits, split_tiles;              // most splits of a row tile's keys; tiles from which a further split begins
     int waves;                            // of a workgroup, PA_WAVE_ROWS rows each: 8, or 4
@@ -101,6 +103,13 @@ __host__ __device__ inline int pa_splits_of(const int key_tiles, const int split
 {
     const int n = (key_tiles + split_tiles - 1) / split_tiles;
     return n < 1 ? 1 : (n > most ? most : n);
+}
+
+// tiles of a sequence's keys, as far as a row tile sees them
+__host__ __device__ inline int pa_tiles_of(const int keys, const int most)
+{
+    const int n = (keys + PA_KEYS - 1) / PA_KEYS;
+    return n < most ? n : most;
 }
 
 }  // namespace pto

@@ -1,0 +1,81 @@
+// Launch parameters of a serving step's operators: pages and slots of the cache, attention over the cached latents
+// (internal to the library).
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "prompt_ops.h"
+
+namespace pto {
+
+// n / d for 0 <= n < 2^31 by a product: (high half of n * magic + n) >> shift, magic = floor(2^32 (2^shift - d) / d) + 1 for the
+// smallest 2^shift >= d
+struct Divisor {
+    uint32_t magic;
+    int shift;
+};
+inline Divisor divisor_of(const uint32_t d)
+{
+    int shift = 0;
+    while ((1ull << shift) < d) ++shift;
+    return {(uint32_t)(((1ull << 32) * ((1ull << shift) - d)) / d + 1), shift};
+}
+__device__ __forceinline__ int divide(const int n, const Divisor d) { return (int)((__umulhi((uint32_t)n, d.magic) + (uint32_t)n) >> d.shift); }
+
+// ---- pages and slots (paged_layout.hip)
+
+struct CachePagesParams {
+    const int32_t *before, *after;        // [B]
+    int32_t *bt;                          // [B, maxblk]
+    int32_t *stack;                       // [room]
+    const int32_t *count;                 // [1]
+    int32_t *left;                        // [1], may be count
+    long long room;
+    int B, maxblk, bs;
+};
+hipError_t cache_pages_launch(const CachePagesParams &p, hipStream_t stream);
+
+constexpr int SLOTS_MAX_WORDS = 16;
+struct CacheSlotsParams {
+    const int32_t *new_lens, *all_lens;   // [B]
+    const int32_t *bt;                    // [B, maxblk]
+    int32_t *cu_q, *cu_k;                 // [B + 1], cu_k or null
+    long long *positions, *slots;         // [T]
+    const int32_t *parents;               // [T] or null
+    unsigned long long *mask;             // [T, words] or null
+    long long T;
+    int B, maxblk, bs, words;
+    int cus;
+};
+hipError_t cache_slots_launch(const CacheSlotsParams &p, hipStream_t stream);
+
+// ---- attention over the cached latents (latent_attention.hip)
+
+constexpr int LA_ROWS = 64;               // (token, head) rows of a workgroup
+constexpr int LA_KEYS = 32;               // keys of a tile
+constexpr int LA_OPEN = 6;                // what a row tile's beginning and end cost, in tiles
+constexpr int LA_LEAST = 8;               // tiles of the shortest piece that keys are divided into
+
+struct LaParams {
+    const uint16_t *q, *qr;               // [total_q, heads, 512], [total_q, heads, 64] bf16
+    long long q_t, q_h, qr_t, qr_h, o_t, o_h;   // strides in elements
+    CacheRows cache;
+    const int32_t *bt;                    // [B, maxblk]
+    const int32_t *cu_q;                  // [B + 1]
+    const int32_t *lens;                  // [B]
+    const unsigned long long *mask;       // [total_q, words] or null
+    uint16_t *out;
+    float *lse;                           // [total_q, heads] or null
+    float *part_o, *part_ml;              // [2 * groups] pieces of LA_ROWS rows: 512 sums, (maximum, sum)
+    int32_t *joins;                       // [entries][4]: first piece, pieces, first row, rows
+    long long total_q;
+    int B, maxblk, bs, heads, words;
+    int window, sinks;                    // window 0: all keys
+    int groups;                           // workgroups, a multiple of eight
+    int by_tile, entries;                 // joins by row tile (of all sequences), else by workgroup; how many there are
+    Divisor of_heads, of_bs;
+    float scale_log2;
+};
+hipError_t latent_attention_launch(const LaParams &p, hipStream_t stream);
+
+}  // namespace pto

@@ -127,8 +127,9 @@ PyObject *raise_status(const int rc)
 
 // Workspace from torch's caching allocator on the current stream, then the launch on that stream; the block goes back
 // to the allocator at once, which is in stream order, as for a tensor that goes out of scope after the call.
-template <typename Args, typename Bytes, typename Launch>
-PyObject *enqueue(const c10::Device &device, Args &a, Bytes bytes, Launch launch)
+// `holder` has the workspace's fields where the arguments themselves do not.
+template <typename Args, typename Bytes, typename Launch, typename Holder>
+PyObject *enqueue(const c10::Device &device, Args &a, Bytes bytes, Launch launch, Holder *holder)
 {
     c10::DeviceGuard guard(device);
     const hipStream_t stream = c10::hip::getCurrentHIPStream(device.index()).stream();
@@ -136,12 +137,18 @@ PyObject *enqueue(const c10::Device &device, Args &a, Bytes bytes, Launch launch
     int rc = bytes(&a, &need);
     if (rc != PTO_OK) return raise_status(rc);
     void *ws = need > 0 ? c10::hip::HIPCachingAllocator::raw_alloc_with_stream(need, stream) : nullptr;
-    a.workspace = ws;
-    a.workspace_bytes = need;
+    holder->workspace = ws;
+    holder->workspace_bytes = need;
     rc = launch(&a, stream);
     if (ws != nullptr) c10::hip::HIPCachingAllocator::raw_delete(ws);
     if (rc != PTO_OK) return raise_status(rc);
     Py_RETURN_TRUE;
+}
+
+template <typename Args, typename Bytes, typename Launch>
+PyObject *enqueue(const c10::Device &device, Args &a, Bytes bytes, Launch launch)
+{
+    return enqueue(device, a, bytes, launch, &a);
 }
 
 // every exception of torch's accessors (a tensor subclass without storage, an allocator that is out of memory) leaves
@@ -575,49 +582,176 @@ PyObject *cache_read_call(PyObject *, PyObject *const *args, Py_ssize_t n)
 }
 
 // query, key, value, cu_seqlens_q, cu_seqlens_k, attention_out, softmax_scale, query_rope, key_rope, softmax_lse (each or
-// None), causal
+// None): whether they are taken as they are
+bool prompt_args(Call &c, PyObject *const *args, PtoPromptAttentionArgs &a)
+{
+    a.softmax_scale = static_cast<float>(c.real(6));
+    const at::Tensor &q = c.tensor(0, true), &cu_q = c.of(3, I32), &cu_k = c.of(4, I32);
+    if (!c.ok || !dims(q, 3) || !dims(cu_q, 1) || !dims(cu_k, 1) || cu_q.size(0) != cu_k.size(0) || cu_q.size(0) < 2) return false;
+    const c10::ScalarType type = q.scalar_type();
+    if (type != BF16 && type != FP16) return false;
+    a.d = q.size(2);
+    c.rows_of(0, type);
+    const at::Tensor &k = c.rows_of(1, type, a.d), &v = c.rows_of(2, type, a.d), &out = c.rows_of(5, type, a.d);
+    if (!c.ok || !dims(k, 3) || k.sizes() != v.sizes() || out.sizes() != q.sizes() || !writable(out) || clash_any(out, {&q, &k, &v, &cu_q, &cu_k}) ||
+        c.none(7) != c.none(8))
+        return false;
+    a.fp16 = type == FP16;
+    a.b = cu_q.size(0) - 1, a.total_q = q.size(0), a.total_k = k.size(0), a.heads = q.size(1), a.kv_heads = k.size(1);
+    a.query_stride_t = row_stride(q), a.query_stride_h = head_stride(q), a.key_stride_t = row_stride(k), a.key_stride_h = head_stride(k);
+    a.value_stride_t = row_stride(v), a.value_stride_h = head_stride(v), a.out_stride_t = row_stride(out), a.out_stride_h = head_stride(out);
+    if (!c.none(7)) {
+        const at::Tensor &qr = c.rows_of(7, type, 64), &kr = c.rows_of(8, type, 64);
+        if (!c.ok || !dims(qr, 3) || qr.size(0) != a.total_q || qr.size(1) != a.heads || kr.size(0) != a.total_k ||
+            (heads_of(kr) != 1 && heads_of(kr) != a.kv_heads) || clash(out, qr) || clash(out, kr))
+            return false;
+        alignas(16) static char none_there[16];                   // (an empty tensor may have no memory)
+        a.query_rope = qr.numel() > 0 ? c.ptr<void>(qr) : none_there, a.query_rope_stride_t = row_stride(qr), a.query_rope_stride_h = head_stride(qr);
+        a.key_rope = kr.numel() > 0 ? c.ptr<void>(kr) : none_there, a.key_rope_stride_t = row_stride(kr), a.key_rope_stride_h = head_stride(kr);
+    }
+    if (!c.none(9)) {
+        const at::Tensor &lse = c.shaped(9, FP32, {a.total_q, a.heads});
+        if (!c.ok || clash_any(lse, {&out, &q, &k, &v, &cu_q, &cu_k})) return false;
+        if (!c.none(7) && (clash(lse, c.tensor(7, true)) || clash(lse, c.tensor(8, true)))) return false;
+        a.lse = c.out<float>(lse);
+    }
+    a.query = c.ptr<void>(q), a.key = c.ptr<void>(k), a.value = c.ptr<void>(v), a.out = c.out<void>(out);
+    a.cu_seqlens_q = c.ptr<int32_t>(cu_q), a.cu_seqlens_k = c.ptr<int32_t>(cu_k);
+    return c.ok;
+}
+
+// ... and causal
 PyObject *prompt_attention_call(PyObject *, PyObject *const *args, Py_ssize_t n)
 {
-    if (n != 11) return declined();
+    if (n != 11 || (args[10] != Py_True && args[10] != Py_False)) return declined();
     return guarded([&]() -> PyObject * {
         Call c{args};
         PtoPromptAttentionArgs a{};
-        a.softmax_scale = static_cast<float>(c.real(6));
-        if (args[10] != Py_True && args[10] != Py_False) return declined();
         a.causal = args[10] == Py_True;
-        const at::Tensor &q = c.tensor(0, true), &cu_q = c.of(3, I32), &cu_k = c.of(4, I32);
-        if (!c.ok || !dims(q, 3) || !dims(cu_q, 1) || !dims(cu_k, 1) || cu_q.size(0) != cu_k.size(0) || cu_q.size(0) < 2) return declined();
-        const c10::ScalarType type = q.scalar_type();
-        if (type != BF16 && type != FP16) return declined();
-        a.d = q.size(2);
-        c.rows_of(0, type);
-        const at::Tensor &k = c.rows_of(1, type, a.d), &v = c.rows_of(2, type, a.d), &out = c.rows_of(5, type, a.d);
-        if (!c.ok || !dims(k, 3) || k.sizes() != v.sizes() || out.sizes() != q.sizes() || !writable(out) || clash_any(out, {&q, &k, &v, &cu_q, &cu_k}) ||
-            c.none(7) != c.none(8))
+        if (!prompt_args(c, args, a)) return declined();
+        return enqueue(c.device, a, pto_prompt_attention_workspace_bytes, pto_prompt_attention_launch);
+    });
+}
+
+// ... and window, sinks
+PyObject *prompt_window_call(PyObject *, PyObject *const *args, Py_ssize_t n)
+{
+    if (n != 12) return declined();
+    return guarded([&]() -> PyObject * {
+        Call c{args};
+        PtoPromptWindowArgs a{};
+        a.prompt.causal = 1;
+        a.window = c.integer(10), a.sinks = c.integer(11);
+        if (!prompt_args(c, args, a.prompt)) return declined();
+        return enqueue(c.device, a, pto_prompt_window_workspace_bytes, pto_prompt_window_launch, &a.prompt);
+    });
+}
+
+// lens_before, lens_after, block_table, free_pages, free_count, free_left, block_size
+PyObject *cache_pages_call(PyObject *, PyObject *const *args, Py_ssize_t n)
+{
+    if (n != 7) return declined();
+    return guarded([&]() -> PyObject * {
+        Call c{args};
+        PtoCachePagesArgs a{};
+        a.block_size = c.integer(6);
+        const at::Tensor &before = c.of(0, I32), &after = c.of(1, I32), &bt = c.of(2, I32), &pages = c.of(3, I32), &count = c.of(4, I32, 1), &left = c.of(5, I32, 1);
+        if (!c.ok || !dims(before, 1) || !dims(after, 1) || !dims(bt, 2) || !dims(pages, 1) || before.size(0) < 1 || after.size(0) != before.size(0) ||
+            bt.size(0) != before.size(0) || clash_any(bt, {&before, &after, &pages, &count, &left}) || clash_any(pages, {&before, &after, &count, &left}) ||
+            clash_any(left, {&before, &after}) || (left.const_data_ptr() != count.const_data_ptr() && clash(left, count)))
             return declined();
-        a.fp16 = type == FP16;
-        a.b = cu_q.size(0) - 1, a.total_q = q.size(0), a.total_k = k.size(0), a.heads = q.size(1), a.kv_heads = k.size(1);
-        a.query_stride_t = row_stride(q), a.query_stride_h = head_stride(q), a.key_stride_t = row_stride(k), a.key_stride_h = head_stride(k);
-        a.value_stride_t = row_stride(v), a.value_stride_h = head_stride(v), a.out_stride_t = row_stride(out), a.out_stride_h = head_stride(out);
-        if (!c.none(7)) {
-            const at::Tensor &qr = c.rows_of(7, type, 64), &kr = c.rows_of(8, type, 64);
-            if (!c.ok || !dims(qr, 3) || qr.size(0) != a.total_q || qr.size(1) != a.heads || kr.size(0) != a.total_k ||
-                (heads_of(kr) != 1 && heads_of(kr) != a.kv_heads) || clash(out, qr) || clash(out, kr))
-                return declined();
-            alignas(16) static char none_there[16];                   // (an empty tensor may have no memory)
-            a.query_rope = qr.numel() > 0 ? c.ptr<void>(qr) : none_there, a.query_rope_stride_t = row_stride(qr), a.query_rope_stride_h = head_stride(qr);
-            a.key_rope = kr.numel() > 0 ? c.ptr<void>(kr) : none_there, a.key_rope_stride_t = row_stride(kr), a.key_rope_stride_h = head_stride(kr);
+        a.b = before.size(0), a.max_blocknum_perbatch = bt.size(1), a.room = pages.size(0);
+        a.block_table = c.out<int32_t>(bt), a.free_pages = c.out<int32_t>(pages), a.free_left = c.out<int32_t>(left);
+        a.lens_before = c.ptr<int32_t>(before), a.lens_after = c.ptr<int32_t>(after), a.free_count = c.ptr<int32_t>(count);
+        if (!c.ok) return declined();
+        return enqueue_without_workspace(c.device, a, pto_cache_pages_launch);
+    });
+}
+
+// query_lens, seq_lens, block_table, cu_seqlens_q, cu_seqlens_k (or None), positions, cache_index, block_size, parents, tree_mask (or None both)
+PyObject *cache_slots_call(PyObject *, PyObject *const *args, Py_ssize_t n)
+{
+    if (n != 10) return declined();
+    return guarded([&]() -> PyObject * {
+        Call c{args};
+        PtoCacheSlotsArgs a{};
+        a.block_size = c.integer(7);
+        const at::Tensor &ql = c.of(0, I32), &sl = c.of(1, I32), &bt = c.of(2, I32), &cu_q = c.of(3, I32), &pos = c.of(5, I64), &index = c.of(6, I64);
+        if (!c.ok || !dims(ql, 1) || !dims(sl, 1) || !dims(bt, 2) || !dims(cu_q, 1) || !dims(pos, 1) || !dims(index, 1) || ql.size(0) < 1 || sl.size(0) != ql.size(0) ||
+            bt.size(0) != ql.size(0) || cu_q.size(0) != ql.size(0) + 1 || index.size(0) != pos.size(0) || c.none(8) != c.none(9))
+            return declined();
+        const at::Tensor *out[5] = {&cu_q, &pos, &index}, *in[4] = {&ql, &sl, &bt};
+        int outs = 3, ins = 3;
+        if (!c.none(4)) {
+            const at::Tensor &cu_k = c.shaped(4, I32, {cu_q.size(0)});
+            if (!c.ok) return declined();
+            out[outs++] = &cu_k;
         }
-        if (!c.none(9)) {
-            const at::Tensor &lse = c.shaped(9, FP32, {a.total_q, a.heads});
-            if (!c.ok || clash_any(lse, {&out, &q, &k, &v, &cu_q, &cu_k})) return declined();
-            if (!c.none(7) && (clash(lse, c.tensor(7, true)) || clash(lse, c.tensor(8, true)))) return declined();
+        if (!c.none(8)) {
+            const at::Tensor &parents = c.shaped(8, I32, {pos.size(0)}), &mask = c.of(9, I64);
+            if (!c.ok || !dims(mask, 2) || mask.size(0) != pos.size(0)) return declined();
+            in[ins++] = &parents, out[outs++] = &mask;
+            a.mask_words = mask.size(1);
+        }
+        for (int i = 0; i < outs; ++i) {
+            for (int j = 0; j < ins; ++j)
+                if (clash(*out[i], *in[j])) return declined();
+            for (int j = 0; j < i; ++j)
+                if (clash(*out[i], *out[j])) return declined();
+        }
+        a.b = ql.size(0), a.t = pos.size(0), a.max_blocknum_perbatch = bt.size(1);
+        a.cu_seqlens_q = c.out<int32_t>(cu_q), a.positions = c.out<int64_t>(pos), a.cache_index = c.out<int64_t>(index);
+        if (!c.none(4)) a.cu_seqlens_k = c.out<int32_t>(*out[3]);
+        if (!c.none(8)) a.parents = c.ptr<int32_t>(*in[3]), a.tree_mask = c.out<int64_t>(*out[outs - 1]);
+        a.query_lens = c.ptr<int32_t>(ql), a.seq_lens = c.ptr<int32_t>(sl), a.block_table = c.ptr<int32_t>(bt);
+        if (!c.ok) return declined();
+        return enqueue_without_workspace(c.device, a, pto_cache_slots_launch);
+    });
+}
+
+// query_nope, query_rope, nope, rope, scales (or packed, None, None), block_table, cu_seqlens_q, seq_lens, attention_out, softmax_scale,
+// block_size, window (0: none), sinks, tree_mask, softmax_lse (each or None)
+PyObject *latent_attention_call(PyObject *, PyObject *const *args, Py_ssize_t n)
+{
+    if (n != 15) return declined();
+    return guarded([&]() -> PyObject * {
+        Call c{args};
+        PtoLatentAttentionArgs a{};
+        a.softmax_scale = static_cast<float>(c.real(9));
+        a.block_size = c.integer(10), a.window = c.integer(11), a.sinks = c.integer(12);
+        const at::Tensor &qn = c.rows_of(0, BF16, 512), &qr = c.rows_of(1, BF16, 64), &out = c.rows_of(8, BF16, 512);
+        const at::Tensor *parts[3];
+        if (!c.ok || !cache_args(c, 2, parts, a.cache_rows, a.packed)) return declined();
+        const at::Tensor &bt = c.of(5, I32), &cu = c.of(6, I32), &lens = c.of(7, I32);
+        if (!c.ok || !dims(qn, 3) || !dims(qr, 3) || qr.size(0) != qn.size(0) || qr.size(1) != qn.size(1) || out.sizes() != qn.sizes() || !dims(bt, 2) ||
+            !dims(cu, 1) || !dims(lens, 1) || lens.size(0) < 1 || bt.size(0) != lens.size(0) || cu.size(0) != lens.size(0) + 1 || !writable(out) ||
+            clash_any(out, {&qn, &qr, &bt, &cu, &lens}))
+            return declined();
+        a.b = lens.size(0), a.total_q = qn.size(0), a.heads = qn.size(1), a.max_blocknum_perbatch = bt.size(1);
+        for (const at::Tensor *p : parts)
+            if (p && clash(out, *p)) return declined();
+        const at::Tensor *mask = nullptr;
+        if (!c.none(13)) {
+            mask = &c.of(13, I64);
+            if (!c.ok || !dims(*mask, 2) || mask->size(0) != a.total_q || clash(out, *mask)) return declined();
+            alignas(16) static int64_t none_there[2];                 // (an empty tensor may have no memory)
+            a.tree_mask = mask->numel() > 0 ? c.ptr<int64_t>(*mask) : none_there, a.mask_words = mask->size(1);
+        }
+        if (!c.none(14)) {
+            const at::Tensor &lse = c.shaped(14, FP32, {a.total_q, a.heads});
+            if (!c.ok || clash_any(lse, {&out, &qn, &qr, &bt, &cu, &lens}) || (mask && clash(lse, *mask))) return declined();
+            for (const at::Tensor *p : parts)
+                if (p && clash(lse, *p)) return declined();
             a.lse = c.out<float>(lse);
         }
-        a.query = c.ptr<void>(q), a.key = c.ptr<void>(k), a.value = c.ptr<void>(v), a.out = c.out<void>(out);
-        a.cu_seqlens_q = c.ptr<int32_t>(cu_q), a.cu_seqlens_k = c.ptr<int32_t>(cu_k);
+        a.query_nope_stride_t = row_stride(qn), a.query_nope_stride_h = head_stride(qn), a.query_rope_stride_t = row_stride(qr), a.query_rope_stride_h = head_stride(qr);
+        a.out_stride_t = row_stride(out), a.out_stride_h = head_stride(out);
+        a.query_nope = c.ptr<void>(qn), a.query_rope = c.ptr<void>(qr), a.out = c.out<void>(out);
+        a.nope = c.ptr<void>(*parts[0]);
+        if (!a.packed) a.rope_cache = c.ptr<void>(*parts[1]), a.scales = c.ptr<void>(*parts[2]);
+        a.block_table = c.ptr<int32_t>(bt), a.cu_seqlens_q = c.ptr<int32_t>(cu), a.seq_lens = c.ptr<int32_t>(lens);
         if (!c.ok) return declined();
-        return enqueue(c.device, a, pto_prompt_attention_workspace_bytes, pto_prompt_attention_launch);
+        return enqueue(c.device, a, pto_latent_attention_workspace_bytes, pto_latent_attention_launch);
     });
 }
 
@@ -640,7 +774,8 @@ PyObject *set_wrapper(PyObject *, PyObject *const *args, Py_ssize_t n)
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST(sfa_call),       FAST(sa_antiquant_call), FAST(li_decode_call), FAST(mla_prolog_call),
                          FAST(li_prolog_call), FAST(fused_prolog_call), FAST(set_wrapper),    FAST(rotary_tables_call),
-                         FAST(rotary_embedding_call), FAST(cache_write_call), FAST(cache_read_call), FAST(prompt_attention_call), {nullptr, nullptr, 0, nullptr}};
+                         FAST(rotary_embedding_call), FAST(cache_write_call), FAST(cache_read_call), FAST(prompt_attention_call),
+                         FAST(prompt_window_call), FAST(cache_pages_call), FAST(cache_slots_call), FAST(latent_attention_call), {nullptr, nullptr, 0, nullptr}};
 #undef FAST
 
 }  // namespace

@@ -43,6 +43,14 @@ def prompt_attention(query, key, value, cu_seqlens_q, cu_seqlens_k, attention_ou
     C = _native.load()
     if C.prompt_attention_call(query, key, value, cu_seqlens_q, cu_seqlens_k, attention_out, softmax_scale, query_rope, key_rope, softmax_lse, causal):
         return None
+    q, k, v, cu_q, cu_k, out, scale, qr, kr, lse = _checked("prompt_attention", query, key, value, cu_seqlens_q, cu_seqlens_k, attention_out, softmax_scale,
+                                                            query_rope, key_rope, softmax_lse)
+    if not C.prompt_attention_call(q, k, v, cu_q, cu_k, out, scale, qr, kr, lse, bool(causal)):
+        raise RuntimeError("prompt_attention: these arguments are not supported")
+    return None
+
+
+def _checked(op, query, key, value, cu_seqlens_q, cu_seqlens_k, attention_out, softmax_scale, query_rope, key_rope, softmax_lse):
     q, k, v, out = (as_rows(t, n) for t, n in ((query, "query"), (key, "key"), (value, "value"), (attention_out, "attention_out")))
     cu_q, cu_k = as_torch(cu_seqlens_q, "cu_seqlens_q"), as_torch(cu_seqlens_k, "cu_seqlens_k")
     if q.dtype not in (torch.bfloat16, torch.float16):
@@ -97,7 +105,34 @@ def prompt_attention(query, key, value, cu_seqlens_q, cu_seqlens_k, attention_ou
         refuse_overlap(out, t, f"attention_out and {n}")
     if not math.isfinite(float(softmax_scale)):
         raise ValueError("softmax_scale is not finite")
-    _on_gpu("prompt_attention", [t for t, _ in inputs] + [out] + ([lse] if lse is not None else []))
-    if not C.prompt_attention_call(q, k, v, cu_q, cu_k, out, float(softmax_scale), qr, kr, lse, bool(causal)):
-        raise RuntimeError("prompt_attention: these arguments are not supported")
+    _on_gpu(op, [t for t, _ in inputs] + [out] + ([lse] if lse is not None else []))
+    return q, k, v, cu_q, cu_k, out, float(softmax_scale), qr, kr, lse
+
+
+def prompt_window_attention(query, key, value, cu_seqlens_q, cu_seqlens_k, attention_out, softmax_scale, window, sinks=0, query_rope=None, key_rope=None,
+                            softmax_lse=None):
+    """The same with a window: of the keys up to its own a query sees the last ``window``, its own among them, and the first ``sinks`` of its sequence.
+
+    Arguments as for :func:`prompt_attention`, always causal.  Keys are counted within the sequence, so those that no query sees may as well be left out
+    of it: a chunk of n tokens needs the first ``sinks`` keys and the last ``n - 1 + window`` (read back by ``latent_cache_read``).  The time is
+    that of the keys seen, whatever lies between.
+    """
+    C = _native.load()
+    if window is None:
+        raise ValueError("window: expected a whole number from 1 to 2^30, got None")
+    check_window(window, sinks)
+    if C.prompt_window_call(query, key, value, cu_seqlens_q, cu_seqlens_k, attention_out, softmax_scale, query_rope, key_rope, softmax_lse, window, sinks):
+        return None
+    args = _checked("prompt_window_attention", query, key, value, cu_seqlens_q, cu_seqlens_k, attention_out, softmax_scale, query_rope, key_rope, softmax_lse)
+    if not C.prompt_window_call(*args, window, sinks):
+        raise RuntimeError("prompt_window_attention: these arguments are not supported")
     return None
+
+
+def check_window(window, sinks):
+    if window is not None and (not isinstance(window, int) or isinstance(window, bool) or not 1 <= window <= 1 << 30):
+        raise ValueError(f"window: expected a whole number from 1 to 2^30, got {window!r}")
+    if not isinstance(sinks, int) or isinstance(sinks, bool) or not 0 <= sinks <= 1 << 30:
+        raise ValueError(f"sinks: expected a whole number from 0 to 2^30, got {sinks!r}")
+    if sinks and window is None:
+        raise ValueError("sinks go with a window")
