@@ -398,13 +398,24 @@ __global__ __launch_bounds__(64 * W, 2) void prompt_attention_kernel(const PaPar
         auto softmax = [&](const int count) __attribute__((always_inline)) {
             const int t = tile_at(count);
             if (WINDOW && ((t + 1) * PA_KEYS > wave_least || (t * PA_KEYS < wave_from && (t + 1) * PA_KEYS > p.sinks))) {
+                // (without a branch for each score)
+                const int first = t * PA_KEYS + 4 * half;
+                if (t * PA_KEYS >= p.sinks) {
+                    const uint32_t span = (uint32_t)(sees - from);
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
+                    for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int key = t * PA_KEYS + 32 * h + 8 * (i >> 2) + 4 * half + (i & 3);
-                        if (key >= sees || (key < from && key >= p.sinks)) s[h][i] = -INFINITY;
-                    }
+                        for (int i = 0; i < 16; ++i) s[h][i] = (uint32_t)(first - from + 32 * h + 8 * (i >> 2) + (i & 3)) < span ? s[h][i] : -INFINITY;
+                } else {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const int key = first + 32 * h + 8 * (i >> 2) + (i & 3);
+                            const bool hidden = (key >= sees) | ((key < from) & (key >= p.sinks));
+                            s[h][i] = hidden ? -INFINITY : s[h][i];
+                        }
+                }
             } else if (!WINDOW && (t + 1) * PA_KEYS > wave_least) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
@@ -490,6 +501,18 @@ __global__ __launch_bounds__(64 * W, 2) void prompt_attention_kernel(const PaPar
             if (k_tile < t_end) request_keys(s1);
             if (late) pa_barrier();
             int t = t_begin;
+            auto idle = [&]() __attribute__((always_inline)) {
+                end_products();
+                request_next();
+                if (PHASED) pa_barrier();
+                turn();
+            };
+            // (nor, where the first keys do not stay visible, those in front of its own first window)
+            if (WINDOW && p.sinks == 0) {
+                int own_begin = from_of(wave_least) / PA_KEYS - skip;
+                own_begin = own_begin < own_end ? own_begin : own_end;
+                for (; t < own_begin; ++t) idle();
+            }
             if (t < own_end) {
                 products(yes, no, s0, s2);
                 end_products();
@@ -509,12 +532,7 @@ __global__ __launch_bounds__(64 * W, 2) void prompt_attention_kernel(const PaPar
                 }
                 products(no, yes, s0, s2);
             }
-            for (; t < t_end; ++t) {
-                end_products();
-                request_next();
-                if (PHASED) pa_barrier();
-                turn();
-            }
+            for (; t < t_end; ++t) idle();
             if (PHASED && !late) pa_barrier();                 // (as many as the other half)
         }
 
