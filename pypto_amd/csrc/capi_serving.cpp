@@ -49,11 +49,11 @@ int latent_check(const PtoLatentAttentionArgs *a)
 }
 
 struct LatentPlan {
-    int groups, by_tile, entries;
+    int most_tiles, groups, by_tile, entries;
     size_t o_bytes, ml_bytes, join_bytes;
 };
 
-// The device divides the work, since lengths are there.  Here only as many workgroups as there can be pieces of LA_LEAST tiles, one to a
+// The device divides the work, since lengths are there.  Here only as many workgroups as there can be pieces of LA_LEAST units, one to a
 // compute unit at most (a workgroup's LDS is most of one's), and memory for two pieces of each.
 LatentPlan latent_plan(const PtoLatentAttentionArgs *a)
 {
@@ -61,11 +61,13 @@ LatentPlan latent_plan(const PtoLatentAttentionArgs *a)
     const long long cus = cu_count() > 0 ? cu_count() : 256;
     const long long row_tiles = a->total_q * a->heads / pto::LA_ROWS + (a->b < a->total_q ? a->b : a->total_q);    // at most
     long long tiles = (a->max_blocknum_perbatch * a->block_size + pto::LA_KEYS - 1) / pto::LA_KEYS;
-    if (a->window > 0) {
-        const long long w = (a->window + a->sinks + pto::LA_ROWS) / pto::LA_KEYS + 4;
+    if (a->window > 0) {                                   // of a row tile's tokens, the window of the first to the last one's last key, and the first keys
+        const long long reach = a->window + (pto::LA_ROWS - 2) / a->heads + 1;
+        const long long w = (a->sinks + pto::LA_KEYS - 1) / pto::LA_KEYS + (reach + pto::LA_KEYS - 1) / pto::LA_KEYS + 1;
         tiles = w < tiles ? w : tiles;
     }
-    const double pieces = (double)row_tiles * (double)(tiles + pto::LA_OPEN) / (pto::LA_LEAST + pto::LA_OPEN);
+    pl.most_tiles = (int)tiles;
+    const double pieces = (double)row_tiles * (double)(tiles + pto::LA_OPEN) / pto::LA_LEAST;
     const long long groups = pieces < (double)cus ? (long long)pieces + 1 : cus;
     pl.groups = (int)((groups + 7) / 8 * 8);
     pl.by_tile = row_tiles <= pl.groups;
@@ -209,6 +211,10 @@ int pto_latent_attention_launch(const PtoLatentAttentionArgs *a, void *hip_strea
     p.words = a->tree_mask ? (int)a->mask_words : 0;
     p.window = (int)a->window;
     p.sinks = (int)a->sinks;
+    p.most_keys = (int)(a->max_blocknum_perbatch * a->block_size);
+    p.most_tiles = pl.most_tiles;
+    p.per_entry = (int)((a->b + pto::LA_THREADS - 1) / pto::LA_THREADS);
+    p.seq_entries = (int)((a->b + p.per_entry - 1) / p.per_entry);
     p.groups = pl.groups;
     p.by_tile = pl.by_tile;
     p.entries = pl.entries;

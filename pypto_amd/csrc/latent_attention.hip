@@ -15,6 +15,8 @@
 // which the workgroups divide evenly, an XCD's neighbouring pieces to neighbouring workgroups.  A boundary near a row tile's edge moves there.
 // Where one falls inside, both sides write their sums, maxima and 512 sums of products, in fp32, and a second launch joins them: two pieces at most
 // to a workgroup, so the memory for them does not depend on lengths, which the host does not know.
+#include <type_traits>
+
 #include "common.h"
 #include "serving_ops.h"
 
@@ -36,7 +38,7 @@ constexpr float TAU = 8.0f;                               // log2 units: the ref
 constexpr float LOW = -1.7e38f;                           // reference maximum of a row that has seen no key yet
 constexpr int PIECE = LA_ROWS * DN;                       // floats of a piece's sums
 
-__device__ const u32x4 no_page[(DN + 2 * DR + 16) / 16] = {};   // what a key without a page reads
+__device__ const u32x4 no_page[4 * (DN + 2 * DR + 16) / 16] = {};      // what four keys without a page read, a whole row of the cache each
 
 // Row i of a tile's score operand (and of the score accumulator) is key tile_row_of(i) of the tile: the two middle bits of i move below its two
 // lowest.  A transposing V^T read then addresses keys r, r+4, r+8, r+12 with each of its half-waves, four rows whose 64-byte pieces lie
@@ -83,88 +85,86 @@ __device__ __forceinline__ uint32_t opaque(uint32_t x)
     return x;
 }
 template <typename T>
-__device__ __forceinline__ T global(const uint64_t at)
+__device__ __forceinline__ T global(const uint8_t *base, const uint32_t offset)
 {
-    return *(const __attribute__((address_space(1))) T *)(at);
+    return *(const __attribute__((address_space(1))) T *)((const __attribute__((address_space(1))) uint8_t *)base + offset);
 }
-__device__ __forceinline__ long long lane_of(const long long x, const int from)
+// a scalar load, of what no launch that this one may run beside writes
+template <typename T>
+__device__ __forceinline__ T constant(const T *at)
 {
-    return (long long)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)x, from) | ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), from) << 32));
+    return *(const __attribute__((address_space(4))) T *)at;
+}
+// sums of x over this lane and all lanes before it
+__device__ __forceinline__ long long wave_sums(long long x)
+{
+    auto add = [&](auto ctrl, auto rows) __attribute__((always_inline)) {
+        const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)x, decltype(ctrl)::value, decltype(rows)::value, 0xf, false);
+        const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)((uint64_t)x >> 32), decltype(ctrl)::value, decltype(rows)::value, 0xf, false);
+        x += (long long)((uint64_t)lo | ((uint64_t)hi << 32));
+    };
+    const std::integral_constant<int, 0xf> all;
+    add(std::integral_constant<int, 0x111>{}, all);        // row_shr:1, 2, 4, 8: within rows of sixteen lanes
+    add(std::integral_constant<int, 0x112>{}, all);
+    add(std::integral_constant<int, 0x114>{}, all);
+    add(std::integral_constant<int, 0x118>{}, all);
+    add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});     // row_bcast:15: rows 0 and 2 into 1 and 3
+    add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});     // row_bcast:31: the lower half into the upper
+    return x;
+}
+__device__ __forceinline__ long long first_of(const long long x)
+{
+    return (long long)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)x) | ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32));
 }
 
-// 64 sequences, one to a lane, as the kernel takes them: whatever the tables say, inside the tensors.
-struct Sequences {
+// A sequence as the kernel takes it: whatever the tables say, inside the tensors.
+struct Sequence {
     int q0, n, keys;                                       // first token, tokens, keys
     int tiles, row_tiles;                                  // units of a row tile but LA_OPEN; row tiles
-    long long upto;                                        // units of this sequence and all before it (of these 64)
-    int tiles_upto;                                        // row tiles, the same
 };
-__device__ __forceinline__ Sequences sequences_from(const LaParams &p, const int base)
+__device__ __forceinline__ void count_tiles(const LaParams &p, Sequence &c)
 {
-    Sequences c;
-    const int b = base + (threadIdx.x & 63), in = b < p.B ? b : p.B - 1;
+    c.row_tiles = (c.n * p.heads + LA_ROWS - 1) / LA_ROWS;
+    c.tiles = (c.keys + KT - 1) / KT;
+    c.tiles = c.tiles < p.most_tiles ? c.tiles : p.most_tiles;
+}
+__device__ __forceinline__ Sequence sequence(const LaParams &p, const int b)
+{
+    Sequence c;
     const int total = (int)p.total_q;
-    int lo = p.cu_q[in], hi = p.cu_q[in + 1], keys = p.lens[in];
+    int lo = p.cu_q[b], hi = p.cu_q[b + 1], keys = p.lens[b];
     lo = lo < 0 ? 0 : (lo > total ? total : lo);
     hi = hi < lo ? lo : (hi > total ? total : hi);
-    const long long most = (long long)p.maxblk * p.bs;
-    keys = keys < 0 ? 0 : (keys > most ? (int)most : keys);
+    keys = keys < 0 ? 0 : (keys > p.most_keys ? p.most_keys : keys);
     c.q0 = lo, c.n = hi - lo, c.keys = keys;
-    c.row_tiles = b < p.B ? (c.n * p.heads + LA_ROWS - 1) / LA_ROWS : 0;
-    c.tiles = (keys + KT - 1) / KT;
-    if (p.window > 0) {                                    // of a row tile's tokens, the window of the first to the last one's last key, and the first keys
-        const long long reach = (long long)p.window + (LA_ROWS - 2) / p.heads + 1;
-        const long long w = (p.sinks + KT - 1) / KT + (reach + KT - 1) / KT + 1;
-        c.tiles = w < c.tiles ? (int)w : c.tiles;
-    }
-    c.upto = (long long)c.row_tiles * (c.tiles + LA_OPEN);
-    c.tiles_upto = c.row_tiles;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const uint32_t ylo = __shfl_up((uint32_t)c.upto, d), yhi = __shfl_up((uint32_t)((uint64_t)c.upto >> 32), d);
-        const int t = __shfl_up(c.tiles_upto, d);
-        if ((int)(threadIdx.x & 63) >= d) c.upto += (long long)((uint64_t)ylo | ((uint64_t)yhi << 32)), c.tiles_upto += t;
-    }
+    count_tiles(p, c);
     return c;
 }
 
-// The row tile that unit u is in.
+// x / d for 0 <= x < 2^51, d >= 1 and a quotient below 2^31: of the product with 1 / d the whole part is off by one at most
+__device__ __forceinline__ int quotient(const long long x, const int d)
+{
+    int q = (int)((double)x * (1.0 / (double)d));
+    if ((long long)q * d > x) --q;
+    if ((long long)(q + 1) * d <= x) ++q;
+    return q;
+}
+
+// The row tile that a unit is in.
 struct Place {
     int b, q0, n, keys, tiles, row_tile, ordinal;          // ordinal: among the row tiles of all sequences
     long long begin;                                       // its first unit
 };
-__device__ __forceinline__ Place place_of(const LaParams &p, const long long u)
-{
-    // (looked up anew each time: kept from one row tile to the next, the 64 sequences would take the registers of the products' operands)
-    Sequences c = sequences_from(p, 0);
-    int base = 0, tiles_before = 0;
-    long long before = 0;
-    for (;;) {
-        const long long here = lane_of(c.upto, 63);
-        if (u < before + here || base + 64 >= p.B) break;
-        before += here;
-        tiles_before += __builtin_amdgcn_readlane(c.tiles_upto, 63);
-        base += 64;
-        c = sequences_from(p, base);
-    }
-    const uint64_t behind = __ballot(c.upto > u - before);
-    const int who = behind ? __builtin_ctzll(behind) : 63;
-    Place at;
-    at.b = base + who;
-    at.q0 = __builtin_amdgcn_readlane(c.q0, who), at.n = __builtin_amdgcn_readlane(c.n, who);
-    at.keys = __builtin_amdgcn_readlane(c.keys, who), at.tiles = __builtin_amdgcn_readlane(c.tiles, who);
-    const long long first = before + (who > 0 ? lane_of(c.upto, who - 1) : 0);
-    at.row_tile = (int)((u - first) / (at.tiles + LA_OPEN));
-    at.ordinal = tiles_before + (who > 0 ? __builtin_amdgcn_readlane(c.tiles_upto, who - 1) : 0) + at.row_tile;
-    at.begin = first + (long long)at.row_tile * (at.tiles + LA_OPEN);
-    return at;
-}
 
 // A boundary `x` units into a row tile of `len`, moved to its edge where that is near.
 constexpr int NEAR_BEGIN = LA_OPEN + 3, NEAR_END = 3;
 __device__ __forceinline__ int moved(const int x, const int len) { return x <= NEAR_BEGIN ? 0 : (x >= len - NEAR_END ? len : x); }
 
-__global__ __launch_bounds__(512) void latent_attention_kernel(const LaParams p)
+constexpr int THREADS = LA_THREADS;
+
+// QUADS: pages and the cache hold whole fours of rows.
+template <bool QUADS>
+__global__ __launch_bounds__(THREADS) void latent_attention_kernel(const LaParams p)
 {
     __shared__ __attribute__((aligned(16))) uint8_t pool[POOL];
 
@@ -174,15 +174,59 @@ __global__ __launch_bounds__(512) void latent_attention_kernel(const LaParams p)
     const int kh = w >> 2;                                 // the half kh of the tile's keys
     const uint32_t pool_lds = (uint32_t)(uintptr_t)(lds_byte_t *)pool;
 
-    long long units = 0;
-    int row_tiles = 0;
-    for (int base = 0; base < p.B; base += 64) {
-        const Sequences c = sequences_from(p, base);
-        units += lane_of(c.upto, 63), row_tiles += __builtin_amdgcn_readlane(c.tiles_upto, 63);
+    // Units and row tiles of the sequences up to each: an entry to a thread, of as many sequences as that takes.
+    __shared__ long long upto[THREADS], of_waves[THREADS / 64];
+    __shared__ int tiles_upto[THREADS], tiles_of_waves[THREADS / 64];
+    __shared__ int seq_q0[THREADS], seq_n[THREADS], seq_keys[THREADS];         // of an entry's first sequence
+    const int per_entry = p.per_entry, entries = p.seq_entries;
+    {
+        long long mine = 0;
+        int row_tiles = 0;
+        for (int j = 0; j < per_entry; ++j) {
+            const int b = tid * per_entry + j;
+            if (b < p.B) {
+                const Sequence c = sequence(p, b);
+                if (j == 0) seq_q0[tid] = c.q0, seq_n[tid] = c.n, seq_keys[tid] = c.keys;
+                mine += (long long)c.row_tiles * (c.tiles + LA_OPEN), row_tiles += c.row_tiles;
+            }
+        }
+        mine = wave_sums(mine);
+        const long long both = wave_sums((long long)row_tiles);
+        if ((tid & 63) == 63) of_waves[w] = mine, tiles_of_waves[w] = (int)both;
+        __syncthreads();
+        int before = 0;
+        for (int i = 0; i < w; ++i) mine += of_waves[i], before += tiles_of_waves[i];
+        upto[tid] = mine;
+        tiles_upto[tid] = (int)both + before;
+        __syncthreads();
     }
-    // workgroups that take part, so that none gets less than LA_LEAST tiles and a beginning; this one's number among them
-    const long long pieces = units / (LA_LEAST + LA_OPEN);
-    const int groups = pieces < 1 ? 1 : (pieces < p.groups ? (int)pieces : p.groups);
+    const long long units = first_of(upto[THREADS - 1]);
+    const int row_tiles = __builtin_amdgcn_readfirstlane(tiles_upto[THREADS - 1]);
+    auto place_of = [&](const long long u) __attribute__((always_inline)) {
+        int e = 0;                                         // entries that end in front of u
+        for (int i = 0; i < entries; i += 64) e += __popcll(__ballot(upto[i + (tid & 63)] <= u));
+        long long first = e > 0 ? first_of(upto[e - 1]) : 0;
+        int tiles_before = e > 0 ? __builtin_amdgcn_readfirstlane(tiles_upto[e - 1]) : 0;
+        Place at;
+        at.b = e * per_entry;
+        Sequence c;
+        c.q0 = __builtin_amdgcn_readfirstlane(seq_q0[e]), c.n = __builtin_amdgcn_readfirstlane(seq_n[e]), c.keys = __builtin_amdgcn_readfirstlane(seq_keys[e]);
+        count_tiles(p, c);
+        for (int j = 1; j < per_entry; ++j) {              // (only of more than THREADS sequences)
+            const long long next = first + (long long)c.row_tiles * (c.tiles + LA_OPEN);
+            if (next > u || at.b + 1 >= p.B) break;
+            first = next, tiles_before += c.row_tiles, ++at.b;
+            c = sequence(p, at.b);
+        }
+        at.q0 = c.q0, at.n = c.n, at.keys = c.keys, at.tiles = c.tiles;
+        at.row_tile = __builtin_amdgcn_readfirstlane(quotient(u - first, c.tiles + LA_OPEN));
+        at.ordinal = tiles_before + at.row_tile;
+        at.begin = first + (long long)at.row_tile * (c.tiles + LA_OPEN);
+        return at;
+    };
+    // workgroups that take part, so that none gets less than LA_LEAST units; this one's number among them
+    const long long most = (long long)p.groups * LA_LEAST;
+    const int pieces = units < most ? (int)units / LA_LEAST : p.groups, groups = pieces > 0 ? pieces : 1;
     const int per_xcd = (groups + 7) / 8, slot = blockIdx.x >> 3;
     const int g = (int)(blockIdx.x & 7) * per_xcd + slot;
     const bool there = slot < per_xcd && g < groups;
@@ -195,21 +239,32 @@ __global__ __launch_bounds__(512) void latent_attention_kernel(const LaParams p)
         }
     }
     if (!there) return;
-    auto boundary = [&](const int i) {
-        if (i >= groups) return units;
-        const long long raw = units * i / groups;
-        if (i == 0) return 0ll;
-        const Place at = place_of(p, raw);
-        return at.begin + moved((int)(raw - at.begin), at.tiles + LA_OPEN);
-    };
-    long long u = boundary(g);
-    const long long u_end = boundary(g + 1);
+    // the line's even divisions: units * i / groups
+    long long share = (long long)((double)units / (double)groups);
+    if (share * groups > units) --share;
+    const int rest = (int)(units - share * groups);
+    auto division = [&](const int i) { return share * i + (rest * i) / groups; };
+    long long u = 0, u_end = units, want = division(g + 1 < groups ? g + 1 : g);
+    int step = g + 1 < groups ? 0 : 1;                     // looked for: this workgroup's end, its beginning, the next row tile
     bool said = false;                                     // (not by_tile) this workgroup's entry is written
     bool first_segment = true;
 
-    while (u < u_end) {
+    while (units > 0) {
         const int l = (int)opaque(tid & 63), half = l >> 5, col = l & 31, l16 = l & 15, quarter = l >> 4;
-        const Place at = place_of(p, u);
+        const Place at = place_of(want);
+        if (step < 2) {
+            const long long edge = at.begin + moved((int)(want - at.begin), at.tiles + LA_OPEN);
+            if (step == 0) {
+                u_end = edge, want = division(g), step = 1;
+                continue;
+            }
+            u = edge, step = 2;
+            if (u >= u_end) break;
+            if (u == at.begin + at.tiles + LA_OPEN) {
+                want = u;
+                continue;
+            }
+        }
         const int len = at.tiles + LA_OPEN;
         const long long end = at.begin + len;
         const long long to = u_end < end ? u_end : end;
@@ -224,8 +279,10 @@ __global__ __launch_bounds__(512) void latent_attention_kernel(const LaParams p)
         if (tid == 0 && u == at.begin && (p.by_tile || !whole)) {
             int n = 0;
             if (!whole) {                                  // pieces: one more than there are boundaries inside, those before unit end - NEAR_END
-                const long long past = ((end - NEAR_END) * groups + units - 1) / units;
-                n = (int)(past < groups ? past : groups) - g;
+                const long long edge = end - NEAR_END;
+                n = (int)((double)edge * (double)groups / (double)units) - g;
+                n = n > 1 ? n - 1 : 1;
+                while (g + n < groups && division(g + n) < edge) ++n;
             }
             int32_t *const join = p.joins + 4 * (p.by_tile ? at.ordinal : (int)blockIdx.x);
             join[0] = piece, join[1] = n, join[2] = at.q0 * p.heads + row0, join[3] = rows - row0 < LA_ROWS ? rows - row0 : LA_ROWS;
@@ -285,56 +342,57 @@ __global__ __launch_bounds__(512) void latent_attention_kernel(const LaParams p)
                 dma16(p.qr + (long long)(at.q0 + tok) * p.qr_t + (long long)head * p.qr_h + 8 * ((l & 7) ^ (l >> 3)), pool_lds + Q_ROPE_AT + w * 1024);
             }
 
-            // Gather: wave w takes keys 4w .. 4w+3 of every tile, two rows per load, a lane 16 channels; the rope part of the four rows 8 bytes
-            // per lane.  Keys past the sequence's last one stand in with it: what lies behind it is never looked at.
+            // Gather: wave w takes keys 4w .. 4w+3 of every tile, a quarter of its lanes each, a lane 32 channels of the latents (one scale) and
+            // four of the rope part.  QUADS: the four are neighbours in the cache, so one scalar look-up and one address serve them.  Keys past
+            // the sequence's last one are those of the same four that are left in its page (their scores are hidden, and check_scales
+            // keeps what they hold out of the sums), else stand in with the last one.
             struct Raw {
                 u32x4 v[2];
-                float sc[2];
+                float sc;
                 u32x2 rope;
             };
             Raw raw[2];                                    // tile n in raw[n & 1]
-            const uint64_t nope_at = reinterpret_cast<uint64_t>(p.cache.nope), rope_at = reinterpret_cast<uint64_t>(p.cache.rope),
-                           scale_at = reinterpret_cast<uint64_t>(p.cache.scale), none = reinterpret_cast<uint64_t>(no_page);
-            int page, within;                              // of key 4w + l / 16 of the tile whose rows are asked for next
-            auto ask_page = [&](const int n) __attribute__((always_inline)) {
-                int key = key_of_tile(n) + 4 * w + quarter;
-                key = key < at.keys ? key : at.keys - 1;
-                const int block = divide(key, p.of_bs);
-                within = key - block * p.bs;
-                page = p.bt[(long long)at.b * p.maxblk + block];       // (at.keys is no more than the table's pages hold)
+            struct Page {
+                int page, within;
             };
-            auto gather = [&](Raw &r) __attribute__((always_inline)) {
-                const long long row_in = (long long)page * p.bs + within;
-                const int row = page >= 0 && row_in < p.cache.rows ? (int)row_in : -1;
-                int rows4[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) rows4[i] = __builtin_amdgcn_readlane(row, 16 * i);
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int mine = half ? rows4[2 * i + 1] : rows4[2 * i];
-                    const uint64_t v = mine >= 0 ? nope_at + (uint64_t)(uint32_t)mine * (uint32_t)p.cache.nope_pitch : none;
-                    const uint64_t sc = mine >= 0 ? scale_at + (uint64_t)(uint32_t)mine * (uint32_t)p.cache.scale_pitch : none;
-                    r.v[i] = global<u32x4>(v + 16 * col);
-                    r.sc[i] = global<float>(sc + 4 * (col >> 3));
-                }
-                r.rope = global<u32x2>((row >= 0 ? rope_at + (uint64_t)(uint32_t)row * (uint32_t)p.cache.rope_pitch : none) + 8 * l16);
+            auto page_of = [&](const int n) __attribute__((always_inline)) {
+                int key = key_of_tile(n) + 4 * w + (QUADS ? 0 : quarter);
+                const int last_key = QUADS ? (at.keys - 1) & ~3 : at.keys - 1;
+                key = key < last_key ? key : last_key;
+                const int block = divide(key, p.of_bs);    // (the block table has it: at.keys is no more than its pages hold)
+                const int32_t *const entry = p.bt + (long long)at.b * p.maxblk + block;
+                return Page{QUADS ? constant<int32_t>(entry) : *entry, key - block * p.bs};
+            };
+            const uint32_t rows_on = QUADS ? quarter : 0;
+            const uint32_t v_off = rows_on * (uint32_t)p.cache.nope_pitch + 32 * l16, sc_off = rows_on * (uint32_t)p.cache.scale_pitch + 4 * (l16 >> 2),
+                           rope_off = rows_on * (uint32_t)p.cache.rope_pitch + 8 * l16;
+            auto gather = [&](Raw &r, const Page k) __attribute__((always_inline)) {
+                const long long row = (long long)k.page * p.bs + k.within;
+                const bool there = k.page >= 0 && row < p.cache.rows;
+                const uint8_t *const none = reinterpret_cast<const uint8_t *>(no_page);
+                const uint8_t *const v = there ? p.cache.nope + row * p.cache.nope_pitch : none;
+                const uint8_t *const sc = there ? p.cache.scale + row * p.cache.scale_pitch : none;
+                const uint8_t *const rope = there ? p.cache.rope + row * p.cache.rope_pitch : none;
+                r.v[0] = global<u32x4>(v, v_off);
+                r.v[1] = global<u32x4>(v + 16, v_off);
+                r.sc = global<float>(sc, sc_off);
+                r.rope = global<u32x2>(rope, rope_off);
             };
             // A scale that is no number, or with which 127 steps are not finite, would be in the sums of rows that do not see the key (0 times it):
             // such a group's values become zeros and the key's rope channels, which are in scores alone, no numbers.  A row that sees the
             // key is then no number, others are not touched.
             auto check_scales = [&](Raw &r) __attribute__((always_inline)) {
-                const bool bad0 = !(fabsf(r.sc[0]) < 2.6e36f), bad1 = !(fabsf(r.sc[1]) < 2.6e36f);
-                const uint64_t any0 = __ballot(bad0), any1 = __ballot(bad1);
-                if (__builtin_expect((any0 | any1) != 0, 0)) {
-                    r.sc[0] = bad0 ? 0.f : r.sc[0], r.sc[1] = bad1 ? 0.f : r.sc[1];
-                    const uint64_t of = quarter & 2 ? any1 : any0;
-                    if ((uint32_t)(quarter & 1 ? of >> 32 : of) != 0) r.rope = u32x2{0x7fc07fc0u, 0x7fc07fc0u};
+                const bool bad = !(fabsf(r.sc) < 2.6e36f);
+                const uint64_t any = __ballot(bad);
+                if (__builtin_expect(any != 0, 0)) {
+                    r.sc = bad ? 0.f : r.sc;
+                    if (((any >> (16 * quarter)) & 0xffff) != 0) r.rope = u32x2{0x7fc07fc0u, 0x7fc07fc0u};
                 }
             };
             // The tile's rows into LDS, in eight pieces of a dword per lane and one of the rope channels.  Of a row's 64 latent pieces of eight
-            // channels the even ones come first, then the odd ones: a lane's sixteen channels are a piece of either half, and lanes next to
-            // each other write next to each other.
-            const uint32_t emit_off = (uint32_t)((4 * w + half) * PITCH + 16 * col);
+            // channels number 4 j + k lies at k * 16 + j: a lane's four pieces are one of each k, and lanes next to each other write next to
+            // each other.
+            const uint32_t emit_off = (uint32_t)((4 * w + quarter) * PITCH + 16 * l16);
             const uint32_t emit_rope_off = (uint32_t)((4 * w + quarter) * PITCH + DN * 2 + 8 * l16);
             u32x4 dq;
             auto emit = [&](Raw &r, const uint32_t tile, const int d) __attribute__((always_inline)) {
@@ -342,29 +400,27 @@ __global__ __launch_bounds__(512) void latent_attention_kernel(const LaParams p)
                 if (d == 8) {
                     *reinterpret_cast<u32x2 *>(pool + tile + emit_rope_off) = r.rope;
                 } else {
-                    const u32x2 x = dequant_dword(r.v[d >> 2][d & 3], r.sc[d >> 2]);
+                    const u32x2 x = dequant_dword(r.v[d >> 2][d & 3], r.sc);
                     if (d & 1) {
                         dq[2] = x[0], dq[3] = x[1];
-                        *reinterpret_cast<u32x4 *>(pool + tile + emit_off + (2 * (d >> 2)) * PITCH + 512 * ((d & 3) >> 1)) = dq;
+                        *reinterpret_cast<u32x4 *>(pool + tile + emit_off + 256 * (d >> 1)) = dq;
                     } else {
                         dq[0] = x[0], dq[1] = x[1];
                     }
                 }
             };
-            ask_page(0);
-            gather(raw[0]);
-            ask_page(1);
-            gather(raw[1]);
-            ask_page(2);
+            Page page = page_of(0), page1 = page_of(1), page2 = page_of(2), page3 = page_of(3);
+            gather(raw[0], page);
+            gather(raw[1], page1);
             // the waves' own queries have landed; those of the others when every wave has come here
             __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
             __syncthreads();
-            // Q^T: of the latent part lane (row, quarter) holds the channels of the tile rows' 16-byte pieces 16*quarter + ks, of
+            // Q^T: of the latent part lane (row, quarter) holds the channels of the tile rows' 16-byte pieces at 16*quarter + ks, of
             // the rope part channels 16*quarter + 8*ks .. +7
             bf16x8 qf[18];
 #pragma unroll
             for (int ks = 0; ks < 16; ++ks)
-                qf[ks] = *reinterpret_cast<const bf16x8 *>(pool + (16 * hq + l16) * (DN * 2) + 16 * ((32 * (quarter & 1) + 2 * ks + (quarter >> 1)) ^ l16));
+                qf[ks] = *reinterpret_cast<const bf16x8 *>(pool + (16 * hq + l16) * (DN * 2) + 16 * ((4 * ks + quarter) ^ l16));
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks)
                 qf[16 + ks] = *reinterpret_cast<const bf16x8 *>(pool + Q_ROPE_AT + (16 * hq + l16) * (DR * 2) + 16 * ((2 * quarter + ks) ^ (l16 & 7)));
@@ -381,8 +437,8 @@ __global__ __launch_bounds__(512) void latent_attention_kernel(const LaParams p)
             if (tid < 2) reinterpret_cast<int *>(pool + FLAG_AT)[tid] = -1;
 #pragma unroll
             for (int d = 0; d < 9; ++d) emit(raw[0], 2 * TILE, d);
-            gather(raw[0]);
-            ask_page(3);
+            gather(raw[0], page2);
+            page2 = page_of(4);
             __syncthreads();
 
             // Score operand: row `a` of the wave's sixteen is key tile_row_of(16*kh + a); the accumulator then holds in lane
@@ -460,7 +516,8 @@ __global__ __launch_bounds__(512) void latent_attention_kernel(const LaParams p)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int key = first + key_of[e];
-                        if (!(key < my_sees && (key >= my_from || key < p.sinks) && ((drafted >> key_of[e]) & 1))) sv[e] = -INFINITY;
+                        const bool seen = (key < my_sees) & ((key >= my_from) | (key < p.sinks)) & (((drafted >> key_of[e]) & 1) != 0);
+                        sv[e] = seen ? sv[e] : -INFINITY;          // (without a branch for each score)
                     }
                 }
                 mx = fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3]));
@@ -500,6 +557,7 @@ __global__ __launch_bounds__(512) void latent_attention_kernel(const LaParams p)
             // tile of r goes into buffer `next`, the rows of the tile two further are asked for, and the pages of the one behind it
             auto values = [&](auto next_tag, const int n4, const uint32_t prev, const uint32_t next, Raw &r, const int pbuf) __attribute__((always_inline)) {
                 constexpr bool NEXT = decltype(next_tag)::value;
+                Page further;
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int mp = 0; mp < 8; ++mp) {
@@ -508,9 +566,10 @@ __global__ __launch_bounds__(512) void latent_attention_kernel(const LaParams p)
                     __builtin_amdgcn_sched_barrier(0);
                     if (mp == 0) load_v(prev, 1, 0), load_p(pbuf, 1, 0);
                     if (mp == 1) load_v(prev, 1, 1), load_p(pbuf, 1, 1);
-                    if (NEXT) {
+                    if (NEXT) {                            // (pages before rows: loads come back in order)
                         emit(r, next, mp);
-                        if (mp == 7) emit(r, next, 8), gather(r), ask_page(n4);
+                        if (mp == 4) further = page_of(n4);
+                        if (mp == 7) emit(r, next, 8), gather(r, page), page = further;
                     }
                     __builtin_amdgcn_sched_barrier(0);
                 }
@@ -552,8 +611,8 @@ __global__ __launch_bounds__(512) void latent_attention_kernel(const LaParams p)
             scores(cur);
 #pragma unroll
             for (int d = 0; d < 9; ++d) emit(raw[1], next, d);
-            gather(raw[1]);
-            ask_page(4);
+            gather(raw[1], page3);
+            page = page2;                                  // of tile n + 3
             take_scores(0);
             move_maxima(0, true);
             prev = cur;
@@ -609,7 +668,7 @@ __global__ __launch_bounds__(512) void latent_attention_kernel(const LaParams p)
                     for (int q4 = 0; q4 < 4; ++q4) {
                         const f32x16 &a = o[2 * hb + d];
                         const u32x2 pk = {pack_bf16x2(a[4 * q4] * iv, a[4 * q4 + 1] * iv), pack_bf16x2(a[4 * q4 + 2] * iv, a[4 * q4 + 3] * iv)};
-                        const int chunk = 16 * (w & 3) + 2 * (4 * d + q4) + (w >> 2);            // of the row, in channel order
+                        const int chunk = 32 * (w & 1) + 4 * (4 * d + q4) + (w >> 1);            // of the row, in channel order
                         *reinterpret_cast<u32x2 *>(pool + (32 * hb + col) * (DN * 2) + 16 * (chunk ^ col) + 8 * half) = pk;
                     }
             }
@@ -627,8 +686,9 @@ __global__ __launch_bounds__(512) void latent_attention_kernel(const LaParams p)
             }
         }
         __syncthreads();                                   // (the next row tile's queries go over these)
-        u = to;
+        u = want = to;
         first_segment = false;
+        if (u >= u_end) break;
     }
     if (!p.by_tile && tid == 0 && !said) p.joins[4 * blockIdx.x + 1] = 0;
 }
@@ -688,7 +748,7 @@ __global__ __launch_bounds__(256) void latent_join_kernel(const LaParams p)
     uint16_t *dst = p.out + (long long)tok * p.o_t + (long long)head * p.o_h;
 #pragma unroll
     for (int q4 = 0; q4 < 4; ++q4) {
-        const int chunk = 16 * (w & 3) + 2 * (4 * d + q4) + (w >> 2);
+        const int chunk = 32 * (w & 1) + 4 * (4 * d + q4) + (w >> 1);
         *reinterpret_cast<u32x2_a2 *>(dst + 8 * chunk + 4 * half) =
             u32x2{pack_bf16x2(acc[q4][0] * inv, acc[q4][1] * inv), pack_bf16x2(acc[q4][2] * inv, acc[q4][3] * inv)};
     }
@@ -698,7 +758,8 @@ __global__ __launch_bounds__(256) void latent_join_kernel(const LaParams p)
 
 hipError_t latent_attention_launch(const LaParams &p, hipStream_t stream)
 {
-    hipLaunchKernelGGL(latent_attention_kernel, dim3((unsigned)p.groups), dim3(512), 0, stream, p);
+    if (p.bs % 4 == 0 && p.cache.rows % 4 == 0) hipLaunchKernelGGL((latent_attention_kernel<true>), dim3((unsigned)p.groups), dim3(THREADS), 0, stream, p);
+    else hipLaunchKernelGGL((latent_attention_kernel<false>), dim3((unsigned)p.groups), dim3(THREADS), 0, stream, p);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL(latent_join_kernel, dim3((unsigned)p.entries * 32), dim3(256), 0, stream, p);

@@ -54,7 +54,8 @@ hipError_t cache_slots_launch(const CacheSlotsParams &p, hipStream_t stream);
 constexpr int LA_ROWS = 64;               // (token, head) rows of a workgroup
 constexpr int LA_KEYS = 32;               // keys of a tile
 constexpr int LA_OPEN = 6;                // what a row tile's beginning and end cost, in tiles
-constexpr int LA_LEAST = 8;               // tiles of the shortest piece that keys are divided into
+constexpr int LA_THREADS = 512;          // of a workgroup
+constexpr int LA_LEAST = 6;               // units of the shortest piece that the line is divided into
 
 struct LaParams {
     const uint16_t *q, *qr;               // [total_q, heads, 512], [total_q, heads, 64] bf16
@@ -71,6 +72,8 @@ struct LaParams {
     long long total_q;
     int B, maxblk, bs, heads, words;
     int window, sinks;                    // window 0: all keys
+    int most_keys, most_tiles;            // of a sequence, as the block table and the window have it
+    int per_entry, seq_entries;           // sequences that a workgroup's thread counts; threads that count any
     int groups;                           // workgroups, a multiple of eight
     int by_tile, entries;                 // joins by row tile (of all sequences), else by workgroup; how many there are
     Divisor of_heads, of_bs;
