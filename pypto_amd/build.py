@@ -17,7 +17,7 @@ EXT_PATH = os.path.join(HERE, "_C" + (sysconfig.get_config_var("EXT_SUFFIX") or 
 
 HIP_SOURCES = ["sfa_kernels.hip", "li_kernels.hip", "lip_kernels.hip", "mlap_kernels.hip", "prolog_fused.hip",
                "rotary_kernels.hip", "latent_cache_kernels.hip", "prompt_attention.hip",
-               "paged_layout.hip", "latent_attention.hip", "capi.cpp", "capi_prompt.cpp", "capi_serving.cpp"]
+               "paged_layout.hip", "latent_attention.hip", "latent_wide.hip", "capi.cpp", "capi_prompt.cpp", "capi_serving.cpp"]
 HIPCC_FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
     # fuse a*b+c only where the source writes it in one expression; files that need exact

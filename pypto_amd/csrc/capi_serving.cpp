@@ -49,31 +49,39 @@ int latent_check(const PtoLatentAttentionArgs *a)
 }
 
 struct LatentPlan {
-    int most_tiles, groups, by_tile, entries;
+    int wide, most_tiles, groups, by_tile, entries;
     size_t o_bytes, ml_bytes, join_bytes;
 };
 
 // The device divides the work, since lengths are there.  Here only as many workgroups as there can be pieces of LA_LEAST units, one to a
 // compute unit at most (a workgroup's LDS is most of one's), and memory for two pieces of each.
+// 128 rows to a workgroup take 0.6 of the time that 64 take for as many, but twice the bytes for a piece: for sequences that fill them, and where the keys that
+// the table has room for could keep each compute unit for 40 tiles of 64 rows (24 sequences of 25 to 63 tokens, 128 heads, 500 to 9000 keys: 1390 us, with
+// 64 rows 1660; single tokens of 32 sequences over 2052 keys, 128 heads: 57, with 64 rows 52).
 LatentPlan latent_plan(const PtoLatentAttentionArgs *a)
 {
     LatentPlan pl{};
     const long long cus = cu_count() > 0 ? cu_count() : 256;
-    const long long row_tiles = a->total_q * a->heads / pto::LA_ROWS + (a->b < a->total_q ? a->b : a->total_q);    // at most
-    long long tiles = (a->max_blocknum_perbatch * a->block_size + pto::LA_KEYS - 1) / pto::LA_KEYS;
-    if (a->window > 0) {                                   // of a row tile's tokens, the window of the first to the last one's last key, and the first keys
-        const long long reach = a->window + (pto::LA_ROWS - 2) / a->heads + 1;
+    auto row_tiles_of = [&](const int rows) { return a->total_q * a->heads / rows + (a->b < a->total_q ? a->b : a->total_q); };         // at most
+    auto tiles_of = [&](const int rows) {
+        const long long all = (a->max_blocknum_perbatch * a->block_size + pto::LA_KEYS - 1) / pto::LA_KEYS;
+        if (a->window == 0) return all;
+        // of a row tile's tokens, the window of the first to the last one's last key, and the first keys
+        const long long reach = a->window + (rows - 2) / a->heads + 1;
         const long long w = (a->sinks + pto::LA_KEYS - 1) / pto::LA_KEYS + (reach + pto::LA_KEYS - 1) / pto::LA_KEYS + 1;
-        tiles = w < tiles ? w : tiles;
-    }
+        return w < all ? w : all;
+    };
+    pl.wide = a->total_q * a->heads >= 96 * a->b && (double)row_tiles_of(pto::LA_ROWS) * (double)tiles_of(pto::LA_ROWS) >= 40.0 * (double)cus;
+    const int rows = pl.wide ? pto::LA_WIDE_ROWS : pto::LA_ROWS;
+    const long long row_tiles = row_tiles_of(rows), tiles = tiles_of(rows);
     pl.most_tiles = (int)tiles;
     const double pieces = (double)row_tiles * (double)(tiles + pto::LA_OPEN) / pto::LA_LEAST;
     const long long groups = pieces < (double)cus ? (long long)pieces + 1 : cus;
     pl.groups = (int)((groups + 7) / 8 * 8);
     pl.by_tile = row_tiles <= pl.groups;
     pl.entries = (int)(pl.by_tile ? (row_tiles > 0 ? row_tiles : 1) : pl.groups);
-    pl.o_bytes = (size_t)2 * pl.groups * pto::LA_ROWS * 512 * sizeof(float);
-    pl.ml_bytes = (size_t)2 * pl.groups * pto::LA_ROWS * 2 * sizeof(float);
+    pl.o_bytes = (size_t)2 * pl.groups * rows * 512 * sizeof(float);
+    pl.ml_bytes = (size_t)2 * pl.groups * rows * 2 * sizeof(float);
     pl.join_bytes = (size_t)pl.entries * 4 * sizeof(int32_t);
     return pl;
 }
@@ -213,7 +221,9 @@ int pto_latent_attention_launch(const PtoLatentAttentionArgs *a, void *hip_strea
     p.sinks = (int)a->sinks;
     p.most_keys = (int)(a->max_blocknum_perbatch * a->block_size);
     p.most_tiles = pl.most_tiles;
-    p.per_entry = (int)((a->b + pto::LA_THREADS - 1) / pto::LA_THREADS);
+    const int threads = pl.wide ? pto::LA_WIDE_THREADS : pto::LA_THREADS;
+    p.wide = pl.wide;
+    p.per_entry = (int)((a->b + threads - 1) / threads);
     p.seq_entries = (int)((a->b + p.per_entry - 1) / p.per_entry);
     p.groups = pl.groups;
     p.by_tile = pl.by_tile;

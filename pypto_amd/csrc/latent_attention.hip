@@ -15,18 +15,11 @@
 // which the workgroups divide evenly, an XCD's neighbouring pieces to neighbouring workgroups.  A boundary near a row tile's edge moves there.
 // Where one falls inside, both sides write their sums, maxima and 512 sums of products, in fp32, and a second launch joins them: two pieces at most
 // to a workgroup, so the memory for them does not depend on lengths, which the host does not know.
-#include <type_traits>
-
-#include "common.h"
-#include "serving_ops.h"
+#include "latent_line.h"
 
 namespace pto {
 namespace {
 
-constexpr int DN = 512, DR = 64;
-constexpr int KT = LA_KEYS;
-constexpr int PITCH = (DN + DR + 8) * 2;                  // bytes of a tile row: 512 latent and 64 rope channels as bf16, 16 spare
-constexpr int TILE = KT * PITCH;
 constexpr int P_AT = 3 * TILE;                            // two buffers of P^T: [row half][k-step][lane] 16 bytes
 constexpr int P_BYTES = 4096;
 constexpr int MAX_AT = P_AT + 2 * P_BYTES;                // [key half][64 rows] fp32: maxima (and at the end the sums)
@@ -34,23 +27,9 @@ constexpr int ALPHA_AT = MAX_AT + 2 * 64 * 4;             // [64 rows] fp32: res
 constexpr int FLAG_AT = ALPHA_AT + 64 * 4;                // two words: the last tile whose maxima moved, by parity of the tile
 constexpr int POOL = FLAG_AT + 16;
 constexpr int Q_ROPE_AT = LA_ROWS * DN * 2;               // query staging: 64 rows x 1024 bytes, then 64 x 128
-constexpr float TAU = 8.0f;                               // log2 units: the reference maximum moves only when exceeded by 2^8
-constexpr float LOW = -1.7e38f;                           // reference maximum of a row that has seen no key yet
 constexpr int PIECE = LA_ROWS * DN;                       // floats of a piece's sums
+constexpr int THREADS = LA_THREADS;
 
-__device__ const u32x4 no_page[4 * (DN + 2 * DR + 16) / 16] = {};      // what four keys without a page read, a whole row of the cache each
-
-// Row i of a tile's score operand (and of the score accumulator) is key tile_row_of(i) of the tile: the two middle bits of i move below its two
-// lowest.  A transposing V^T read then addresses keys r, r+4, r+8, r+12 with each of its half-waves, four rows whose 64-byte pieces lie
-// 16 banks apart at this pitch; any 16 consecutive keys, in whatever order, still serve the score operand reads without a conflict.
-__device__ __forceinline__ constexpr int tile_row_of(const int i) { return (i & 16) | ((i & 3) << 2) | ((i >> 2) & 3); }
-
-__device__ __forceinline__ void both_halves(const float x, float &lo, float &hi)
-{
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    lo = __uint_as_float(r[0]);
-    hi = __uint_as_float(r[1]);
-}
 // max and sum over the four lanes l, l ^ 16, l ^ 32, l ^ 48, in every one of them
 __device__ __forceinline__ float quarters_max(const float x)
 {
@@ -67,101 +46,6 @@ __device__ __forceinline__ float quarters_sum(const float x)
     return lo + hi;
 }
 
-// one dword of int8 times the scale: two dwords of bf16, each product rounded to fp32 and then to bf16
-__device__ __forceinline__ u32x2 dequant_dword(const uint32_t r, const float sc)
-{
-    float f0, f1, f2, f3;
-    asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_0" : "=v"(f0) : "v"(r));
-    asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_1" : "=v"(f1) : "v"(r));
-    asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_2" : "=v"(f2) : "v"(r));
-    asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_3" : "=v"(f3) : "v"(r));
-    return u32x2{pack_bf16x2(f0 * sc, f1 * sc), pack_bf16x2(f2 * sc, f3 * sc)};
-}
-
-// (what hangs on the lane alone is made anew for each row tile instead of being kept)
-__device__ __forceinline__ uint32_t opaque(uint32_t x)
-{
-    asm("" : "+v"(x));
-    return x;
-}
-template <typename T>
-__device__ __forceinline__ T global(const uint8_t *base, const uint32_t offset)
-{
-    return *(const __attribute__((address_space(1))) T *)((const __attribute__((address_space(1))) uint8_t *)base + offset);
-}
-// a scalar load, of what no launch that this one may run beside writes
-template <typename T>
-__device__ __forceinline__ T constant(const T *at)
-{
-    return *(const __attribute__((address_space(4))) T *)at;
-}
-// sums of x over this lane and all lanes before it
-__device__ __forceinline__ long long wave_sums(long long x)
-{
-    auto add = [&](auto ctrl, auto rows) __attribute__((always_inline)) {
-        const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)x, decltype(ctrl)::value, decltype(rows)::value, 0xf, false);
-        const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)((uint64_t)x >> 32), decltype(ctrl)::value, decltype(rows)::value, 0xf, false);
-        x += (long long)((uint64_t)lo | ((uint64_t)hi << 32));
-    };
-    const std::integral_constant<int, 0xf> all;
-    add(std::integral_constant<int, 0x111>{}, all);        // row_shr:1, 2, 4, 8: within rows of sixteen lanes
-    add(std::integral_constant<int, 0x112>{}, all);
-    add(std::integral_constant<int, 0x114>{}, all);
-    add(std::integral_constant<int, 0x118>{}, all);
-    add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});     // row_bcast:15: rows 0 and 2 into 1 and 3
-    add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});     // row_bcast:31: the lower half into the upper
-    return x;
-}
-__device__ __forceinline__ long long first_of(const long long x)
-{
-    return (long long)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)x) | ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32));
-}
-
-// A sequence as the kernel takes it: whatever the tables say, inside the tensors.
-struct Sequence {
-    int q0, n, keys;                                       // first token, tokens, keys
-    int tiles, row_tiles;                                  // units of a row tile but LA_OPEN; row tiles
-};
-__device__ __forceinline__ void count_tiles(const LaParams &p, Sequence &c)
-{
-    c.row_tiles = (c.n * p.heads + LA_ROWS - 1) / LA_ROWS;
-    c.tiles = (c.keys + KT - 1) / KT;
-    c.tiles = c.tiles < p.most_tiles ? c.tiles : p.most_tiles;
-}
-__device__ __forceinline__ Sequence sequence(const LaParams &p, const int b)
-{
-    Sequence c;
-    const int total = (int)p.total_q;
-    int lo = p.cu_q[b], hi = p.cu_q[b + 1], keys = p.lens[b];
-    lo = lo < 0 ? 0 : (lo > total ? total : lo);
-    hi = hi < lo ? lo : (hi > total ? total : hi);
-    keys = keys < 0 ? 0 : (keys > p.most_keys ? p.most_keys : keys);
-    c.q0 = lo, c.n = hi - lo, c.keys = keys;
-    count_tiles(p, c);
-    return c;
-}
-
-// x / d for 0 <= x < 2^51, d >= 1 and a quotient below 2^31: of the product with 1 / d the whole part is off by one at most
-__device__ __forceinline__ int quotient(const long long x, const int d)
-{
-    int q = (int)((double)x * (1.0 / (double)d));
-    if ((long long)q * d > x) --q;
-    if ((long long)(q + 1) * d <= x) ++q;
-    return q;
-}
-
-// The row tile that a unit is in.
-struct Place {
-    int b, q0, n, keys, tiles, row_tile, ordinal;          // ordinal: among the row tiles of all sequences
-    long long begin;                                       // its first unit
-};
-
-// A boundary `x` units into a row tile of `len`, moved to its edge where that is near.
-constexpr int NEAR_BEGIN = LA_OPEN + 3, NEAR_END = 3;
-__device__ __forceinline__ int moved(const int x, const int len) { return x <= NEAR_BEGIN ? 0 : (x >= len - NEAR_END ? len : x); }
-
-constexpr int THREADS = LA_THREADS;
-
 // QUADS: pages and the cache hold whole fours of rows.
 template <bool QUADS>
 __global__ __launch_bounds__(THREADS) void latent_attention_kernel(const LaParams p)
@@ -174,148 +58,23 @@ __global__ __launch_bounds__(THREADS) void latent_attention_kernel(const LaParam
     const int kh = w >> 2;                                 // the half kh of the tile's keys
     const uint32_t pool_lds = (uint32_t)(uintptr_t)(lds_byte_t *)pool;
 
-    // Units and row tiles of the sequences up to each: an entry to a thread, of as many sequences as that takes.
-    __shared__ long long upto[THREADS], of_waves[THREADS / 64];
-    __shared__ int tiles_upto[THREADS], tiles_of_waves[THREADS / 64];
-    __shared__ int seq_q0[THREADS], seq_n[THREADS], seq_keys[THREADS];         // of an entry's first sequence
-    const int per_entry = p.per_entry, entries = p.seq_entries;
-    {
-        long long mine = 0;
-        int row_tiles = 0;
-        for (int j = 0; j < per_entry; ++j) {
-            const int b = tid * per_entry + j;
-            if (b < p.B) {
-                const Sequence c = sequence(p, b);
-                if (j == 0) seq_q0[tid] = c.q0, seq_n[tid] = c.n, seq_keys[tid] = c.keys;
-                mine += (long long)c.row_tiles * (c.tiles + LA_OPEN), row_tiles += c.row_tiles;
-            }
-        }
-        mine = wave_sums(mine);
-        const long long both = wave_sums((long long)row_tiles);
-        if ((tid & 63) == 63) of_waves[w] = mine, tiles_of_waves[w] = (int)both;
-        __syncthreads();
-        int before = 0;
-        for (int i = 0; i < w; ++i) mine += of_waves[i], before += tiles_of_waves[i];
-        upto[tid] = mine;
-        tiles_upto[tid] = (int)both + before;
-        __syncthreads();
-    }
-    const long long units = first_of(upto[THREADS - 1]);
-    const int row_tiles = __builtin_amdgcn_readfirstlane(tiles_upto[THREADS - 1]);
-    auto place_of = [&](const long long u) __attribute__((always_inline)) {
-        int e = 0;                                         // entries that end in front of u
-        for (int i = 0; i < entries; i += 64) e += __popcll(__ballot(upto[i + (tid & 63)] <= u));
-        long long first = e > 0 ? first_of(upto[e - 1]) : 0;
-        int tiles_before = e > 0 ? __builtin_amdgcn_readfirstlane(tiles_upto[e - 1]) : 0;
-        Place at;
-        at.b = e * per_entry;
-        Sequence c;
-        c.q0 = __builtin_amdgcn_readfirstlane(seq_q0[e]), c.n = __builtin_amdgcn_readfirstlane(seq_n[e]), c.keys = __builtin_amdgcn_readfirstlane(seq_keys[e]);
-        count_tiles(p, c);
-        for (int j = 1; j < per_entry; ++j) {              // (only of more than THREADS sequences)
-            const long long next = first + (long long)c.row_tiles * (c.tiles + LA_OPEN);
-            if (next > u || at.b + 1 >= p.B) break;
-            first = next, tiles_before += c.row_tiles, ++at.b;
-            c = sequence(p, at.b);
-        }
-        at.q0 = c.q0, at.n = c.n, at.keys = c.keys, at.tiles = c.tiles;
-        at.row_tile = __builtin_amdgcn_readfirstlane(quotient(u - first, c.tiles + LA_OPEN));
-        at.ordinal = tiles_before + at.row_tile;
-        at.begin = first + (long long)at.row_tile * (c.tiles + LA_OPEN);
-        return at;
-    };
-    // workgroups that take part, so that none gets less than LA_LEAST units; this one's number among them
-    const long long most = (long long)p.groups * LA_LEAST;
-    const int pieces = units < most ? (int)units / LA_LEAST : p.groups, groups = pieces > 0 ? pieces : 1;
-    const int per_xcd = (groups + 7) / 8, slot = blockIdx.x >> 3;
-    const int g = (int)(blockIdx.x & 7) * per_xcd + slot;
-    const bool there = slot < per_xcd && g < groups;
-    // Which row tiles are joined, and from how many pieces: said by the workgroup that has the first of them, for every other entry that there are none.
-    if (tid == 0) {
-        if (p.by_tile) {
-            for (int i = row_tiles + (int)blockIdx.x; i < p.entries; i += (int)gridDim.x) p.joins[4 * i + 1] = 0;
-        } else if (!there) {
-            p.joins[4 * blockIdx.x + 1] = 0;
-        }
-    }
-    if (!there) return;
-    // the line's even divisions: units * i / groups
-    long long share = (long long)((double)units / (double)groups);
-    if (share * groups > units) --share;
-    const int rest = (int)(units - share * groups);
-    auto division = [&](const int i) { return share * i + (rest * i) / groups; };
-    long long u = 0, u_end = units, want = division(g + 1 < groups ? g + 1 : g);
-    int step = g + 1 < groups ? 0 : 1;                     // looked for: this workgroup's end, its beginning, the next row tile
-    bool said = false;                                     // (not by_tile) this workgroup's entry is written
-    bool first_segment = true;
-
-    while (units > 0) {
+    __shared__ LineTable<THREADS> table;
+    const Line<LA_ROWS, THREADS> line(p, table);
+    if (!line.begin()) return;
+    Place at;
+    int i_begin, i_end;
+    while (line.next(at, i_begin, i_end)) {
         const int l = (int)opaque(tid & 63), half = l >> 5, col = l & 31, l16 = l & 15, quarter = l >> 4;
-        const Place at = place_of(want);
-        if (step < 2) {
-            const long long edge = at.begin + moved((int)(want - at.begin), at.tiles + LA_OPEN);
-            if (step == 0) {
-                u_end = edge, want = division(g), step = 1;
-                continue;
-            }
-            u = edge, step = 2;
-            if (u >= u_end) break;
-            if (u == at.begin + at.tiles + LA_OPEN) {
-                want = u;
-                continue;
-            }
-        }
-        const int len = at.tiles + LA_OPEN;
-        const long long end = at.begin + len;
-        const long long to = u_end < end ? u_end : end;
-        const bool whole = u == at.begin && to == end;
-        int i_begin = (int)(u - at.begin) - LA_OPEN;
-        i_begin = i_begin < 0 ? 0 : i_begin;
-        int i_end = (int)(to - at.begin) - LA_OPEN;
-
-        // the piece's place, and what is to be joined
-        const int piece = 2 * g + (first_segment ? 0 : 1);
-        const int rows = at.n * p.heads, row0 = at.row_tile * LA_ROWS;
-        if (tid == 0 && u == at.begin && (p.by_tile || !whole)) {
-            int n = 0;
-            if (!whole) {                                  // pieces: one more than there are boundaries inside, those before unit end - NEAR_END
-                const long long edge = end - NEAR_END;
-                n = (int)((double)edge * (double)groups / (double)units) - g;
-                n = n > 1 ? n - 1 : 1;
-                while (g + n < groups && division(g + n) < edge) ++n;
-            }
-            int32_t *const join = p.joins + 4 * (p.by_tile ? at.ordinal : (int)blockIdx.x);
-            join[0] = piece, join[1] = n, join[2] = at.q0 * p.heads + row0, join[3] = rows - row0 < LA_ROWS ? rows - row0 : LA_ROWS;
-            said = true;
-        }
-
-        // What the row tile's tokens see, and which of the units are which tiles of keys.
-        const int last = rows - 1 - row0 < LA_ROWS - 1 ? rows - 1 - row0 : LA_ROWS - 1;       // its last row
-        const int tok0 = divide(row0, p.of_heads), tok1 = divide(row0 + last, p.of_heads);
-        const bool tree = p.mask != nullptr;
-        const int context = at.keys - at.n > 0 ? at.keys - at.n : 0;                           // keys before the tree
-        auto sees_of = [&](const int tok) {
-            const int s = tok + 1 + at.keys - at.n;
-            return tree ? at.keys : (s < 0 ? 0 : s);
-        };
-        auto from_of = [&](const int sees) { return p.window > 0 && sees > p.window ? sees - p.window : 0; };
-        const int least = tree ? context : sees_of(tok0), most = sees_of(tok1);                // keys that all, that some rows see (but for windows)
-        const int low_first = from_of(sees_of(tok0)), low_last = from_of(sees_of(tok1));       // where windows begin
-        const int key_tiles = (most + KT - 1) / KT;
-        int sink_tiles = (p.sinks + KT - 1) / KT;
-        sink_tiles = sink_tiles < low_first / KT ? sink_tiles : low_first / KT;
-        const int skip = low_first / KT - sink_tiles;
-        i_end = i_end < key_tiles - skip ? i_end : key_tiles - skip;
+        const Sight<LA_ROWS> sight(p, at);
+        const int last = sight.last;                       // of the row tile's rows
+        i_end = i_end < sight.tiles ? i_end : sight.tiles;
         const int ntiles = i_end > i_begin ? i_end - i_begin : 0;
-        auto key_of_tile = [&](const int n) {              // the first key of tile n of this piece
-            const int i = i_begin + (n < ntiles ? n : ntiles - 1);
-            return KT * (i < sink_tiles ? i : i + skip);
-        };
+        auto key_of_tile = [&](const int n) { return sight.first_key(i_begin + (n < ntiles ? n : ntiles - 1)); };      // the first key of tile n of this piece
         // of this lane's row of scores
-        const int my_row = row0 + 16 * hq + l16;
-        const int my_tok = divide(my_row < rows ? my_row : rows - 1, p.of_heads);
-        const int my_sees = sees_of(my_tok), my_from = from_of(my_sees);
-        const unsigned long long *const my_mask = tree ? p.mask + (long long)(at.q0 + my_tok) * p.words : nullptr;
+        const int my_row = sight.row0 + 16 * hq + l16;
+        const int my_tok = divide(my_row < sight.rows ? my_row : sight.rows - 1, p.of_heads);
+        const int my_sees = sight.sees(my_tok);
+        const unsigned long long *const my_mask = p.mask ? p.mask + (long long)(at.q0 + my_tok) * p.words : nullptr;
 
         f32x16 o[4];                                       // block 2*hb + d: rows 32*hb .., value channels 64w + 32d ..
 #pragma unroll
@@ -332,62 +91,35 @@ __global__ __launch_bounds__(THREADS) void latent_attention_kernel(const LaParam
             static_assert(Q_ROPE_AT + LA_ROWS * DR * 2 <= 2 * TILE, "the first tile goes to buffer 2");
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int j = 8 * w + i, r = row0 + (j < last ? j : last);
+                const int j = 8 * w + i, r = sight.row0 + (j < last ? j : last);
                 const int tok = divide(r, p.of_heads), head = r - tok * p.heads;
                 dma16_base(p.q + (long long)(at.q0 + tok) * p.q_t + (long long)head * p.q_h, (uint32_t)(16 * (l ^ (j & 15))), pool_lds + j * (DN * 2));
             }
             {
-                const int j = 8 * w + (l >> 3), r = row0 + (j < last ? j : last);
+                const int j = 8 * w + (l >> 3), r = sight.row0 + (j < last ? j : last);
                 const int tok = divide(r, p.of_heads), head = r - tok * p.heads;
                 dma16(p.qr + (long long)(at.q0 + tok) * p.qr_t + (long long)head * p.qr_h + 8 * ((l & 7) ^ (l >> 3)), pool_lds + Q_ROPE_AT + w * 1024);
             }
 
             // Gather: wave w takes keys 4w .. 4w+3 of every tile, a quarter of its lanes each, a lane 32 channels of the latents (one scale) and
-            // four of the rope part.  QUADS: the four are neighbours in the cache, so one scalar look-up and one address serve them.  Keys past
-            // the sequence's last one are those of the same four that are left in its page (their scores are hidden, and check_scales
-            // keeps what they hold out of the sums), else stand in with the last one.
+            // four of the rope part.
             struct Raw {
                 u32x4 v[2];
                 float sc;
                 u32x2 rope;
             };
             Raw raw[2];                                    // tile n in raw[n & 1]
-            struct Page {
-                int page, within;
-            };
-            auto page_of = [&](const int n) __attribute__((always_inline)) {
-                int key = key_of_tile(n) + 4 * w + (QUADS ? 0 : quarter);
-                const int last_key = QUADS ? (at.keys - 1) & ~3 : at.keys - 1;
-                key = key < last_key ? key : last_key;
-                const int block = divide(key, p.of_bs);    // (the block table has it: at.keys is no more than its pages hold)
-                const int32_t *const entry = p.bt + (long long)at.b * p.maxblk + block;
-                return Page{QUADS ? constant<int32_t>(entry) : *entry, key - block * p.bs};
-            };
+            constexpr int NEAR = QUADS ? 4 : 1;
+            auto page_of_tile = [&](const int n) __attribute__((always_inline)) { return page_of<NEAR>(p, at, key_of_tile(n) + 4 * w + (QUADS ? 0 : quarter)); };
             const uint32_t rows_on = QUADS ? quarter : 0;
             const uint32_t v_off = rows_on * (uint32_t)p.cache.nope_pitch + 32 * l16, sc_off = rows_on * (uint32_t)p.cache.scale_pitch + 4 * (l16 >> 2),
                            rope_off = rows_on * (uint32_t)p.cache.rope_pitch + 8 * l16;
             auto gather = [&](Raw &r, const Page k) __attribute__((always_inline)) {
-                const long long row = (long long)k.page * p.bs + k.within;
-                const bool there = k.page >= 0 && row < p.cache.rows;
-                const uint8_t *const none = reinterpret_cast<const uint8_t *>(no_page);
-                const uint8_t *const v = there ? p.cache.nope + row * p.cache.nope_pitch : none;
-                const uint8_t *const sc = there ? p.cache.scale + row * p.cache.scale_pitch : none;
-                const uint8_t *const rope = there ? p.cache.rope + row * p.cache.rope_pitch : none;
-                r.v[0] = global<u32x4>(v, v_off);
-                r.v[1] = global<u32x4>(v + 16, v_off);
-                r.sc = global<float>(sc, sc_off);
-                r.rope = global<u32x2>(rope, rope_off);
-            };
-            // A scale that is no number, or with which 127 steps are not finite, would be in the sums of rows that do not see the key (0 times it):
-            // such a group's values become zeros and the key's rope channels, which are in scores alone, no numbers.  A row that sees the
-            // key is then no number, others are not touched.
-            auto check_scales = [&](Raw &r) __attribute__((always_inline)) {
-                const bool bad = !(fabsf(r.sc) < 2.6e36f);
-                const uint64_t any = __ballot(bad);
-                if (__builtin_expect(any != 0, 0)) {
-                    r.sc = bad ? 0.f : r.sc;
-                    if (((any >> (16 * quarter)) & 0xffff) != 0) r.rope = u32x2{0x7fc07fc0u, 0x7fc07fc0u};
-                }
+                const RowAt row = row_at(p, k);
+                r.v[0] = global<u32x4>(row.nope, v_off);
+                r.v[1] = global<u32x4>(row.nope + 16, v_off);
+                r.sc = global<float>(row.scale, sc_off);
+                r.rope = global<u32x2>(row.rope, rope_off);
             };
             // The tile's rows into LDS, in eight pieces of a dword per lane and one of the rope channels.  Of a row's 64 latent pieces of eight
             // channels number 4 j + k lies at k * 16 + j: a lane's four pieces are one of each k, and lanes next to each other write next to
@@ -396,7 +128,7 @@ __global__ __launch_bounds__(THREADS) void latent_attention_kernel(const LaParam
             const uint32_t emit_rope_off = (uint32_t)((4 * w + quarter) * PITCH + DN * 2 + 8 * l16);
             u32x4 dq;
             auto emit = [&](Raw &r, const uint32_t tile, const int d) __attribute__((always_inline)) {
-                if (d == 0) check_scales(r);
+                if (d == 0) check_scale<16>(r.sc, r.rope);
                 if (d == 8) {
                     *reinterpret_cast<u32x2 *>(pool + tile + emit_rope_off) = r.rope;
                 } else {
@@ -409,7 +141,7 @@ __global__ __launch_bounds__(THREADS) void latent_attention_kernel(const LaParam
                     }
                 }
             };
-            Page page = page_of(0), page1 = page_of(1), page2 = page_of(2), page3 = page_of(3);
+            Page page = page_of_tile(0), page1 = page_of_tile(1), page2 = page_of_tile(2), page3 = page_of_tile(3);
             gather(raw[0], page);
             gather(raw[1], page1);
             // the waves' own queries have landed; those of the others when every wave has come here
@@ -438,7 +170,7 @@ __global__ __launch_bounds__(THREADS) void latent_attention_kernel(const LaParam
 #pragma unroll
             for (int d = 0; d < 9; ++d) emit(raw[0], 2 * TILE, d);
             gather(raw[0], page2);
-            page2 = page_of(4);
+            page2 = page_of_tile(4);
             __syncthreads();
 
             // Score operand: row `a` of the wave's sixteen is key tile_row_of(16*kh + a); the accumulator then holds in lane
@@ -504,21 +236,10 @@ __global__ __launch_bounds__(THREADS) void latent_attention_kernel(const LaParam
 #pragma unroll
                 for (int e = 0; e < 4; ++e) sv[e] = s[e];
                 const int first = key_of_tile(n);
-                const bool below = first + KT <= least;                                        // (uniform)
-                if (!(below && (first >= low_last || first + KT <= p.sinks))) {
-                    uint32_t drafted = ~0u;                // of the tile's keys, those in front of the tree and those of it that the row sees
-                    if (tree && !below) {
-                        const int node = first - context, at_word = node >> 6, shift = node & 63;
-                        auto word = [&](const int i) { return i < 0 ? ~0ull : (i < p.words ? my_mask[i] : 0ull); };
-                        const unsigned long long lo = word(at_word), hi = word(at_word + 1);
-                        drafted = (uint32_t)((lo >> shift) | (shift ? hi << (64 - shift) : 0ull));
-                    }
+                if (!sight.whole(first)) {                 // (uniform)
+                    const uint32_t seen = sight.seen(first, my_sees, my_mask);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int key = first + key_of[e];
-                        const bool seen = (key < my_sees) & ((key >= my_from) | (key < p.sinks)) & (((drafted >> key_of[e]) & 1) != 0);
-                        sv[e] = seen ? sv[e] : -INFINITY;          // (without a branch for each score)
-                    }
+                    for (int e = 0; e < 4; ++e) sv[e] = (seen >> key_of[e]) & 1 ? sv[e] : -INFINITY;
                 }
                 mx = fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3]));
             };
@@ -568,7 +289,7 @@ __global__ __launch_bounds__(THREADS) void latent_attention_kernel(const LaParam
                     if (mp == 1) load_v(prev, 1, 1), load_p(pbuf, 1, 1);
                     if (NEXT) {                            // (pages before rows: loads come back in order)
                         emit(r, next, mp);
-                        if (mp == 4) further = page_of(n4);
+                        if (mp == 4) further = page_of_tile(n4);
                         if (mp == 7) emit(r, next, 8), gather(r, page), page = further;
                     }
                     __builtin_amdgcn_sched_barrier(0);
@@ -637,6 +358,9 @@ __global__ __launch_bounds__(THREADS) void latent_attention_kernel(const LaParam
         l_run = quarters_sum(l_run);
         float *const sums = reinterpret_cast<float *>(pool + MAX_AT), *const il = reinterpret_cast<float *>(pool + ALPHA_AT);
         __syncthreads();
+        // (what is known of the row tile comes back from LDS: see LineTable)
+        const bool whole = line.one(table.whole) != 0;
+        const int piece = line.one(table.piece), rows = line.one(table.rows), row0 = line.one(table.row0), first = line.one(table.first);
         if (l < 16) sums[64 * kh + 16 * hq + l16] = l_run;
         __syncthreads();
         if (kh == 0 && l < 16) {
@@ -647,7 +371,7 @@ __global__ __launch_bounds__(THREADS) void latent_attention_kernel(const LaParam
                 const f32x2 ml = {m_run, sum};
                 *reinterpret_cast<f32x2 *>(p.part_ml + ((long long)piece * LA_ROWS + r) * 2) = ml;
             } else if (p.lse && row0 + r < rows) {
-                p.lse[(long long)at.q0 * p.heads + row0 + r] = sum == 0.f ? -INFINITY : (m_run + __builtin_amdgcn_logf(sum)) * 0.693147180559945f;
+                p.lse[(long long)first * p.heads + row0 + r] = sum == 0.f ? -INFINITY : (m_run + __builtin_amdgcn_logf(sum)) * 0.693147180559945f;
             }
         }
         if (!whole) {
@@ -681,41 +405,40 @@ __global__ __launch_bounds__(THREADS) void latent_attention_kernel(const LaParam
                 const int r = row0 + 8 * w + e;
                 if (r < rows) {
                     const int tok = divide(r, p.of_heads), head = r - tok * p.heads;
-                    *reinterpret_cast<u32x4_a2 *>(p.out + (long long)(at.q0 + tok) * p.o_t + (long long)head * p.o_h + 8 * l) = v[e];
+                    *reinterpret_cast<u32x4_a2 *>(p.out + (long long)(first + tok) * p.o_t + (long long)head * p.o_h + 8 * l) = v[e];
                 }
             }
         }
         __syncthreads();                                   // (the next row tile's queries go over these)
-        u = want = to;
-        first_segment = false;
-        if (u >= u_end) break;
     }
-    if (!p.by_tile && tid == 0 && !said) p.joins[4 * blockIdx.x + 1] = 0;
+    line.done();
 }
 
 // The pieces of row tiles that workgroups share: out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i, in the order of the keys.  A workgroup
-// joins block i of wave w's channels (as the attention kernel's registers have them) of an entry's rows, four 16-byte values to a lane, its four
-// waves a quarter of the pieces each.
+// joins one accumulator block (32 rows, 32 channels, as the attention kernels' registers have them) of an entry's rows, four 16-byte values to a
+// lane, its four waves a quarter of the pieces each.
+template <bool WIDE>
 __global__ __launch_bounds__(256) void latent_join_kernel(const LaParams p)
 {
+    constexpr int TILE_ROWS = WIDE ? LA_WIDE_ROWS : LA_ROWS, BLOCKS = TILE_ROWS / 2, OF_WAVE = WIDE ? 16 : 4;
     __shared__ f32x4 sums[3][4][64];
     __shared__ float stats[3][2][32];
     const int l = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = l >> 5, col = l & 31;
-    const int32_t *const join = p.joins + 4 * (blockIdx.x >> 5);
+    const int32_t *const join = p.joins + 4 * (blockIdx.x / BLOCKS);
     const int n = join[1];
     if (n <= 1) return;
     const int first = join[0], row0 = join[2], rows = join[3];
-    const int w = (blockIdx.x & 31) >> 2, i = blockIdx.x & 3, hb = i >> 1, d = i & 1;
+    const int w = (blockIdx.x % BLOCKS) / OF_WAVE, i = blockIdx.x % OF_WAVE;
+    const int group = WIDE ? i >> 2 : i >> 1, c = WIDE ? i & 3 : i & 1;            // of 32 rows; of 32 of the wave's channels
     // where the pieces are: that of the first workgroup is said; the others' ranges begin inside the row tile, so it is their first
-    const int g = first >> 1;
-    auto place = [&](const int k) { return (long long)(k == 0 ? first : 2 * (g + k)); };
+    auto place = [&](const int k) { return (long long)(k == 0 ? first : 2 * ((first >> 1) + k)); };
     float top = LOW, total = 0.f;
     f32x4 acc[4];
 #pragma unroll
     for (int q4 = 0; q4 < 4; ++q4) acc[q4] = f32x4{0.f, 0.f, 0.f, 0.f};
     for (int k = wave; k < n; k += 4) {
-        const f32x2 ml = *reinterpret_cast<const f32x2 *>(p.part_ml + (place(k) * LA_ROWS + 32 * hb + col) * 2);
-        const float *src = p.part_o + place(k) * PIECE + ((w * 16 + 4 * i) * 64 + l) * 4;
+        const f32x2 ml = *reinterpret_cast<const f32x2 *>(p.part_ml + (place(k) * TILE_ROWS + 32 * group + col) * 2);
+        const float *src = p.part_o + place(k) * (TILE_ROWS * DN) + ((w * OF_WAVE + i) * 256 + l) * 4;
         f32x4 x[4];
 #pragma unroll
         for (int q4 = 0; q4 < 4; ++q4) x[q4] = *reinterpret_cast<const f32x4 *>(src + q4 * 256);
@@ -739,16 +462,16 @@ __global__ __launch_bounds__(256) void latent_join_kernel(const LaParams p)
 #pragma unroll
         for (int q4 = 0; q4 < 4; ++q4) acc[q4] = acc[q4] * a + sums[k][q4][l] * b;
     }
-    const int row = 32 * hb + col;
+    const int row = 32 * group + col;
     if (row >= rows) return;
     const long long r = (long long)row0 + row;
-    if (p.lse && w == 0 && d == 0 && half == 0) p.lse[r] = total == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(total)) * 0.693147180559945f;
+    if (p.lse && w == 0 && c == 0 && half == 0) p.lse[r] = total == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(total)) * 0.693147180559945f;
     const float inv = total == 0.f ? 0.f : 1.0f / total;
     const int tok = divide((int)r, p.of_heads), head = (int)r - tok * p.heads;
     uint16_t *dst = p.out + (long long)tok * p.o_t + (long long)head * p.o_h;
 #pragma unroll
     for (int q4 = 0; q4 < 4; ++q4) {
-        const int chunk = 32 * (w & 1) + 4 * (4 * d + q4) + (w >> 1);
+        const int chunk = WIDE ? 4 * (4 * c + q4) + w : 32 * (w & 1) + 4 * (4 * c + q4) + (w >> 1);
         *reinterpret_cast<u32x2_a2 *>(dst + 8 * chunk + 4 * half) =
             u32x2{pack_bf16x2(acc[q4][0] * inv, acc[q4][1] * inv), pack_bf16x2(acc[q4][2] * inv, acc[q4][3] * inv)};
     }
@@ -758,11 +481,17 @@ __global__ __launch_bounds__(256) void latent_join_kernel(const LaParams p)
 
 hipError_t latent_attention_launch(const LaParams &p, hipStream_t stream)
 {
+    if (p.wide) {
+        const hipError_t e = latent_attention_wide_launch(p, stream);
+        if (e != hipSuccess) return e;
+        hipLaunchKernelGGL((latent_join_kernel<true>), dim3((unsigned)p.entries * (LA_WIDE_ROWS / 2)), dim3(256), 0, stream, p);
+        return hipGetLastError();
+    }
     if (p.bs % 4 == 0 && p.cache.rows % 4 == 0) hipLaunchKernelGGL((latent_attention_kernel<true>), dim3((unsigned)p.groups), dim3(THREADS), 0, stream, p);
     else hipLaunchKernelGGL((latent_attention_kernel<false>), dim3((unsigned)p.groups), dim3(THREADS), 0, stream, p);
-    hipError_t e = hipGetLastError();
+    const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(latent_join_kernel, dim3((unsigned)p.entries * 32), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((latent_join_kernel<false>), dim3((unsigned)p.entries * (LA_ROWS / 2)), dim3(256), 0, stream, p);
     return hipGetLastError();
 }
 

@@ -55,6 +55,7 @@ constexpr int LA_ROWS = 64;               // (token, head) rows of a workgroup
 constexpr int LA_KEYS = 32;               // keys of a tile
 constexpr int LA_OPEN = 6;                // what a row tile's beginning and end cost, in tiles
 constexpr int LA_THREADS = 512;          // of a workgroup
+constexpr int LA_WIDE_ROWS = 128, LA_WIDE_THREADS = 256;    // the same of the form for many rows
 constexpr int LA_LEAST = 6;               // units of the shortest piece that the line is divided into
 
 struct LaParams {
@@ -67,18 +68,20 @@ struct LaParams {
     const unsigned long long *mask;       // [total_q, words] or null
     uint16_t *out;
     float *lse;                           // [total_q, heads] or null
-    float *part_o, *part_ml;              // [2 * groups] pieces of LA_ROWS rows: 512 sums, (maximum, sum)
+    float *part_o, *part_ml;              // [2 * groups] pieces of a row tile: 512 sums a row, (maximum, sum) a row
     int32_t *joins;                       // [entries][4]: first piece, pieces, first row, rows
     long long total_q;
     int B, maxblk, bs, heads, words;
     int window, sinks;                    // window 0: all keys
     int most_keys, most_tiles;            // of a sequence, as the block table and the window have it
     int per_entry, seq_entries;           // sequences that a workgroup's thread counts; threads that count any
+    int wide;                             // row tiles of LA_WIDE_ROWS
     int groups;                           // workgroups, a multiple of eight
     int by_tile, entries;                 // joins by row tile (of all sequences), else by workgroup; how many there are
     Divisor of_heads, of_bs;
     float scale_log2;
 };
 hipError_t latent_attention_launch(const LaParams &p, hipStream_t stream);
+hipError_t latent_attention_wide_launch(const LaParams &p, hipStream_t stream);      // without the joining launch
 
 }  // namespace pto
