@@ -69,7 +69,7 @@ __global__ __launch_bounds__(THREADS) void latent_attention_kernel(const LaParam
         const int last = sight.last;                       // of the row tile's rows
         i_end = i_end < sight.tiles ? i_end : sight.tiles;
         const int ntiles = i_end > i_begin ? i_end - i_begin : 0;
-        auto key_of_tile = [&](const int n) { return sight.first_key(i_begin + (n < ntiles ? n : ntiles - 1)); };      // the first key of tile n of this piece
+        auto key_of_tile = [&](const int n) { return sight.first_key(i_begin + n); };      // the first key of tile n of this piece
         // of this lane's row of scores
         const int my_row = sight.row0 + 16 * hq + l16;
         const int my_tok = divide(my_row < sight.rows ? my_row : sight.rows - 1, p.of_heads);
@@ -85,6 +85,17 @@ __global__ __launch_bounds__(THREADS) void latent_attention_kernel(const LaParam
         float l_run = 0.f;                                 // and this lane's share of the sum of exp2(s - m_run)
 
         if (ntiles > 0) {                                  // uniform
+            // Gather: wave w takes keys 4w .. 4w+3 of every tile, a quarter of its lanes each, a lane 32 channels of the latents (one scale) and
+            // four of the rope part.
+            struct Raw {
+                u32x4 v[2];
+                float sc;
+                u32x2 rope;
+            };
+            Raw raw[2];                                    // tile n in raw[n & 1]
+            constexpr int NEAR = QUADS ? 4 : 1;
+            auto page_of_tile = [&](const int n) __attribute__((always_inline)) { return page_of<NEAR>(p, at, key_of_tile(n) + 4 * w + (QUADS ? 0 : quarter)); };
+            Page page = page_of_tile(0), page1 = page_of_tile(1), page2 = page_of_tile(2), page3 = page_of_tile(3);
             // The queries, staged through LDS in the tile buffers 0 and 1: wave w asks for rows 8w .. 8w+7, a row's latent part per request,
             // 16-byte chunk i of row j at i ^ (j & 15) so that the fragment reads touch every bank once.  Rows past the last one read it
             // and are never stored.
@@ -101,16 +112,6 @@ __global__ __launch_bounds__(THREADS) void latent_attention_kernel(const LaParam
                 dma16(p.qr + (long long)(at.q0 + tok) * p.qr_t + (long long)head * p.qr_h + 8 * ((l & 7) ^ (l >> 3)), pool_lds + Q_ROPE_AT + w * 1024);
             }
 
-            // Gather: wave w takes keys 4w .. 4w+3 of every tile, a quarter of its lanes each, a lane 32 channels of the latents (one scale) and
-            // four of the rope part.
-            struct Raw {
-                u32x4 v[2];
-                float sc;
-                u32x2 rope;
-            };
-            Raw raw[2];                                    // tile n in raw[n & 1]
-            constexpr int NEAR = QUADS ? 4 : 1;
-            auto page_of_tile = [&](const int n) __attribute__((always_inline)) { return page_of<NEAR>(p, at, key_of_tile(n) + 4 * w + (QUADS ? 0 : quarter)); };
             const uint32_t rows_on = QUADS ? quarter : 0;
             const uint32_t v_off = rows_on * (uint32_t)p.cache.nope_pitch + 32 * l16, sc_off = rows_on * (uint32_t)p.cache.scale_pitch + 4 * (l16 >> 2),
                            rope_off = rows_on * (uint32_t)p.cache.rope_pitch + 8 * l16;
@@ -141,12 +142,16 @@ __global__ __launch_bounds__(THREADS) void latent_attention_kernel(const LaParam
                     }
                 }
             };
-            Page page = page_of_tile(0), page1 = page_of_tile(1), page2 = page_of_tile(2), page3 = page_of_tile(3);
             gather(raw[0], page);
             gather(raw[1], page1);
-            // the waves' own queries have landed; those of the others when every wave has come here
-            __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
-            __syncthreads();
+            __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));      // (the wave's queries, too)
+            asm volatile("" ::: "memory");
+#pragma unroll
+            for (int d = 0; d < 9; ++d) emit(raw[0], 2 * TILE, d);
+            gather(raw[0], page2);
+            page2 = page_of_tile(4);
+            if (tid < 2) reinterpret_cast<int *>(pool + FLAG_AT)[tid] = -1;
+            __syncthreads();                               // the queries and the first tile are there
             // Q^T: of the latent part lane (row, quarter) holds the channels of the tile rows' 16-byte pieces at 16*quarter + ks, of
             // the rope part channels 16*quarter + 8*ks .. +7
             bf16x8 qf[18];
@@ -166,13 +171,6 @@ __global__ __launch_bounds__(THREADS) void latent_attention_kernel(const LaParam
                 for (int i = 0; i < 18; ++i) qf[i] = __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, qf[i]) ^ 0x80008000u);
             }
             if (sc_log2 == 0.f) sc_log2 = 1.17549435e-38f;
-            if (tid < 2) reinterpret_cast<int *>(pool + FLAG_AT)[tid] = -1;
-#pragma unroll
-            for (int d = 0; d < 9; ++d) emit(raw[0], 2 * TILE, d);
-            gather(raw[0], page2);
-            page2 = page_of_tile(4);
-            __syncthreads();
-
             // Score operand: row `a` of the wave's sixteen is key tile_row_of(16*kh + a); the accumulator then holds in lane
             // (row, quarter) the keys 4*quarter + r, the k-order of the second product's B operand.
             // (quarters 256 bytes apart: whichever sixteen lanes the LDS serves together, their rows alone decide the banks)
@@ -330,6 +328,7 @@ __global__ __launch_bounds__(THREADS) void latent_attention_kernel(const LaParam
             // the first tile: its maxima are moved at once
             first_k(cur);
             scores(cur);
+            __syncthreads();                               // every wave has its queries: the next tile goes over them
 #pragma unroll
             for (int d = 0; d < 9; ++d) emit(raw[1], next, d);
             gather(raw[1], page3);
@@ -360,7 +359,7 @@ __global__ __launch_bounds__(THREADS) void latent_attention_kernel(const LaParam
         __syncthreads();
         // (what is known of the row tile comes back from LDS: see LineTable)
         const bool whole = line.one(table.whole) != 0;
-        const int piece = line.one(table.piece), rows = line.one(table.rows), row0 = line.one(table.row0), first = line.one(table.first);
+        const int piece = line.one(table.piece), first = line.one(table.place.q0), rows = line.one(table.place.n) * p.heads, row0 = line.one(table.place.row_tile) * LA_ROWS;
         if (l < 16) sums[64 * kh + 16 * hq + l16] = l_run;
         __syncthreads();
         if (kh == 0 && l < 16) {

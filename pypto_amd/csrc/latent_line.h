@@ -28,16 +28,22 @@ __device__ __forceinline__ void both_halves(const float x, float &lo, float &hi)
     lo = __uint_as_float(r[0]);
     hi = __uint_as_float(r[1]);
 }
-// one dword of int8 times the scale: two dwords of bf16, each product rounded to fp32 and then to bf16
-__device__ __forceinline__ u32x2 dequant_dword(const uint32_t r, const float sc)
+// int8 times the scale as bf16, each product rounded to fp32 and then to bf16: of a dword's lower and upper two
+__device__ __forceinline__ uint32_t dequant_lower(const uint32_t r, const float sc)
 {
-    float f0, f1, f2, f3;
+    float f0, f1;
     asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_0" : "=v"(f0) : "v"(r));
     asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_1" : "=v"(f1) : "v"(r));
-    asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_2" : "=v"(f2) : "v"(r));
-    asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_3" : "=v"(f3) : "v"(r));
-    return u32x2{pack_bf16x2(f0 * sc, f1 * sc), pack_bf16x2(f2 * sc, f3 * sc)};
+    return pack_bf16x2(f0 * sc, f1 * sc);
 }
+__device__ __forceinline__ uint32_t dequant_upper(const uint32_t r, const float sc)
+{
+    float f0, f1;
+    asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_2" : "=v"(f0) : "v"(r));
+    asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_3" : "=v"(f1) : "v"(r));
+    return pack_bf16x2(f0 * sc, f1 * sc);
+}
+__device__ __forceinline__ u32x2 dequant_dword(const uint32_t r, const float sc) { return u32x2{dequant_lower(r, sc), dequant_upper(r, sc)}; }
 
 // (what hangs on the lane alone is made anew for each row tile instead of being kept)
 __device__ __forceinline__ uint32_t opaque(uint32_t x)
@@ -132,8 +138,8 @@ struct LineTable {
     int q0[THREADS], n[THREADS], keys[THREADS];            // of an entry's first sequence
     long long units, share, end, next;                     // end: of this workgroup's part; next: the unit behind the row tile's part in hand
     int groups, g, rest, said;
-    int whole, piece, first, rows, row0;                   // of the row tile in hand: no other workgroup's too; its piece's place; the sequence's first token, its
-                                                           // rows, the row tile's first
+    Place place;                                           // the row tile in hand, or (fresh) the one that begins this workgroup's part
+    int fresh, whole, piece;                               // whole: no other workgroup has a part of it; its piece's place
 };
 
 // The line of all units, and this workgroup's part of it.
@@ -187,21 +193,19 @@ struct Line {
         long long share = (long long)((double)units / (double)groups);
         if (share * groups > units) --share;
         const int rest = (int)(units - share * groups);
-        const long long last = g + 1 < groups ? boundary(share, rest, groups, g + 1) : units, u = g > 0 ? boundary(share, rest, groups, g) : 0;
-        // (written by every thread alike, so that no wave waits for another)
-        t.units = units, t.share = share, t.groups = groups, t.rest = rest, t.g = g, t.first = -1;
-        t.end = last, t.next = u;
+        // (half of the waves look for this workgroup's end, the others for its beginning; each value is written by several threads alike)
+        t.units = units, t.share = share, t.groups = groups, t.rest = rest, t.g = g;
         if (tid == 0) t.said = 0;
+        const int upper = __builtin_amdgcn_readfirstlane(tid >= THREADS / 2);
+        const long long u = division(share, rest, groups, g + upper < groups ? g + upper : g);
+        const Place at = place_of(u);
+        const int len = at.tiles + LA_OPEN, x = moved((int)(u - at.begin), len);
+        if (upper) t.end = g + 1 < groups ? at.begin + x : units;
+        else t.next = at.begin + x, t.place = at, t.fresh = x < len ? 1 : 0;
+        __syncthreads();
         return true;
     }
     __device__ __forceinline__ static long long division(const long long share, const int rest, const int groups, const int i) { return share * i + (rest * i) / groups; }
-    __device__ __forceinline__ long long boundary(const long long share, const int rest, const int groups, const int i) const
-    {
-        const long long u = division(share, rest, groups, i);
-        const Place at = place_of(u);
-        return at.begin + moved((int)(u - at.begin), at.tiles + LA_OPEN);
-    }
-
     // the row tile that unit u of the line is in
     __device__ __forceinline__ Place place_of(const long long u) const
     {
@@ -233,9 +237,13 @@ struct Line {
     __device__ __forceinline__ bool next(Place &at, int &i_begin, int &i_end) const
     {
         const long long u = first_of(t.next), u_end = first_of(t.end);
-        const bool first_part = one(t.first) < 0;
         if (u >= u_end) return false;
-        at = place_of(u);
+        const int fresh = one(t.fresh);                    // 1: the place is that of u, which nothing of was done; 0: that of something else; -1: of the row tile in front
+        const bool first_part = fresh >= 0;
+        at.b = one(t.place.b), at.q0 = one(t.place.q0), at.n = one(t.place.n), at.keys = one(t.place.keys), at.tiles = one(t.place.tiles);
+        at.row_tile = one(t.place.row_tile), at.ordinal = one(t.place.ordinal), at.begin = first_of(t.place.begin);
+        if (fresh < 0 && (at.row_tile + 1) * ROWS < at.n * p.heads) ++at.row_tile, ++at.ordinal, at.begin = u;
+        else if (fresh <= 0) at = place_of(u);
         const int len = at.tiles + LA_OPEN;
         const long long end = at.begin + len, to = u_end < end ? u_end : end;
         const bool whole = u == at.begin && to == end;
@@ -257,7 +265,7 @@ struct Line {
             t.said = 1;
         }
         __syncthreads();                                   // (everyone has read what is written now)
-        t.next = to, t.whole = whole, t.piece = piece, t.first = at.q0, t.rows = rows, t.row0 = row0;
+        t.next = to, t.whole = whole, t.piece = piece, t.place = at, t.fresh = -1;
         return true;
     }
     __device__ __forceinline__ void done() const

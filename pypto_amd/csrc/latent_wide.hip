@@ -81,35 +81,20 @@ __global__ __launch_bounds__(THREADS) void latent_attention_wide_kernel(const La
         const int last = sight.last;                       // of the row tile's rows
         i_end = i_end < sight.tiles ? i_end : sight.tiles;
         const int ntiles = i_end > i_begin ? i_end - i_begin : 0;
-        auto key_of_tile = [&](const int n) { return sight.first_key(i_begin + (n < ntiles ? n : ntiles - 1)); };
+        auto key_of_tile = [&](const int n) { return sight.first_key(i_begin + n); };
         f32x16 o[16];                                      // block 4*rg + c: rows 32*rg .., value channels at 128w + 32c ..
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc_clear(o[i]);
         float m_run = LOW, l_run = 0.f;                    // of this lane's row: reference maximum, log2 domain; sum of exp2(s - m_run)
 
         if (ntiles > 0) {                                  // uniform
-            // Queries: a wave's own 32 rows, a row's latent part per request, 16-byte chunk i of row j at i ^ (j & 15).  Rows past the last one
-            // read it and are never stored.
-            const uint32_t q_lds = pool_lds + w * (32 * DN * 2);
-#pragma unroll 4
-            for (int j = 0; j < 32; ++j) {
-                const int r = sight.row0 + (32 * w + j < last ? 32 * w + j : last);
-                const int tok = divide(r, p.of_heads), head = r - tok * p.heads;
-                dma16_base(p.q + (long long)(at.q0 + tok) * p.q_t + (long long)head * p.q_h, (uint32_t)(16 * (l ^ (j & 15))), q_lds + j * (DN * 2));
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int j = 8 * i + (l >> 3), r = sight.row0 + (32 * w + j < last ? 32 * w + j : last);
-                const int tok = divide(r, p.of_heads), head = r - tok * p.heads;
-                dma16(p.qr + (long long)(at.q0 + tok) * p.qr_t + (long long)head * p.qr_h + 8 * ((l & 7) ^ (j & 7)), pool_lds + Q_ROPE_AT + (4 * w + i) * 1024);
-            }
-
             // Gather: wave w takes keys 8w .. 8w+7 of every tile, eight lanes each, a lane 64 channels of the latents (one scale) and eight of the
             // rope part.
             u32x4 raw[4], raw_rope;
             float raw_scale, next_scale;
             constexpr int NEAR = EIGHTS ? 8 : 1;
             auto row_of_tile = [&](const int n) __attribute__((always_inline)) { return page_of<NEAR>(p, at, key_of_tile(n) + 8 * w + (EIGHTS ? 0 : l >> 3)); };
+            Page page = row_of_tile(0), page1 = row_of_tile(1), page2 = row_of_tile(2);
             // (what hangs on the lane alone is made where it is used: kept, it would take the registers of the products' operands)
             auto lane = [&]() {
                 uint32_t x = tid & 63;
@@ -128,29 +113,40 @@ __global__ __launch_bounds__(THREADS) void latent_attention_wide_kernel(const La
                 const uint32_t x = lane();
                 raw_rope = global<u32x4>(row.rope, (EIGHTS ? x >> 3 : 0) * (uint32_t)p.cache.rope_pitch + 16 * (x & 7));
             };
-            // A tile's rows into LDS, in sixteen pieces of a dword per lane and one of the rope channels.  Of a row's 64 latent pieces of eight
-            // channels number 4 j + k lies at k * 16 + j.
+            // A tile's rows into LDS, in 32 pieces of two values per lane (one to a product: five vector instructions fit beside it) and one of the rope
+            // channels.  Of a row's 64 latent pieces of eight channels number 4 j + k lies at k * 16 + j.
             const uint32_t emit_off = (uint32_t)((8 * w + (l >> 3)) * PITCH + 32 * (l & 7));
             u32x4 dq;
             auto emit = [&](const uint32_t tile, const int d) __attribute__((always_inline)) {
-                const u32x2 x = dequant_dword(raw[d >> 2][d & 3], raw_scale);
-                if (d & 1) {
-                    dq[2] = x[0], dq[3] = x[1];
-                    *reinterpret_cast<u32x4 *>(pool + tile + emit_off + 256 * ((d >> 1) & 3) + 16 * (d >> 3)) = dq;
-                } else {
-                    dq[0] = x[0], dq[1] = x[1];
-                }
+                const uint32_t r = raw[d >> 3][(d >> 1) & 3];
+                dq[d & 3] = d & 1 ? dequant_upper(r, raw_scale) : dequant_lower(r, raw_scale);
+                if ((d & 3) == 3) *reinterpret_cast<u32x4 *>(pool + tile + emit_off + 256 * ((d >> 2) & 3) + 16 * (d >> 4)) = dq;
             };
             auto emit_rope = [&](const uint32_t tile) __attribute__((always_inline)) {
                 *reinterpret_cast<u32x4 *>(pool + tile + emit_off + (DN * 2 - 16 * (lane() & 7))) = raw_rope;
             };
-            Page page = row_of_tile(0), page1 = row_of_tile(1), page2 = row_of_tile(2);
+            // Queries: a wave's own 32 rows, a row's latent part per request, 16-byte chunk i of row j at i ^ (j & 15).  Rows past the last one
+            // read it and are never stored.
+            const uint32_t q_lds = pool_lds + w * (32 * DN * 2);
+#pragma unroll 4
+            for (int j = 0; j < 32; ++j) {
+                const int r = sight.row0 + (32 * w + j < last ? 32 * w + j : last);
+                const int tok = divide(r, p.of_heads), head = r - tok * p.heads;
+                dma16_base(p.q + (long long)(at.q0 + tok) * p.q_t + (long long)head * p.q_h, (uint32_t)(16 * (l ^ (j & 15))), q_lds + j * (DN * 2));
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int j = 8 * i + (l >> 3), r = sight.row0 + (32 * w + j < last ? 32 * w + j : last);
+                const int tok = divide(r, p.of_heads), head = r - tok * p.heads;
+                dma16(p.qr + (long long)(at.q0 + tok) * p.qr_t + (long long)head * p.qr_h + 8 * ((l & 7) ^ (j & 7)), pool_lds + Q_ROPE_AT + (4 * w + i) * 1024);
+            }
+
             {
                 const RowAt row = row_at(p, page);
                 ask_scale(row);
+                ask_rope(row);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) ask_latent(row, i);
-                ask_rope(row);
             }
             __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));      // (the queries too)
             asm volatile("" ::: "memory");
@@ -172,17 +168,17 @@ __global__ __launch_bounds__(THREADS) void latent_attention_wide_kernel(const La
             __syncthreads();                               // every wave has its queries: the tiles may go over them
             raw_scale = next_scale;
             check_scale<8>(raw_scale, raw_rope);
-            {
+            {                                              // (in the order of the loop's requests, or its first waits would be for the wrong ones)
                 const RowAt row = row_at(p, page1);
                 ask_scale(row);
+                emit_rope(0);
+                ask_rope(row);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
 #pragma unroll
-                    for (int d = 0; d < 4; ++d) emit(0, 4 * i + d);
+                    for (int d = 0; d < 8; ++d) emit(0, 8 * i + d);
                     ask_latent(row, i);
                 }
-                emit_rope(0);
-                ask_rope(row);
             }
 
             const int krow = tile_row_of(col);
@@ -212,31 +208,33 @@ __global__ __launch_bounds__(THREADS) void latent_attention_wide_kernel(const La
                     seen = sight.seen(first, sight.sees(tok), p.mask ? p.mask + (long long)(at.q0 + tok) * p.words : nullptr) >> (lane() >> 5);
                 }
             };
+            // The score products' key operands, AHEAD of their use; the rope part first, whose queries are read beside it.
+            constexpr int AHEAD = 4;
+            bf16x8 fa[8];
+            auto read_k = [&](const uint32_t tile, const int m) __attribute__((always_inline)) {
+                const int ks = m - DR / 16;
+                return *reinterpret_cast<const bf16x8 *>(pool + tile + (m < DR / 16 ? rbase + 32 * m : kbase + 512 * (ks & 1) + 16 * (ks >> 1)));
+            };
             // Scores of tile n, at `cur`; the next tile goes into `next`, the one behind it is asked for, and the first operands of the products
             // against V of the tile at `prev` are read.
             auto scores = [&](const uint32_t cur, const uint32_t prev, const uint32_t next, const RowAt &row, const int pbuf) __attribute__((always_inline)) {
-                // (the rope part first, whose queries are read beside it)
-                auto read_k = [&](const int m) {
-                    const int ks = m - DR / 16;
-                    return *reinterpret_cast<const bf16x8 *>(pool + cur + (m < DR / 16 ? rbase + 32 * m : kbase + 512 * (ks & 1) + 16 * (ks >> 1)));
-                };
-                bf16x8 fa[8], qr[DR / 16];
+                bf16x8 qr[DR / 16];
+#pragma unroll
+                for (int m = 0; m < AHEAD; ++m) fa[m] = read_k(cur, m);
 #pragma unroll
                 for (int e = 0; e < DR / 16; ++e) qr[e] = *reinterpret_cast<const bf16x8 *>(pool + Q_ROPE_AT + 4096 * w + 128 * (lane() & 31) + 16 * ((2 * e + half) ^ (lane() & 7)));
-#pragma unroll
-                for (int e = 0; e < 4; ++e) fa[e] = read_k(e);
 #pragma unroll
                 for (int m = 0; m < KSTEPS; ++m) {
                     if (m == 0) s_product_first(s, fa[0], qr[0]);
                     else s_product(s, fa[m & 7], m < DR / 16 ? qr[m % (DR / 16)] : qf[m >= DR / 16 ? m - DR / 16 : 0]);
                     __builtin_amdgcn_sched_barrier(0);
-                    if (m + 4 < KSTEPS) fa[(m + 4) & 7] = read_k(m + 4);
+                    if (m + AHEAD < KSTEPS) fa[(m + AHEAD) & 7] = read_k(cur, m + AHEAD);
                     if (m == 1) raw_scale = next_scale, check_scale<8>(raw_scale, raw_rope);
                     if (m == 2) ask_scale(row);
-                    if (m >= 3 && m < 19) emit(next, m - 3);
-                    if (m >= 7 && m < 23 && (m - 7) % 4 == 0) ask_latent(row, (m - 7) / 4);
-                    if (m == 20) emit_rope(next);
-                    if (m == 21) ask_rope(row);
+                    if (m >= 3 && m < 35) emit(next, m - 3);
+                    if (m >= 11 && (m - 11) % 8 == 0) ask_latent(row, (m - 11) / 8);
+                    if (m == 4) emit_rope(next);
+                    if (m == 5) ask_rope(row);
                     if (m >= 25 && m < 33 && (m & 1)) load_p(pbuf, 0, (m - 25) >> 1);
                     if (m == 33 || m == 34) load_v(prev, m - 33);
                     __builtin_amdgcn_sched_barrier(0);
@@ -315,6 +313,7 @@ __global__ __launch_bounds__(THREADS) void latent_attention_wide_kernel(const La
                     if (rg == 0 && i + 2 < 8) load_v(prev, i + 2);
                     if (i == 3) load_p(pbuf, 1, rg);
                     if (SM && mp > 0) softmax_step(mp - 1, n, pbuf ^ 1);
+                    if (SM && mp == 28) page = row_of_tile(n + 3);
                     __builtin_amdgcn_sched_barrier(0);
                 }
             };
@@ -330,7 +329,6 @@ __global__ __launch_bounds__(THREADS) void latent_attention_wide_kernel(const La
             for (int n = 0; n < ntiles; ++n) {
                 // (what branches stands here: around a branch among the products registers would move)
                 const RowAt row = row_at(p, page);
-                page = row_of_tile(n + 3);
                 look(n);
                 scores(cur, prev, next, row, pbuf);
                 values(std::true_type{}, prev, pbuf, n);
@@ -353,7 +351,7 @@ __global__ __launch_bounds__(THREADS) void latent_attention_wide_kernel(const La
         __syncthreads();
         // (what is known of the row tile comes back from LDS: see LineTable)
         const bool whole = line.one(table.whole) != 0;
-        const int piece = line.one(table.piece), rows = line.one(table.rows), row0 = line.one(table.row0), first = line.one(table.first);
+        const int piece = line.one(table.piece), first = line.one(table.place.q0), rows = line.one(table.place.n) * p.heads, row0 = line.one(table.place.row_tile) * ROWS;
         float *const il = reinterpret_cast<float *>(pool + ALPHA_AT);
         if (half == 0) {
             const int r = 32 * w + col;

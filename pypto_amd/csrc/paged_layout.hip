@@ -3,6 +3,8 @@
 //
 // All of it is whole numbers from lengths: sums over the sequences before one, then a look-up per page or token.  Bound by the chain
 // of latencies (lengths, sums, table), not by bytes; the sums are made again by every workgroup rather than by a launch of their own.
+#include <type_traits>
+
 #include "common.h"
 #include "serving_ops.h"
 
@@ -54,62 +56,160 @@ __device__ __forceinline__ int last_up_to(const uint32_t *at, const int n, const
 }
 
 // One workgroup: what is given back decides what can be taken, and the count of free pages is read and written in one place.  Per 1024 sequences the
-// pages are counted out and dealt to the threads, whichever sequence they are of.
-constexpr int PG_THREADS = 1024;
+// pages are counted out and dealt to the threads, neighbouring ones to neighbouring threads, whichever sequence they are of: which one that is is
+// looked up where there are no more pages than threads, else marked where a sequence's pages begin and carried on by a running maximum, for 8192
+// pages at a time, whose loads are then on their way together.  A chain of latencies (lengths, sums, table, sums, stack): 32 sequences of which some pass a
+// page's end 5.6 us; 1000 of which 50 end and 50 begin, 11 000 pages in all, 19 (one page to a thread at a time, each looked up, 27; counts of the waves
+// added one by one instead of by a scan over lanes, 27).
+constexpr int PG_THREADS = 1024, PG_EACH = 8, PG_WINDOW = PG_THREADS * PG_EACH;
+
+// sums of x and of y over this lane and all lanes before it
+__device__ __forceinline__ void wave_sums(int &x, int &y)
+{
+    auto add = [&](auto ctrl, auto rows) __attribute__((always_inline)) {
+        x += __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, decltype(rows)::value, 0xf, false);
+        y += __builtin_amdgcn_update_dpp(0, y, decltype(ctrl)::value, decltype(rows)::value, 0xf, false);
+    };
+    const std::integral_constant<int, 0xf> all;
+    add(std::integral_constant<int, 0x111>{}, all);        // row_shr:1, 2, 4, 8: within rows of sixteen lanes
+    add(std::integral_constant<int, 0x112>{}, all);
+    add(std::integral_constant<int, 0x114>{}, all);
+    add(std::integral_constant<int, 0x118>{}, all);
+    add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});     // row_bcast:15: rows 0 and 2 into 1 and 3
+    add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});     // row_bcast:31: the lower half into the upper
+}
 
 __global__ __launch_bounds__(PG_THREADS) void cache_pages_kernel(const CachePagesParams p)
 {
-    __shared__ uint32_t of_waves[PG_THREADS / 64], begin[PG_THREADS];
-    __shared__ int from[PG_THREADS];
-    const int tid = threadIdx.x;
+    constexpr int WAVES = PG_THREADS / 64;
+    __shared__ int of_waves[2][WAVES], counts[PG_EACH * WAVES];
+    __shared__ uint32_t begin[2][PG_THREADS];
+    __shared__ int from[2][PG_THREADS];
+    __shared__ uint16_t of[PG_WINDOW];
+    const int tid = threadIdx.x, l = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     auto pages = [&](const int n) {
         const long long k = n > 0 ? ((long long)n + p.bs - 1) / p.bs : 0;
         return (int)(k < p.maxblk ? k : p.maxblk);
     };
     const int given = *p.count;
     int top = given < 0 ? 0 : (given < p.room ? given : (int)p.room);
+    uint32_t taken = 0, totals[2] = {0, 0};
     for (int way = 0; way < 2; ++way) {                    // pages given back, then pages taken
-        uint32_t taken = 0;
         for (int base = 0; base < p.B; base += PG_THREADS) {
-            const int b = base + tid, here = p.B - base < PG_THREADS ? p.B - base : PG_THREADS;
-            int lo = 0, n = 0;
-            if (b < p.B) {
-                const int had = pages(p.before[b]), has = pages(p.after[b]);
-                lo = way == 0 ? has : had;
-                n = way == 0 ? had - has : has - had;
-                n = n > 0 ? n : 0;
-            }
-            uint32_t total;
-            const uint32_t upto = block_sums<PG_THREADS>((uint32_t)n, of_waves, total);
-            if (total == 0) continue;                      // (the same for all threads)
-            begin[tid] = upto - (uint32_t)n;
-            from[tid] = lo;
-            __syncthreads();
-            for (uint32_t e0 = 0; e0 < total; e0 += PG_THREADS) {
-                const uint32_t e = e0 + tid;
-                int32_t *entry = nullptr;
-                if (e < total) {
-                    const int s = last_up_to<PG_THREADS>(begin, here, e);
-                    entry = p.bt + (long long)(base + s) * p.maxblk + from[s] + (int)(e - begin[s]);
+            const int here = p.B - base < PG_THREADS ? p.B - base : PG_THREADS;
+            if (way == 0 || p.B > PG_THREADS) {            // (all pages of a table are fewer than 2^31)
+                int had = 0, has = 0;
+                if (tid < here) had = pages(p.before[base + tid]), has = pages(p.after[base + tid]);
+                const int back = had > has ? had - has : 0, more = has > had ? has - had : 0;
+                int x = back, y = more;
+                wave_sums(x, y);
+                if (l == 63) of_waves[0][w] = x, of_waves[1][w] = y;
+                __syncthreads();
+                totals[0] = totals[1] = 0;
+#pragma unroll
+                for (int i = 0; i < WAVES; ++i) {
+                    if (i == w) x += totals[0], y += totals[1];
+                    totals[0] += of_waves[0][i], totals[1] += of_waves[1][i];
                 }
+                begin[0][tid] = x - back, begin[1][tid] = y - more;
+                from[0][tid] = has, from[1][tid] = had;
+                __syncthreads();
+            }
+            const uint32_t total = totals[way];            // (the same for all threads)
+            for (uint32_t e0 = 0; e0 < total; e0 += PG_WINDOW) {
+                const bool few = total <= PG_THREADS;
+                if (!few) {                                // of[i]: the sequence that page e0 + i is of
+#pragma unroll
+                    for (int j = 0; j < PG_EACH; ++j) of[j * PG_THREADS + tid] = 0;
+                    __syncthreads();
+                    const int mine = tid < here ? (int)((tid + 1 < here ? begin[way][tid + 1] : total) - begin[way][tid]) : 0;
+                    const long long at = (long long)begin[way][tid] - e0;
+                    if (mine > 0 && at < PG_WINDOW && at + mine > 0) of[at > 0 ? at : 0] = (uint16_t)tid;
+                    __syncthreads();
+                    // (a thread's eight are neighbours here)
+                    int most = 0, run[PG_EACH];
+#pragma unroll
+                    for (int j = 0; j < PG_EACH; ++j) {
+                        const int x = of[PG_EACH * tid + j];
+                        most = most > x ? most : x;
+                        run[j] = most;
+                    }
+                    int x = most;
+#pragma unroll
+                    for (int d = 1; d < 64; d *= 2) {
+                        const int y = __shfl_up(x, d);
+                        if (l >= d) x = x > y ? x : y;
+                    }
+                    if (l == 63) of_waves[0][w] = x;
+                    int before = __shfl_up(x, 1);
+                    if (l == 0) before = 0;
+                    __syncthreads();
+                    for (int i = 0; i < w; ++i) before = before > of_waves[0][i] ? before : of_waves[0][i];
+#pragma unroll
+                    for (int j = 0; j < PG_EACH; ++j) of[PG_EACH * tid + j] = (uint16_t)(run[j] > before ? run[j] : before);
+                    __syncthreads();
+                }
+                int32_t *entry[PG_EACH];
+                int page[PG_EACH];
+#pragma unroll
+                for (int j = 0; j < PG_EACH; ++j) {
+                    const uint32_t e = e0 + j * PG_THREADS + tid;
+                    entry[j] = nullptr;
+                    if (e < total) {
+                        const int s = few ? last_up_to<PG_THREADS>(begin[way], here, e) : of[j * PG_THREADS + tid];
+                        entry[j] = p.bt + (long long)(base + s) * p.maxblk + from[way][s] + (int)(e - begin[way][s]);
+                    }
+                    if (few) break;                        // (uniform)
+                }
+                const int n = few ? 1 : PG_EACH;
                 if (way == 0) {
-                    const int page = entry ? *entry : -1;
-                    uint32_t back;
-                    const uint32_t at = block_sums<PG_THREADS>(page >= 0 ? 1 : 0, of_waves, back);
-                    const long long to = (long long)top + at - 1;
-                    if (page >= 0 && to < p.room) p.stack[to] = page;
-                    top = (long long)top + back < p.room ? top + (int)back : (int)p.room;
-                } else if (entry) {
-                    const long long at = (long long)top - 1 - taken - e;
-                    *entry = at >= 0 ? p.stack[at] : -1;
+#pragma unroll
+                    for (int j = 0; j < PG_EACH; ++j)
+                        if (j < n) page[j] = entry[j] ? *entry[j] : -1;
+                    // pages that there are, in order: by the eighth of the window, then by the wave
+                    uint64_t there[PG_EACH];
+#pragma unroll
+                    for (int j = 0; j < PG_EACH; ++j)
+                        if (j < n) {
+                            there[j] = __ballot(page[j] >= 0);
+                            if (l == 0) counts[j * WAVES + w] = __popcll(there[j]);
+                        }
+                    __syncthreads();
+                    static_assert(PG_EACH * WAVES == 128, "two counts to a lane");
+                    const int c0 = 2 * l < n * WAVES ? counts[2 * l] : 0, c1 = 2 * l < n * WAVES ? counts[2 * l + 1] : 0;
+                    int with = c0 + c1, other = 0;
+                    wave_sums(with, other);
+#pragma unroll
+                    for (int j = 0; j < PG_EACH; ++j) {
+                        if (j >= n) break;
+                        const int pair = j * (WAVES / 2) + w / 2;
+                        const long long to = (long long)top + __builtin_amdgcn_readlane(with, pair) - __builtin_amdgcn_readlane(c1, pair)
+                                     - (w & 1 ? 0 : __builtin_amdgcn_readlane(c0, pair));
+                        const long long at = to + __popcll(there[j] & ((1ull << l) - 1));
+                        if (page[j] >= 0 && at < p.room) p.stack[at] = page[j];
+                    }
+                    const long long all = (long long)top + __builtin_amdgcn_readlane(with, 63);
+                    top = all < p.room ? (int)all : (int)p.room;
+                    __syncthreads();
+                } else {
+#pragma unroll
+                    for (int j = 0; j < PG_EACH; ++j)
+                        if (j < n) {
+                            const long long at = (long long)top - 1 - taken - (e0 + j * PG_THREADS + tid);
+                            page[j] = entry[j] && at >= 0 ? p.stack[at] : -1;
+                        }
+#pragma unroll
+                    for (int j = 0; j < PG_EACH; ++j)
+                        if (j < n && entry[j]) *entry[j] = page[j];
+                    __syncthreads();
                 }
             }
-            taken = add_up_to_most(taken, total);
-            __syncthreads();
+            if (way == 1) taken += total;
+            if (p.B > PG_THREADS) __syncthreads();
         }
-        __syncthreads();
-        if (way == 1 && tid == 0) *p.left = (long long)top - taken > 0 ? top - (int)taken : 0;
+        __syncthreads();                                   // (the pages on the stack are there for all)
     }
+    if (tid == 0) *p.left = (long long)top - taken > 0 ? top - (int)taken : 0;
 }
 
 // A workgroup takes the tokens t0 .. t1 - 1, a thread one at a time; the beginnings of up to 1024 sequences are in LDS.
