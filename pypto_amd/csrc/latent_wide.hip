@@ -30,10 +30,12 @@ constexpr int PIECE = ROWS * DN;
 // O^T stays in the accumulation registers: anything but products on it, inside the loop, would move it into the others.
 __device__ __forceinline__ void acc_product(f32x16 &acc, const bf16x8 a, const bf16x8 b) { acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, acc, 0, 0, 0); }
 // (a product of zeros: written one by one, a block's registers would come together in the others first)
+// A product needs two wait states behind a vector instruction that wrote one of its operands, and for products in assembly the compiler counts none: here
+// the zeros were written last, and without the wait the first block was what had been in their registers.
 __device__ __forceinline__ void acc_clear(f32x16 &acc)
 {
     const bf16x8 zero = {};
-    asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %1, 0" : "=a"(acc) : "v"(zero));
+    asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %1, 0" : "=a"(acc) : "v"(zero));
 }
 __device__ __forceinline__ void acc_scale(f32x16 &acc, const float alpha)
 {
@@ -53,8 +55,8 @@ __device__ __forceinline__ f32x4 acc_read(const f32x16 &acc, const int q4)
     return f32x4{r0, r1, r2, r3};
 }
 // The scores' accumulator stays out of them: products on one destination after the other (no wait states among them), then the wait
-// that a vector instruction's read needs.
-__device__ __forceinline__ void s_product_first(f32x16 &s, const bf16x8 a, const bf16x8 b) { asm("v_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(s) : "v"(a), "v"(b)); }
+// that a vector instruction's read needs.  Their operands come from LDS, or stay in registers from before the loop (a wait in front of each cost 1 %).
+__device__ __forceinline__ void s_product_first(f32x16 &s, const bf16x8 a, const bf16x8 b) { asm("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(s) : "v"(a), "v"(b)); }
 __device__ __forceinline__ void s_product(f32x16 &s, const bf16x8 a, const bf16x8 b) { asm("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(s) : "v"(a), "v"(b)); }
 __device__ __forceinline__ void s_done(f32x16 &s) { asm volatile("s_nop 15\n\ts_nop 3" : "+v"(s)); }
 __device__ __forceinline__ void products_to_vector() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
