@@ -435,18 +435,30 @@ __global__ __launch_bounds__(256) void latent_join_kernel(const LaParams p)
     f32x4 acc[4];
 #pragma unroll
     for (int q4 = 0; q4 < 4; ++q4) acc[q4] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int k = wave; k < n; k += 4) {
-        const f32x2 ml = *reinterpret_cast<const f32x2 *>(p.part_ml + (place(k) * TILE_ROWS + 32 * group + col) * 2);
-        const float *src = p.part_o + place(k) * (TILE_ROWS * DN) + ((w * OF_WAVE + i) * 256 + l) * 4;
-        f32x4 x[4];
+    auto take = [&](const int k0, auto count) __attribute__((always_inline)) {
+        constexpr int EACH = decltype(count)::value;       // pieces asked for at once
+        f32x2 ml[EACH];
+        f32x4 x[EACH][4];
 #pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4) x[q4] = *reinterpret_cast<const f32x4 *>(src + q4 * 256);
-        const float m = fmaxf(top, ml[0]), a = __builtin_amdgcn_exp2f(top - m), b = __builtin_amdgcn_exp2f(ml[0] - m);
-        top = m;
-        total = total * a + ml[1] * b;
+        for (int j = 0; j < EACH; ++j) {
+            const long long at = place(k0 + 4 * j);
+            ml[j] = *reinterpret_cast<const f32x2 *>(p.part_ml + (at * TILE_ROWS + 32 * group + col) * 2);
+            const float *src = p.part_o + at * (TILE_ROWS * DN) + ((w * OF_WAVE + i) * 256 + l) * 4;
 #pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4) acc[q4] = acc[q4] * a + x[q4] * b;
-    }
+            for (int q4 = 0; q4 < 4; ++q4) x[j][q4] = *reinterpret_cast<const f32x4 *>(src + q4 * 256);
+        }
+#pragma unroll
+        for (int j = 0; j < EACH; ++j) {
+            const float m = fmaxf(top, ml[j][0]), a = __builtin_amdgcn_exp2f(top - m), b = __builtin_amdgcn_exp2f(ml[j][0] - m);
+            top = m;
+            total = total * a + ml[j][1] * b;
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4) acc[q4] = acc[q4] * a + x[j][q4] * b;
+        }
+    };
+    int k = wave;
+    for (; k + 12 < n; k += 16) take(k, std::integral_constant<int, 4>{});
+    for (; k < n; k += 4) take(k, std::integral_constant<int, 1>{});
     if (wave > 0) {
 #pragma unroll
         for (int q4 = 0; q4 < 4; ++q4) sums[wave - 1][q4][l] = acc[q4];
