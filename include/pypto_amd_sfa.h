@@ -733,7 +733,8 @@ int pto_cache_slots_launch(const PtoCacheSlotsArgs *args, void *hip_stream);
  * the keys before the sequence's query tokens and, of theirs, key j where bit j % 64 of word j / 64 of its mask is set.  Rows that see no key are
  * zeros, their lse -infinity; rows of no sequence stay as they were.  Keys that a row does not see may hold anything, infinite scales too.
  * Positions without a page (an entry below zero, or a page outside the cache) read as zeros, as latents and as rope; keys that the table is too
- * short for do not exist.  Beginnings outside the queries are moved into them.
+ * short for do not exist.  Beginnings outside the queries are moved into them; where they do not ascend nothing outside is touched, but what is
+ * written is not determined.
  *
  * Constraints: total_q * heads below 2^31 - 65536; mask_words up to 16, not together with a window.  Alignment: queries 16 bytes, their strides
  * multiples of 8 elements; cache arrays 16 bytes; the others their element's.  The workspace holds partial results: launches that may run at the

@@ -49,7 +49,7 @@ int latent_check(const PtoLatentAttentionArgs *a)
 }
 
 struct LatentPlan {
-    int wide, most_tiles, groups, by_tile, entries;
+    int wide, most_tiles, row_tiles, groups, by_tile, entries;
     size_t o_bytes, ml_bytes, join_bytes;
 };
 
@@ -75,6 +75,7 @@ LatentPlan latent_plan(const PtoLatentAttentionArgs *a)
     const int rows = pl.wide ? pto::LA_WIDE_ROWS : pto::LA_ROWS;
     const long long row_tiles = row_tiles_of(rows), tiles = tiles_of(rows);
     pl.most_tiles = (int)tiles;
+    pl.row_tiles = (int)row_tiles;
     const double pieces = (double)row_tiles * (double)(tiles + pto::LA_OPEN) / pto::LA_LEAST;
     const long long groups = pieces < (double)cus ? (long long)pieces + 1 : cus;
     pl.groups = (int)((groups + 7) / 8 * 8);
@@ -226,6 +227,7 @@ int pto_latent_attention_launch(const PtoLatentAttentionArgs *a, void *hip_strea
     p.per_entry = (int)((a->b + threads - 1) / threads);
     p.seq_entries = (int)((a->b + p.per_entry - 1) / p.per_entry);
     p.groups = pl.groups;
+    p.most_row_tiles = pl.row_tiles;
     p.by_tile = pl.by_tile;
     p.entries = pl.entries;
     p.of_heads = pto::divisor_of((uint32_t)a->heads);

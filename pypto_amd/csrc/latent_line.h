@@ -135,7 +135,8 @@ __device__ __forceinline__ int moved(const int x, const int len) { return x <= N
 template <int THREADS>
 struct LineTable {
     long long upto[THREADS], of_waves[THREADS / 64];
-    int tiles_upto[THREADS], tiles_of_waves[THREADS / 64];
+    long long tiles_of_waves[THREADS / 64];
+    int tiles_upto[THREADS];
     int q0[THREADS], n[THREADS], keys[THREADS];            // of an entry's first sequence
     long long units, share, end, next;                     // end: of this workgroup's part; next: the unit behind the row tile's part in hand
     int groups, g, rest, said;
@@ -157,25 +158,26 @@ struct Line {
     __device__ __forceinline__ bool begin() const
     {
         const int tid = threadIdx.x, w = tid >> 6;
-        long long mine = 0;
-        int own_tiles = 0;
+        long long mine = 0, tiles = 0;
         for (int j = 0; j < p.per_entry; ++j) {
             const int b = tid * p.per_entry + j;
             if (b < p.B) {
                 const Sequence c = sequence<ROWS>(p, b);
                 if (j == 0) t.q0[tid] = c.q0, t.n[tid] = c.n, t.keys[tid] = c.keys;
-                mine += (long long)c.row_tiles * (c.tiles + LA_OPEN), own_tiles += c.row_tiles;
+                mine += (long long)c.row_tiles * (c.tiles + LA_OPEN), tiles += c.row_tiles;
             }
         }
         mine = wave_sums(mine);
-        int tiles = (int)wave_sums((long long)own_tiles);
+        tiles = wave_sums(tiles);
         if ((tid & 63) == 63) t.of_waves[w] = mine, t.tiles_of_waves[w] = tiles;
         __syncthreads();
         for (int i = 0; i < w; ++i) mine += t.of_waves[i], tiles += t.tiles_of_waves[i];
         t.upto[tid] = mine;
-        t.tiles_upto[tid] = tiles;
+        t.tiles_upto[tid] = tiles <= p.most_row_tiles ? (int)tiles : -1;
         __syncthreads();
-        const long long units = first_of(t.upto[THREADS - 1]);
+        // (sequences that overlap, of beginnings that do not ascend, may be more than there are rows and joins for: then nothing is done)
+        const int all_tiles = one(t.tiles_upto[THREADS - 1]);
+        const long long units = all_tiles < 0 ? 0 : first_of(t.upto[THREADS - 1]);
         // workgroups that take part, so that none gets less than LA_LEAST units
         const int pieces = units < (long long)p.groups * LA_LEAST ? (int)units / LA_LEAST : p.groups, groups = pieces > 0 ? pieces : 1;
         const int per_xcd = (groups + 7) / 8, slot = blockIdx.x >> 3, g = (int)(blockIdx.x & 7) * per_xcd + slot;
@@ -184,7 +186,7 @@ struct Line {
             // Which row tiles are joined, and from how many pieces, is said by the workgroup that has the first of them; for every other entry that
             // there are none
             if (p.by_tile) {
-                for (int i = one(t.tiles_upto[THREADS - 1]) + (int)blockIdx.x; i < p.entries; i += (int)gridDim.x) p.joins[4 * i + 1] = 0;
+                for (int i = (all_tiles < 0 ? 0 : all_tiles) + (int)blockIdx.x; i < p.entries; i += (int)gridDim.x) p.joins[4 * i + 1] = 0;
             } else if (!there) {
                 p.joins[4 * blockIdx.x + 1] = 0;
             }

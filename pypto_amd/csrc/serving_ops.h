@@ -79,6 +79,7 @@ struct LaParams {
     int per_entry, seq_entries;           // sequences that a workgroup's thread counts; threads that count any
     int wide;                             // row tiles of LA_WIDE_ROWS
     int groups;                           // workgroups, a multiple of eight
+    int most_row_tiles;                   // of sequences that do not overlap
     int by_tile, entries;                 // joins by row tile (of all sequences), else by workgroup; how many there are
     Divisor of_heads, of_bs;
     float scale_log2;

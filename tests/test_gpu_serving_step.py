@@ -174,3 +174,62 @@ def test_a_prompt_with_a_window_and_single_tokens_over_the_cache_it_left(window,
     through = torch.stack([latent_out[:, h].float() @ w_uv[h].float().T for h in range(HEADS)], dim=1)
     assert float((through - out.float()).norm() / out.float().norm()) <= 0.03
     assert float((latent_lse - lse).abs().max()) <= 0.03 * float(lse.abs().max())
+
+
+def test_what_is_refused_on_the_device():
+    """Outputs in the memory of inputs, addresses and strides that the kernels do not take: nothing is launched."""
+    z = lambda *s, dtype=BF: torch.zeros(s, dtype=dtype, device=DEV)  # noqa: E731
+    within = lambda t, dtype, *s: t.reshape(-1).view(dtype)[:torch.Size(s).numel()].view(s)  # noqa: E731
+
+    def refused(text, op, args, at=None, value=None, kind=ValueError, **kw):
+        with pytest.raises(kind, match=text):
+            op(*(value if i == at else x for i, x in enumerate(args)), **kw)
+
+    pages = [z(3, dtype=I32), z(3, dtype=I32), z(3, 5, dtype=I32), z(20, dtype=I32), z(1, dtype=I32), z(1, dtype=I32), 128]
+    refused("overlap", pypto_amd.cache_pages, pages, 0, within(pages[2], I32, 3))
+    refused("overlap", pypto_amd.cache_pages, pages, 3, pages[2].view(-1)[3:])
+    refused("overlap", pypto_amd.cache_pages, pages, 5, pages[3][:1])
+    refused("block_size", pypto_amd.cache_pages, pages, 6, 0, kind=(ValueError, RuntimeError))
+    slots = [z(3, dtype=I32), z(3, dtype=I32), z(3, 5, dtype=I32), z(4, dtype=I32), z(4, dtype=I32), z(9, dtype=I64), z(9, dtype=I64), 128]
+    refused("overlap", pypto_amd.cache_slots, slots, 6, slots[5])
+    refused("overlap", pypto_amd.cache_slots, slots, 0, within(slots[5], I32, 3))
+    refused("overlap", pypto_amd.cache_slots, slots, parents=within(slots[6], I32, 9), tree_mask=z(9, 1, dtype=I64))
+    refused("mask", pypto_amd.cache_slots, slots, parents=z(9, dtype=I32), tree_mask=z(9, 17, dtype=I64))
+    latent = [z(6, 4, 512), z(6, 4, 64), z(256, 512, dtype=torch.int8), z(256, 64), z(256, 4, dtype=torch.float32), z(2, 3, dtype=I32), z(3, dtype=I32), z(2, dtype=I32),
+              z(6, 4, 512), 0.1, 128]
+    op = pypto_amd.latent_attention
+    for at, shape, dtype in ((0, (6, 4, 512), BF), (5, (2, 3), I32), (6, (3,), I32), (7, (2,), I32)):
+        refused("overlap", op, latent, at, within(latent[8], dtype, *shape))
+    refused("overlap", op, latent, softmax_lse=within(latent[0], torch.float32, 6, 4))
+    refused("overlap", op, latent, tree_mask=within(latent[8], I64, 6, 1))
+    refused("exclude", op, latent, tree_mask=z(6, 1, dtype=I64), window=3)
+    refused("window", op, latent, window=0)
+    refused("tree_mask", op, latent, tree_mask=z(5, 1, dtype=I64))
+    refused("16-byte", op, latent, 0, z(6 * 4 * 512 + 4)[4:].view(6, 4, 512), kind=(ValueError, RuntimeError))
+    refused("multiples of 8", op, latent, 1, z(6, 4, 68)[:, :, :64], kind=(ValueError, RuntimeError))
+    refused("GPU|device", op, latent, 7, torch.zeros(2, dtype=I32), kind=(ValueError, RuntimeError))
+    prompt = [z(6, 4, 128), z(9, 2, 128), z(9, 2, 128), ints([0, 6]), ints([0, 9]), z(6, 4, 128), 0.1, 5]
+    refused("overlap", pypto_amd.prompt_window_attention, prompt, 5, prompt[0])
+    refused("overlap", pypto_amd.prompt_window_attention, prompt, 3, within(prompt[5], I32, 2))
+    refused("window", pypto_amd.prompt_window_attention, prompt, 7, 0)
+
+
+def test_calls_on_two_streams_at_once():
+    """Each with its own workspace: the results of either are those it has alone."""
+    from test_gpu_latent_attention import Call
+    calls = [Call([30, 1, 40], [3000, 9000, 900], HEADS, words=1, seed=i, packed=i == 1) for i in range(4)]
+    alone = []
+    for c in calls:
+        c.run()
+        alone.append((c.out.clone(), c.lse.clone()))
+        c.out.fill_(7.0), c.lse.fill_(7.0)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    for _ in range(5):
+        for c, s in zip(calls, streams):
+            with torch.cuda.stream(s):
+                c.run()
+    torch.cuda.synchronize()
+    for c, (out, lse) in zip(calls, alone):
+        c.check()
+        assert torch.equal(c.out, out) and torch.equal(c.lse, lse)
