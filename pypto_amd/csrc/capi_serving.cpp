@@ -56,8 +56,9 @@ struct LatentPlan {
 // The device divides the work, since lengths are there.  Here only as many workgroups as there can be pieces of LA_LEAST units, one to a
 // compute unit at most (a workgroup's LDS is most of one's), and memory for two pieces of each.
 // 128 rows to a workgroup take 0.6 of the time that 64 take for as many, but twice the bytes for a piece: for sequences that fill them, and where the keys that
-// the table has room for could keep each compute unit for 40 tiles of 64 rows (24 sequences of 25 to 63 tokens, 128 heads, 500 to 9000 keys: 1390 us, with
-// 64 rows 1660; single tokens of 32 sequences over 2052 keys, 128 heads: 57, with 64 rows 52).
+// the table has room for could keep each compute unit for 28 tiles of 64 rows.  With 128 rows and with 64, us, all of 128 heads: 24 sequences of 25 to 63
+// tokens over 500 to 9000 keys 1340 and 1660; 4 of 30 over 2030 keys 98.6 and 111.3; 2 of 30 (30 tiles) 63.9 and 66.1; single tokens of 32 over 2052 (25 tiles)
+// 50.0 and 47.9; one token over 30000 (11) 44.3 and 34.6.
 LatentPlan latent_plan(const PtoLatentAttentionArgs *a)
 {
     LatentPlan pl{};
@@ -71,7 +72,7 @@ LatentPlan latent_plan(const PtoLatentAttentionArgs *a)
         const long long w = (a->sinks + pto::LA_KEYS - 1) / pto::LA_KEYS + (reach + pto::LA_KEYS - 1) / pto::LA_KEYS + 1;
         return w < all ? w : all;
     };
-    pl.wide = a->total_q * a->heads >= 96 * a->b && (double)row_tiles_of(pto::LA_ROWS) * (double)tiles_of(pto::LA_ROWS) >= 40.0 * (double)cus;
+    pl.wide = a->total_q * a->heads >= 96 * a->b && (double)row_tiles_of(pto::LA_ROWS) * (double)tiles_of(pto::LA_ROWS) >= 28.0 * (double)cus;
     const int rows = pl.wide ? pto::LA_WIDE_ROWS : pto::LA_ROWS;
     const long long row_tiles = row_tiles_of(rows), tiles = tiles_of(rows);
     pl.most_tiles = (int)tiles;
