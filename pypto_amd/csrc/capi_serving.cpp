@@ -35,7 +35,8 @@ int latent_check(const PtoLatentAttentionArgs *a)
     if (rc != PTO_OK) return rc;
     if (a->total_q < 0 || a->total_q > MOST_TOKENS || a->heads < 1 || a->heads > 65536 || a->total_q * a->heads > 0x7fff0000ll)
         return fail(PTO_E_INVALID_ARG, "latent_attention: total_q or heads out of range");
-    if (a->max_blocknum_perbatch * a->block_size > 0x7ffffff0ll)
+    static_assert(pto::LA_MOST_KEYS == 0x7fffffff - 15);
+    if (a->max_blocknum_perbatch * a->block_size > pto::LA_MOST_KEYS)
         return fail(PTO_E_INVALID_ARG, "latent_attention: a sequence of the block table holds at most 2^31 - 16 keys");
     if (a->window < 0 || a->window > MOST_TOKENS || a->sinks < 0 || a->sinks > MOST_TOKENS)
         return fail(PTO_E_INVALID_ARG, "latent_attention: window and sinks must be in [0, 2^30]");

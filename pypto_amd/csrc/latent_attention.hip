@@ -240,7 +240,7 @@ __global__ __launch_bounds__(THREADS) void latent_attention_kernel(const LaParam
             auto take_scores = [&](const int n) __attribute__((always_inline)) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) sv[e] = s[e];
-                const int first = key_of_tile(n);
+                const uint32_t first = key_of_tile(n);
                 if (!sight.whole(first)) {                 // (uniform)
                     const uint32_t seen = sight.seen(first, my_sees, my_mask);
 #pragma unroll

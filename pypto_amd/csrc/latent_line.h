@@ -93,7 +93,7 @@ template <int ROWS>
 __device__ __forceinline__ void count_tiles(const LaParams &p, Sequence &c)
 {
     c.row_tiles = (c.n * p.heads + ROWS - 1) / ROWS;
-    c.tiles = (c.keys + KT - 1) / KT;
+    c.tiles = la_tiles_of(c.keys);
     c.tiles = c.tiles < p.most_tiles ? c.tiles : p.most_tiles;
 }
 template <int ROWS>
@@ -298,30 +298,32 @@ struct Sight {
         sink_tiles = (p.sinks + KT - 1) / KT;
         sink_tiles = sink_tiles < low ? sink_tiles : low;
         skip = low - sink_tiles;
-        tiles = (most + KT - 1) / KT - skip;
+        tiles = la_tiles_of(most) - skip;
     }
     __device__ __forceinline__ int sees(const int tok) const
     {
-        const int s = tok + 1 + keys - n;
+        const int s = keys - n + tok + 1;
         return p.mask ? keys : (s < 0 ? 0 : s);
     }
     __device__ __forceinline__ int from(const int s) const { return p.window > 0 && s > p.window ? s - p.window : 0; }
-    __device__ __forceinline__ int first_key(const int i) const { return KT * (i < sink_tiles ? i : i + skip); }
+    // (without a sign: a tile asked for ahead may lie behind the last key, and past 2^31)
+    __device__ __forceinline__ uint32_t first_key(const int i) const { return (uint32_t)KT * (uint32_t)(i < sink_tiles ? i : i + skip); }
     // whether all rows see all 32 keys from this one on
-    __device__ __forceinline__ bool whole(const int first) const
+    __device__ __forceinline__ bool whole(const uint32_t first) const
     {
-        return first + KT <= least && (first >= low_last || first + KT <= p.sinks);
+        return first + KT <= (uint32_t)least && (first >= (uint32_t)low_last || first + KT <= (uint32_t)p.sinks);
     }
     // Bit i: whether a row that sees `s` keys (with this mask, if there is one) sees key first + i.
-    __device__ __forceinline__ uint32_t seen(const int first, const int s, const unsigned long long *mask) const
+    __device__ __forceinline__ uint32_t seen(const uint32_t first_key, const int s, const unsigned long long *mask) const
     {
+        const int first = (int)first_key;                  // (of a tile that has keys)
         auto below = [](int x) {
             x = x < 0 ? 0 : (x > 32 ? 32 : x);
             return (uint32_t)((1ull << x) - 1);
         };
         const int sinks = p.sinks < s ? p.sinks : s;
         uint32_t bits = (below(s - first) & ~below(from(s) - first)) | below(sinks - first);
-        if (mask && first + KT > context) {                // of the tile's keys, those in front of the tree and those of it that the mask names
+        if (mask && first_key + KT > (uint32_t)context) {                // of the tile's keys, those in front of the tree and those of it that the mask names
             const int node = first - context, at_word = node >> 6, shift = node & 63;
             auto word = [&](const int i) { return i < 0 ? ~0ull : (i < p.words ? mask[i] : 0ull); };
             const unsigned long long lo = word(at_word), hi = word(at_word + 1);
@@ -357,10 +359,10 @@ struct RowAt {
     const uint8_t *nope, *scale, *rope;
 };
 template <int NEAR>
-__device__ __forceinline__ Page page_of(const LaParams &p, const Place &at, int key)
+__device__ __forceinline__ Page page_of(const LaParams &p, const Place &at, const uint32_t asked)
 {
-    const int last = NEAR > 1 ? (at.keys - 1) & ~(NEAR - 1) : at.keys - 1;
-    key = key < last ? key : last;
+    const uint32_t last = NEAR > 1 ? (at.keys - 1) & ~(NEAR - 1) : at.keys - 1;
+    const int key = (int)(asked < last ? asked : last);
     const int block = divide(key, p.of_bs);                // (the block table has it: at.keys is no more than its pages hold)
     const int32_t *const entry = p.bt + (long long)at.b * p.maxblk + block;
     return Page{NEAR > 1 ? constant<int32_t>(entry) : *entry, key - block * p.bs};

@@ -207,7 +207,7 @@ __global__ __launch_bounds__(THREADS) void latent_attention_wide_kernel(const La
                 pf[rg] = *reinterpret_cast<const bf16x8 *>(pool + P_AT + pbuf * P_BYTES + ((kk * 4 + rg) * 64 + l) * 16);
             };
             auto look = [&](const int n) __attribute__((always_inline)) {
-                const int first = key_of_tile(n);
+                const uint32_t first = key_of_tile(n);
                 cut = !sight.whole(first);                 // (uniform)
                 if (cut) {
                     const int row = sight.row0 + 32 * w + (int)(lane() & 31), tok = divide(row < sight.rows ? row : sight.rows - 1, p.of_heads);

@@ -53,6 +53,11 @@ hipError_t cache_slots_launch(const CacheSlotsParams &p, hipStream_t stream);
 
 constexpr int LA_ROWS = 64;               // (token, head) rows of a workgroup
 constexpr int LA_KEYS = 32;               // keys of a tile
+constexpr int LA_MOST_KEYS = 0x7ffffff0;  // of a sequence; the first key of a tile, of those asked for ahead too, is then a 32-bit number without a sign,
+constexpr int LA_AHEAD = 4;               // and no more than this many tiles are asked for ahead
+__host__ __device__ constexpr int la_tiles_of(const int keys) { return (int)(((uint32_t)keys + LA_KEYS - 1) / LA_KEYS); }
+static_assert((uint64_t)LA_KEYS * (uint64_t)(la_tiles_of(LA_MOST_KEYS) + LA_AHEAD) + LA_KEYS < (1ull << 32) && la_tiles_of(LA_MOST_KEYS) == (1 << 26) && la_tiles_of(0) == 0,
+              "no key number wraps");
 constexpr int LA_OPEN = 6;                // what a row tile's beginning and end cost, in tiles
 constexpr int LA_THREADS = 512;          // of a workgroup
 constexpr int LA_WIDE_ROWS = 128, LA_WIDE_THREADS = 256;    // the same of the form for many rows
