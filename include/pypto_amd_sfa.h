@@ -730,8 +730,8 @@ int pto_cache_slots_launch(const PtoCacheSlotsArgs *args, void *hip_stream);
  *   out [total_q, heads, 512] bf16;  lse [total_q, heads] fp32 or NULL: the natural logarithm of the sum of exp of a row's scores
  *
  * Without a mask a token sees the keys up to its own; with a window > 0 of these the last `window` and the first `sinks`.  With a mask it sees
- * the keys before the sequence's query tokens and, of theirs, key j where bit j % 64 of word j / 64 of its mask is set.  Rows that see no key are
- * zeros, their lse -infinity; rows of no sequence stay as they were.  Keys that a row does not see may hold anything, infinite scales too.
+ * the keys before the sequence's query tokens and, of theirs, key j where bit j % 64 of word j / 64 of its mask is set (of fewer keys than query tokens
+ * the first tokens have no key).  Rows that see no key are zeros, their lse -infinity; rows of no sequence stay as they were.  Keys that a row does not see may hold anything, infinite scales too.
  * Positions without a page (an entry below zero, or a page outside the cache) read as zeros, as latents and as rope; keys that the table is too
  * short for do not exist.  Beginnings outside the queries are moved into them; where they do not ascend nothing outside is touched, but what is
  * written is not determined.

@@ -65,8 +65,7 @@ def seen_keys(n, keys, window=None, sinks=0, mask=None):
     """[n, keys] truth values: what the last n of `keys` positions see.  mask: [n, words] int64, bits of the n."""
     at, j = torch.arange(keys - n, keys)[:, None], torch.arange(keys)
     if mask is not None:
-        context = max(keys - n, 0)
-        node = j - context
+        node = j - (keys - n)                      # (of fewer keys than tokens, the first tokens have none)
         word = (node // 64).clamp(0, mask.shape[1] - 1)
         drafted = ((mask.cpu()[:, word] >> (node % 64)) & 1).bool() & (node < 64 * mask.shape[1])
         return torch.where(node < 0, True, drafted)

@@ -282,7 +282,7 @@ template <int ROWS>
 struct Sight {
     const LaParams &p;
     int rows, row0, last, n, keys;                         // of the sequence; the row tile's first row, its last one's number in it
-    int context;                                           // keys before the tree
+    int context;                                           // keys before the tree (below zero: as many of its first nodes have no key)
     int least, most, low_last;                             // keys that all, that some rows see (but for windows); where the last row's window begins
     int sink_tiles, skip, tiles;
 
@@ -291,8 +291,8 @@ struct Sight {
         rows = at.n * p.heads, row0 = at.row_tile * ROWS, n = at.n, keys = at.keys;
         last = rows - 1 - row0 < ROWS - 1 ? rows - 1 - row0 : ROWS - 1;
         const int tok0 = divide(row0, p.of_heads), tok1 = divide(row0 + last, p.of_heads);
-        context = keys - n > 0 ? keys - n : 0;
-        least = p.mask ? context : sees(tok0), most = sees(tok1);
+        context = keys - n;
+        least = !p.mask ? sees(tok0) : (context > 0 ? context : 0), most = sees(tok1);
         const int low = from(sees(tok0)) / KT;
         low_last = from(sees(tok1));
         sink_tiles = (p.sinks + KT - 1) / KT;
@@ -323,7 +323,7 @@ struct Sight {
         };
         const int sinks = p.sinks < s ? p.sinks : s;
         uint32_t bits = (below(s - first) & ~below(from(s) - first)) | below(sinks - first);
-        if (mask && first_key + KT > (uint32_t)context) {                // of the tile's keys, those in front of the tree and those of it that the mask names
+        if (mask && (context < 0 || first_key + KT > (uint32_t)context)) {       // of the tile's keys, those in front of the tree and those of it that the mask names
             const int node = first - context, at_word = node >> 6, shift = node & 63;
             auto word = [&](const int i) { return i < 0 ? ~0ull : (i < p.words ? mask[i] : 0ull); };
             const unsigned long long lo = word(at_word), hi = word(at_word + 1);
