@@ -214,7 +214,7 @@ __global__ __launch_bounds__(PG_THREADS) void cache_pages_kernel(const CachePage
 
 // A workgroup takes the tokens t0 .. t1 - 1, a thread one at a time; the beginnings of up to 1024 sequences are in LDS.  512 single tokens 4.1 us, nine prompts of
 // 200 000 tokens in all 4.1, 48 trees of 17 to 63 nodes 5.5 (a node's ancestors are walked up by its own thread, a tree's parents in LDS): a launch, lengths, sums and
-// a table entry, one behind the other.
+// a table entry, one behind the other.  A chain of 1000 nodes 94 with one mask word and with 16 (a walk for each word: 1450), since the last node's steps are behind one another.
 constexpr int SL_THREADS = 256, SL_SEQS = 1024, SL_NODES = 64 * SLOTS_MAX_WORDS, SL_PER = SL_SEQS / SL_THREADS;
 
 __global__ __launch_bounds__(SL_THREADS) void cache_slots_kernel(const CacheSlotsParams p, const int each)
@@ -295,17 +295,25 @@ __global__ __launch_bounds__(SL_THREADS) void cache_slots_kernel(const CacheSlot
                 p.slots[t] = slot;
                 int depth = r;
                 if (p.parents) {
-                    for (int w = 0; w < p.words; ++w) {
+                    // One walk for all words: a parent comes before its child, so the walk ends, and a word that it has left is whole.
+                    int word = p.words;                    // words from this one on are written
+                    auto zeros_down_to = [&](const int w) {
+                        while (word > w) p.mask[t * p.words + --word] = 0;
+                    };
+                    depth = -1;
+                    for (int node = r; node >= 0;) {
+                        const int low = node & ~63, at = low >> 6;
                         unsigned long long bits = 0;
-                        depth = -1;
-                        for (int node = r; node >= 0;) {   // a parent comes before its child, so this ends
-                            if ((node >> 6) == w) bits |= 1ull << (node & 63);
+                        do {                               // the nodes of a word
+                            bits |= 1ull << (node & 63);
                             ++depth;
                             const int of = first + node, up = of >= staged ? parent[of - staged] : p.parents[of];
                             node = up < node ? up : -1;
-                        }
-                        p.mask[t * p.words + w] = bits;
+                        } while (node >= low);
+                        zeros_down_to(at + 1);
+                        if (at < p.words) p.mask[t * p.words + at] = bits, word = at;
                     }
+                    zeros_down_to(0);
                 }
                 p.positions[t] = (long long)first_row[s] + depth;
             }
