@@ -60,7 +60,8 @@ __device__ __forceinline__ f32x4 acc_read(const f32x16 &acc, const int q4)
     return f32x4{r0, r1, r2, r3};
 }
 // The scores' accumulator stays out of them: products on one destination after the other (no wait states among them), then the wait
-// that a vector instruction's read needs.  Their operands come from LDS, or stay in registers from before the loop (a wait in front of each cost 1 %).
+// that a vector instruction's read needs.  Their operands come from LDS, or stay in registers from before the loop (a wait in front of each cost 1 %):
+// whether the compiler put a copy in front of one anyway is read from its listing by tests/test_product_waits.py.
 __device__ __forceinline__ void s_product_first(f32x16 &s, const bf16x8 a, const bf16x8 b) { asm("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(s) : "v"(a), "v"(b)); }
 __device__ __forceinline__ void s_product(f32x16 &s, const bf16x8 a, const bf16x8 b) { asm("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(s) : "v"(a), "v"(b)); }
 __device__ __forceinline__ void s_done(f32x16 &s) { asm volatile("s_nop 15\n\ts_nop 3" : "+v"(s)); }
