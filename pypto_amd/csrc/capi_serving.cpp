@@ -49,43 +49,74 @@ int latent_check(const PtoLatentAttentionArgs *a)
     return PTO_OK;
 }
 
-struct LatentPlan {
-    int wide, most_tiles, row_tiles, groups, by_tile, entries;
+// A form's launch: how its row tiles may be divided, and the memory for their pieces.
+struct LatentForm {
+    int most_tiles, row_tiles, groups, by_tile, entries;
     size_t o_bytes, ml_bytes, join_bytes;
+    size_t bytes() const { return o_bytes + ml_bytes + join_bytes; }
+};
+struct LatentPlan {
+    bool narrow, wide;
+    LatentForm form[2];                   // of 64 rows, of 128
+    size_t bytes, flag;                   // of the workspace; where the word is that says which form it was
 };
 
 // The device divides the work, since lengths are there.  Here only as many workgroups as there can be pieces of LA_LEAST units, one to a
 // compute unit at most (a workgroup's LDS is most of one's), and memory for two pieces of each.
-// 128 rows to a workgroup take 0.6 of the time that 64 take for as many, but twice the bytes for a piece: for sequences that fill them, and where the keys that
-// the table has room for could keep each compute unit for 28 tiles of 64 rows.  With 128 rows and with 64, us, all of 128 heads: 24 sequences of 25 to 63
-// tokens over 500 to 9000 keys 1340 and 1660; 4 of 30 over 2030 keys 98.6 and 111.3; 2 of 30 (30 tiles) 63.9 and 66.1; single tokens of 32 over 2052 (25 tiles)
-// 50.0 and 47.9; one token over 30000 (11) 44.3 and 34.6.
-LatentPlan latent_plan(const PtoLatentAttentionArgs *a)
+LatentForm latent_form(const PtoLatentAttentionArgs *a, const int rows, const long long cus)
 {
-    LatentPlan pl{};
-    const long long cus = cu_count() > 0 ? cu_count() : 256;
-    auto row_tiles_of = [&](const int rows) { return a->total_q * a->heads / rows + (a->b < a->total_q ? a->b : a->total_q); };         // at most
-    auto tiles_of = [&](const int rows) {
-        const long long all = (a->max_blocknum_perbatch * a->block_size + pto::LA_KEYS - 1) / pto::LA_KEYS;
-        if (a->window == 0) return all;
+    LatentForm f{};
+    const long long row_tiles = a->total_q * a->heads / rows + (a->b < a->total_q ? a->b : a->total_q);          // at most
+    long long tiles = (a->max_blocknum_perbatch * a->block_size + pto::LA_KEYS - 1) / pto::LA_KEYS;
+    if (a->window > 0) {
         // of a row tile's tokens, the window of the first to the last one's last key, and the first keys
         const long long reach = a->window + (rows - 2) / a->heads + 1;
         const long long w = (a->sinks + pto::LA_KEYS - 1) / pto::LA_KEYS + (reach + pto::LA_KEYS - 1) / pto::LA_KEYS + 1;
-        return w < all ? w : all;
-    };
-    pl.wide = a->total_q * a->heads >= 96 * a->b && (double)row_tiles_of(pto::LA_ROWS) * (double)tiles_of(pto::LA_ROWS) >= 28.0 * (double)cus;
-    const int rows = pl.wide ? pto::LA_WIDE_ROWS : pto::LA_ROWS;
-    const long long row_tiles = row_tiles_of(rows), tiles = tiles_of(rows);
-    pl.most_tiles = (int)tiles;
-    pl.row_tiles = (int)row_tiles;
+        tiles = w < tiles ? w : tiles;
+    }
+    f.most_tiles = (int)tiles;
+    f.row_tiles = (int)row_tiles;
     const double pieces = (double)row_tiles * (double)(tiles + pto::LA_OPEN) / pto::LA_LEAST;
     const long long groups = pieces < (double)cus ? (long long)pieces + 1 : cus;
-    pl.groups = (int)((groups + 7) / 8 * 8);
-    pl.by_tile = row_tiles <= pl.groups;
-    pl.entries = (int)(pl.by_tile ? (row_tiles > 0 ? row_tiles : 1) : pl.groups);
-    pl.o_bytes = (size_t)2 * pl.groups * rows * 512 * sizeof(float);
-    pl.ml_bytes = (size_t)2 * pl.groups * rows * 2 * sizeof(float);
-    pl.join_bytes = (size_t)pl.entries * 4 * sizeof(int32_t);
+    f.groups = (int)((groups + 7) / 8 * 8);
+    f.by_tile = row_tiles <= f.groups;
+    f.entries = (int)(f.by_tile ? (row_tiles > 0 ? row_tiles : 1) : f.groups);
+    f.o_bytes = (size_t)2 * f.groups * rows * 512 * sizeof(float);
+    f.ml_bytes = (size_t)2 * f.groups * rows * 2 * sizeof(float);
+    f.join_bytes = (size_t)f.entries * 4 * sizeof(int32_t);
+    return f;
+}
+
+// 128 rows to a workgroup read a tile of keys half as often, for twice the bytes to a piece and a longer beginning.  What that comes to hangs on lengths:
+// on tiles to a compute unit, which 128 rows want many of, or on row tiles so many that few are cut into pieces, and on how much of 128 rows sequences leave empty
+// (no more than an eighth above what they leave of 64).  The table's width says nothing of them: in a captured step it is that of the longest context there
+// can be.  So where its width leaves both open, both forms are launched and the first one finds from the lengths which of them returns at once; that
+// costs 3 to 5 us.  64 rows and 128, us, of 128 heads where not said otherwise:
+//   single tokens: 1 over 500 keys 19.3 and 24.9, over 30000 (7 tiles of 64 rows to a compute unit) 36.5 and 46.7, over 130000 (32) 72 and 76, over 500000 (122)
+//   222 and 197; 32 over 2052 (16) 47 and 54, over 8000 (62) 110 and 109, over 16000 (125) 207 and 190; 128 over 500 (16) 42 and 58, over 2000 (63) 105 and 112
+//   4 of 30 tokens over 200 keys (7) 36 and 42, over 1000 (30) 71.4 and 69.9, over 2030 (60) 114 and 105
+//   many row tiles: 208 single tokens over 60, 300, 1000 keys 32.7, 61.8, 114 and 29.8, 58.7, 118; 256: 35, 59, 121 and 31, 49, 100; 512: 62, 111, 256 and 52, 89, 212;
+//   5 of 40 tokens over 60, 300, 1000 keys 30.5, 56.6, 106 and 27.2, 53.5, 100; 160 single tokens 30.5, 53, 95 and 28, 60, 93
+//   rows that are padded: 150 of 9 tokens of 16 heads over 60 keys 29.4 and 40, over 1000 119 and 135; 16 of 4 tokens, 40 heads, over 20000 183 and 197
+constexpr long long WIDE_TILES = 40;      // of 64 rows, to a compute unit
+long long wide_row_tiles(const long long cus) { return 3 * cus / 2; }
+
+LatentPlan latent_plan(const PtoLatentAttentionArgs *a)
+{
+    LatentPlan pl{};
+    const long long cus = cu_count() > 0 ? cu_count() : 256, rows = a->total_q * a->heads;
+    pl.form[0] = latent_form(a, pto::LA_ROWS, cus);
+    pl.form[1] = latent_form(a, pto::LA_WIDE_ROWS, cus);
+    const bool many = rows >= wide_row_tiles(cus) * pto::LA_ROWS;
+    const bool unpadded = a->heads % pto::LA_WIDE_ROWS == 0 || rows >= 1024 * a->b;
+    pl.wide = rows >= 96 * a->b && (many || (double)rows * (double)pl.form[0].most_tiles >= (double)(WIDE_TILES * cus * pto::LA_ROWS));
+    pl.narrow = !pl.wide || !many || !unpadded;
+    for (int i = 0; i < 2; ++i)
+        if (i ? pl.wide : pl.narrow) pl.bytes = pl.form[i].bytes() > pl.bytes ? pl.form[i].bytes() : pl.bytes;
+    if (pl.narrow && pl.wide) {
+        pl.flag = (pl.bytes + 15) / 16 * 16;
+        pl.bytes = pl.flag + 16;
+    }
     return pl;
 }
 
@@ -162,8 +193,7 @@ int pto_latent_attention_workspace_bytes(const PtoLatentAttentionArgs *a, size_t
     if (!bytes) return fail(PTO_E_INVALID_ARG, "latent_attention: bytes is NULL");
     const int rc = latent_check(a);
     if (rc != PTO_OK) return rc;
-    const LatentPlan pl = latent_plan(a);
-    *bytes = pl.o_bytes + pl.ml_bytes + pl.join_bytes;
+    *bytes = latent_plan(a).bytes;
     return PTO_OK;
 }
 
@@ -187,9 +217,8 @@ int pto_latent_attention_launch(const PtoLatentAttentionArgs *a, void *hip_strea
         return fail(PTO_E_INVALID_ARG, "latent_attention: pointers must be aligned to their element size");
     if (cu_count() <= 0) return fail(PTO_E_NO_DEVICE, "latent_attention: no usable device is current");
     const LatentPlan pl = latent_plan(a);
-    const size_t need = pl.o_bytes + pl.ml_bytes + pl.join_bytes;
-    if (!a->workspace || a->workspace_bytes < need)
-        return fail(PTO_E_WORKSPACE, "latent_attention: workspace of %zu bytes required, %zu given", need, a->workspace ? a->workspace_bytes : (size_t)0);
+    if (!a->workspace || a->workspace_bytes < pl.bytes)
+        return fail(PTO_E_WORKSPACE, "latent_attention: workspace of %zu bytes required, %zu given", pl.bytes, a->workspace ? a->workspace_bytes : (size_t)0);
     if (!aligned(a->workspace, 16)) return fail(PTO_E_INVALID_ARG, "latent_attention: the workspace must be 16-byte aligned");
 
     pto::LaParams p{};
@@ -211,9 +240,6 @@ int pto_latent_attention_launch(const PtoLatentAttentionArgs *a, void *hip_strea
     p.mask = reinterpret_cast<const unsigned long long *>(a->tree_mask);
     p.out = static_cast<uint16_t *>(a->out);
     p.lse = a->lse;
-    p.part_o = static_cast<float *>(a->workspace);
-    p.part_ml = reinterpret_cast<float *>(static_cast<char *>(a->workspace) + pl.o_bytes);
-    p.joins = reinterpret_cast<int32_t *>(static_cast<char *>(a->workspace) + pl.o_bytes + pl.ml_bytes);
     p.total_q = a->total_q;
     p.B = (int)a->b;
     p.maxblk = (int)a->max_blocknum_perbatch;
@@ -223,19 +249,27 @@ int pto_latent_attention_launch(const PtoLatentAttentionArgs *a, void *hip_strea
     p.window = (int)a->window;
     p.sinks = (int)a->sinks;
     p.most_keys = (int)(a->max_blocknum_perbatch * a->block_size);
-    p.most_tiles = pl.most_tiles;
-    const int threads = pl.wide ? pto::LA_WIDE_THREADS : pto::LA_THREADS;
-    p.wide = pl.wide;
-    p.per_entry = (int)((a->b + threads - 1) / threads);
-    p.seq_entries = (int)((a->b + p.per_entry - 1) / p.per_entry);
-    p.groups = pl.groups;
-    p.most_row_tiles = pl.row_tiles;
-    p.by_tile = pl.by_tile;
-    p.entries = pl.entries;
     p.of_heads = pto::divisor_of((uint32_t)a->heads);
     p.of_bs = pto::divisor_of((uint32_t)a->block_size);
     p.scale_log2 = a->softmax_scale * 1.4426950408889634f;
-    const hipError_t e = pto::latent_attention_launch(p, static_cast<hipStream_t>(hip_stream));
+    char *const ws = static_cast<char *>(a->workspace);
+    if (pl.narrow && pl.wide) p.form = reinterpret_cast<int32_t *>(ws + pl.flag), p.wide_tiles = WIDE_TILES * cu_count(), p.wide_row_tiles = wide_row_tiles(cu_count());
+    pto::LaParams of[2] = {p, p};
+    for (int i = 0; i < 2; ++i) {
+        const LatentForm &f = pl.form[i];
+        const int threads = i ? pto::LA_WIDE_THREADS : pto::LA_THREADS;
+        of[i].part_o = reinterpret_cast<float *>(ws);
+        of[i].part_ml = reinterpret_cast<float *>(ws + f.o_bytes);
+        of[i].joins = reinterpret_cast<int32_t *>(ws + f.o_bytes + f.ml_bytes);
+        of[i].most_tiles = f.most_tiles;
+        of[i].per_entry = (int)((a->b + threads - 1) / threads);
+        of[i].seq_entries = (int)((a->b + of[i].per_entry - 1) / of[i].per_entry);
+        of[i].groups = f.groups;
+        of[i].most_row_tiles = f.row_tiles;
+        of[i].by_tile = f.by_tile;
+        of[i].entries = f.entries;
+    }
+    const hipError_t e = pto::latent_attention_launch(pl.narrow ? &of[0] : nullptr, pl.wide ? &of[1] : nullptr, static_cast<hipStream_t>(hip_stream));
     if (e != hipSuccess) return fail(PTO_E_LAUNCH, "latent_attention: launch failed: %s", hipGetErrorString(e));
     return PTO_OK;
 }

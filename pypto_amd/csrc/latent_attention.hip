@@ -14,7 +14,8 @@
 // Division of the work.  A row tile takes as many units as it has key tiles and LA_OPEN more for its beginning and end; all units lie in one line,
 // which the workgroups divide evenly, an XCD's neighbouring pieces to neighbouring workgroups.  A boundary near a row tile's edge moves there.
 // Where one falls inside, both sides write their sums, maxima and 512 sums of products, in fp32, and a second launch joins them: two pieces at most
-// to a workgroup, so the memory for them does not depend on lengths, which the host does not know.
+// to a workgroup, so the memory for them does not depend on lengths, which the host does not know.  Where lengths decide between this form and that of 128 rows
+// (latent_plan has the rule), both are launched; this one, the first, counts both's tiles, and returns if the call is the other's, or the other does.
 //
 // Bound, once it runs, by LDS: of a tile of 32 keys each of the eight waves reads half for its scores and an eighth of the values for all rows, and the tile is written,
 // 250 KB or 2000 of the 3000 clocks (1.45 us) that it takes; by a beginning of 9 us (sums over the sequences 2.2, its place in the line 1.1, requests 1.5, their
@@ -420,21 +421,28 @@ __global__ __launch_bounds__(THREADS) void latent_attention_kernel(const LaParam
     line.done();
 }
 
+struct JoinMemory {
+    f32x4 sums[3][4][64];
+    float stats[3][2][32];
+};
+
 // The pieces of row tiles that workgroups share: out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i, in the order of the keys.  A workgroup
-// joins one accumulator block (32 rows, 32 channels, as the attention kernels' registers have them) of an entry's rows, four 16-byte values to a
+// joins one accumulator block at a time (32 rows, 32 channels, as the attention kernels' registers have them) of an entry's rows, four 16-byte values to a
 // lane, its four waves a quarter of the pieces each.
 template <bool WIDE>
-__global__ __launch_bounds__(256) void latent_join_kernel(const LaParams p)
+__device__ __forceinline__ void join_block(const LaParams &p, JoinMemory &mem)
 {
     constexpr int TILE_ROWS = WIDE ? LA_WIDE_ROWS : LA_ROWS, BLOCKS = TILE_ROWS / 2, OF_WAVE = WIDE ? 16 : 4;
-    __shared__ f32x4 sums[3][4][64];
-    __shared__ float stats[3][2][32];
+    const int block = blockIdx.x;
+    if (block >= p.entries * BLOCKS) return;
+    auto &sums = mem.sums;
+    auto &stats = mem.stats;
     const int l = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = l >> 5, col = l & 31;
-    const int32_t *const join = p.joins + 4 * (blockIdx.x / BLOCKS);
+    const int32_t *const join = p.joins + 4 * (block / BLOCKS);
     const int n = join[1];
     if (n <= 1) return;
     const int first = join[0], row0 = join[2], rows = join[3];
-    const int w = (blockIdx.x % BLOCKS) / OF_WAVE, i = blockIdx.x % OF_WAVE;
+    const int w = (block % BLOCKS) / OF_WAVE, i = block % OF_WAVE;
     const int group = WIDE ? i >> 2 : i >> 1, c = WIDE ? i & 3 : i & 1;            // of 32 rows; of 32 of the wave's channels
     // where the pieces are: that of the first workgroup is said; the others' ranges begin inside the row tile, so it is their first
     auto place = [&](const int k) { return (long long)(k == 0 ? first : 2 * ((first >> 1) + k)); };
@@ -495,21 +503,41 @@ __global__ __launch_bounds__(256) void latent_join_kernel(const LaParams p)
     }
 }
 
+template <bool WIDE>
+__global__ __launch_bounds__(256) void latent_join_kernel(const LaParams p)
+{
+    __shared__ JoinMemory mem;
+    join_block<WIDE>(p, mem);
+}
+// (five waves to a SIMD as in the other: four, with as many registers as both need, took 28 us instead of 22 for 8 trees of 30 nodes, 128 heads)
+__global__ __launch_bounds__(256, 5) void latent_join_either_kernel(const LaParams narrow, const LaParams wide)
+{
+    __shared__ JoinMemory mem;
+    if (constant(narrow.form) != 0) join_block<true>(wide, mem);
+    else join_block<false>(narrow, mem);
+}
+
 }  // namespace
 
-hipError_t latent_attention_launch(const LaParams &p, hipStream_t stream)
+hipError_t latent_attention_launch(const LaParams *narrow, const LaParams *wide, hipStream_t stream)
 {
-    if (p.wide) {
-        const hipError_t e = latent_attention_wide_launch(p, stream);
+    hipError_t e = hipSuccess;
+    if (narrow) {
+        if (narrow->bs % 4 == 0 && narrow->cache.rows % 4 == 0)
+            hipLaunchKernelGGL((latent_attention_kernel<true>), dim3((unsigned)narrow->groups), dim3(THREADS), 0, stream, *narrow);
+        else
+            hipLaunchKernelGGL((latent_attention_kernel<false>), dim3((unsigned)narrow->groups), dim3(THREADS), 0, stream, *narrow);
+        e = hipGetLastError();
         if (e != hipSuccess) return e;
-        hipLaunchKernelGGL((latent_join_kernel<true>), dim3((unsigned)p.entries * (LA_WIDE_ROWS / 2)), dim3(256), 0, stream, p);
-        return hipGetLastError();
     }
-    if (p.bs % 4 == 0 && p.cache.rows % 4 == 0) hipLaunchKernelGGL((latent_attention_kernel<true>), dim3((unsigned)p.groups), dim3(THREADS), 0, stream, p);
-    else hipLaunchKernelGGL((latent_attention_kernel<false>), dim3((unsigned)p.groups), dim3(THREADS), 0, stream, p);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((latent_join_kernel<false>), dim3((unsigned)p.entries * (LA_ROWS / 2)), dim3(256), 0, stream, p);
+    if (wide) {
+        e = latent_attention_wide_launch(*wide, stream);
+        if (e != hipSuccess) return e;
+    }
+    const unsigned narrow_blocks = narrow ? (unsigned)narrow->entries * (LA_ROWS / 2) : 0, wide_blocks = wide ? (unsigned)wide->entries * (LA_WIDE_ROWS / 2) : 0;
+    if (!wide) hipLaunchKernelGGL((latent_join_kernel<false>), dim3(narrow_blocks), dim3(256), 0, stream, *narrow);
+    else if (!narrow) hipLaunchKernelGGL((latent_join_kernel<true>), dim3(wide_blocks), dim3(256), 0, stream, *wide);
+    else hipLaunchKernelGGL(latent_join_either_kernel, dim3(narrow_blocks > wide_blocks ? narrow_blocks : wide_blocks), dim3(256), 0, stream, *narrow, *wide);
     return hipGetLastError();
 }
 

@@ -135,7 +135,7 @@ __device__ __forceinline__ int moved(const int x, const int len) { return x <= N
 template <int THREADS>
 struct LineTable {
     long long upto[THREADS], of_waves[THREADS / 64];
-    long long tiles_of_waves[THREADS / 64];
+    long long tiles_of_waves[THREADS / 64], wide_of_waves[THREADS / 64];
     int tiles_upto[THREADS];
     int q0[THREADS], n[THREADS], keys[THREADS];            // of an entry's first sequence
     long long units, share, end, next;                     // end: of this workgroup's part; next: the unit behind the row tile's part in hand
@@ -158,18 +158,21 @@ struct Line {
     __device__ __forceinline__ bool begin() const
     {
         const int tid = threadIdx.x, w = tid >> 6;
-        long long mine = 0, tiles = 0;
+        const bool choose = ROWS == LA_ROWS && p.form;     // (uniform)
+        long long mine = 0, tiles = 0, wide = 0;           // wide: tiles, if rows came by LA_WIDE_ROWS
         for (int j = 0; j < p.per_entry; ++j) {
             const int b = tid * p.per_entry + j;
             if (b < p.B) {
                 const Sequence c = sequence<ROWS>(p, b);
                 if (j == 0) t.q0[tid] = c.q0, t.n[tid] = c.n, t.keys[tid] = c.keys;
                 mine += (long long)c.row_tiles * (c.tiles + LA_OPEN), tiles += c.row_tiles;
+                if (choose) wide += (long long)((c.n * p.heads + LA_WIDE_ROWS - 1) / LA_WIDE_ROWS) * c.tiles;
             }
         }
         mine = wave_sums(mine);
         tiles = wave_sums(tiles);
-        if ((tid & 63) == 63) t.of_waves[w] = mine, t.tiles_of_waves[w] = tiles;
+        if (choose) wide = wave_sums(wide);
+        if ((tid & 63) == 63) t.of_waves[w] = mine, t.tiles_of_waves[w] = tiles, t.wide_of_waves[w] = wide;
         __syncthreads();
         for (int i = 0; i < w; ++i) mine += t.of_waves[i], tiles += t.tiles_of_waves[i];
         t.upto[tid] = mine;
@@ -178,6 +181,14 @@ struct Line {
         // (sequences that overlap, of beginnings that do not ascend, may be more than there are rows and joins for: then nothing is done)
         const int all_tiles = one(t.tiles_upto[THREADS - 1]);
         const long long units = all_tiles < 0 ? 0 : first_of(t.upto[THREADS - 1]);
+        if (choose) {                                      // is the call the other form's?  (see latent_plan)
+            const long long here = units - (long long)LA_OPEN * all_tiles;
+            wide = 0;
+            for (int i = 0; i < THREADS / 64; ++i) wide += first_of(t.wide_of_waves[i]);
+            const bool leave = (here >= p.wide_tiles || all_tiles >= p.wide_row_tiles) && 16 * wide <= 9 * here;
+            if (blockIdx.x == 0 && tid == 0) *p.form = leave;
+            if (leave) return false;
+        }
         // workgroups that take part, so that none gets less than LA_LEAST units
         const int pieces = units < (long long)p.groups * LA_LEAST ? (int)units / LA_LEAST : p.groups, groups = pieces > 0 ? pieces : 1;
         const int per_xcd = (groups + 7) / 8, slot = blockIdx.x >> 3, g = (int)(blockIdx.x & 7) * per_xcd + slot;

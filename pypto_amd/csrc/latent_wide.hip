@@ -79,6 +79,7 @@ __global__ __launch_bounds__(THREADS) void latent_attention_wide_kernel(const La
     const uint32_t pool_lds = (uint32_t)(uintptr_t)(lds_byte_t *)pool;
 
     __shared__ LineTable<THREADS> table;
+    if (p.form && constant(p.form) == 0) return;           // (the other form had the call)
     const Line<ROWS, THREADS> line(p, table);
     if (!line.begin()) return;
     Place at;

@@ -82,14 +82,16 @@ struct LaParams {
     int window, sinks;                    // window 0: all keys
     int most_keys, most_tiles;            // of a sequence, as the block table and the window have it
     int per_entry, seq_entries;           // sequences that a workgroup's thread counts; threads that count any
-    int wide;                             // row tiles of LA_WIDE_ROWS
+    int32_t *form;                        // [1]: whether the form of LA_WIDE_ROWS takes the call, which that of LA_ROWS says; null: the host did
+    long long wide_tiles, wide_row_tiles; // ... from this many tiles or row tiles of LA_ROWS on
     int groups;                           // workgroups, a multiple of eight
     int most_row_tiles;                   // of sequences that do not overlap
     int by_tile, entries;                 // joins by row tile (of all sequences), else by workgroup; how many there are
     Divisor of_heads, of_bs;
     float scale_log2;
 };
-hipError_t latent_attention_launch(const LaParams &p, hipStream_t stream);
+// by rows of LA_ROWS, of LA_WIDE_ROWS, or, both given, as the first finds right
+hipError_t latent_attention_launch(const LaParams *narrow, const LaParams *wide, hipStream_t stream);
 hipError_t latent_attention_wide_launch(const LaParams &p, hipStream_t stream);      // without the joining launch
 
 }  // namespace pto
