@@ -80,21 +80,21 @@ int cache_of(const char *op, const void *nope, const void *rope, const void *sca
     return PTO_OK;
 }
 
-int attention_check(const PtoPromptAttentionArgs *a)
+int attention_check(const char *op, const PtoPromptAttentionArgs *a)
 {
-    if (!a) return fail(PTO_E_INVALID_ARG, "prompt_attention: args is NULL");
+    if (!a) return fail(PTO_E_INVALID_ARG, "%s: args is NULL", op);
     if (a->b < 1 || a->b > (1ll << 24) || a->total_q < 0 || a->total_q > MOST_TOKENS || a->total_k < 0 || a->total_k > MOST_TOKENS)
-        return fail(PTO_E_INVALID_ARG, "prompt_attention: b, total_q or total_k out of range");
+        return fail(PTO_E_INVALID_ARG, "%s: b, total_q or total_k out of range", op);
     if (a->kv_heads < 1 || a->heads < 1 || a->heads > 65536 || a->heads % a->kv_heads != 0)
-        return fail(PTO_E_INVALID_ARG, "prompt_attention: heads must be a multiple of kv_heads, up to 65536 (got %lld and %lld)", (long long)a->heads,
+        return fail(PTO_E_INVALID_ARG, "%s: heads must be a multiple of kv_heads, up to 65536 (got %lld and %lld)", op, (long long)a->heads,
                     (long long)a->kv_heads);
     if (a->total_q * (a->heads / a->kv_heads) > 0x7fff0000ll)
-        return fail(PTO_E_INVALID_ARG, "prompt_attention: total_q x heads of a group out of range");
-    if (a->d != 64 && a->d != 128) return fail(PTO_E_INVALID_ARG, "prompt_attention: d must be 64 or 128 (got %lld)", (long long)a->d);
-    if (!a->query_rope != !a->key_rope) return fail(PTO_E_INVALID_ARG, "prompt_attention: query_rope and key_rope come together");
-    if (a->query_rope && a->d != 128) return fail(PTO_E_INVALID_ARG, "prompt_attention: rope parts go with d = 128");
+        return fail(PTO_E_INVALID_ARG, "%s: total_q x heads of a group out of range", op);
+    if (a->d != 64 && a->d != 128) return fail(PTO_E_INVALID_ARG, "%s: d must be 64 or 128 (got %lld)", op, (long long)a->d);
+    if (!a->query_rope != !a->key_rope) return fail(PTO_E_INVALID_ARG, "%s: query_rope and key_rope come together", op);
+    if (a->query_rope && a->d != 128) return fail(PTO_E_INVALID_ARG, "%s: rope parts go with d = 128", op);
     if (!std::isfinite(a->softmax_scale) || !std::isfinite(a->softmax_scale * 1.4426950408889634f))
-        return fail(PTO_E_INVALID_ARG, "prompt_attention: softmax_scale is not finite");
+        return fail(PTO_E_INVALID_ARG, "%s: softmax_scale is not finite", op);
     return PTO_OK;
 }
 
@@ -188,28 +188,28 @@ PromptPlan attention_plan(const PtoPromptAttentionArgs *a, const int64_t window,
     return pl;
 }
 
-int attention_launch(const PtoPromptAttentionArgs *a, const int64_t window, const int64_t sinks, void *hip_stream)
+int attention_launch(const char *op, const PtoPromptAttentionArgs *a, const int64_t window, const int64_t sinks, void *hip_stream)
 {
     if (a->total_q == 0) return PTO_OK;
     if (!a->query || !a->out || !a->cu_seqlens_q || !a->cu_seqlens_k || (a->total_k > 0 && (!a->key || !a->value)))
-        return fail(PTO_E_INVALID_ARG, "prompt_attention: a tensor pointer is NULL");
+        return fail(PTO_E_INVALID_ARG, "%s: a tensor pointer is NULL", op);
     if (!aligned(a->key, 16) || !aligned(a->value, 16) || !aligned(a->key_rope, 16) || a->key_stride_t % 8 != 0 || a->key_stride_h % 8 != 0 ||
         a->value_stride_t % 8 != 0 || a->value_stride_h % 8 != 0 || a->key_rope_stride_t % 8 != 0 || a->key_rope_stride_h % 8 != 0)
-        return fail(PTO_E_INVALID_ARG, "prompt_attention: keys and values must be 16-byte aligned, their strides multiples of 8 elements");
+        return fail(PTO_E_INVALID_ARG, "%s: keys and values must be 16-byte aligned, their strides multiples of 8 elements", op);
     if (!aligned(a->query, 2) || !aligned(a->query_rope, 2) || !aligned(a->out, 2) || !aligned(a->lse, 4) || !aligned(a->cu_seqlens_q, 4) ||
         !aligned(a->cu_seqlens_k, 4))
-        return fail(PTO_E_INVALID_ARG, "prompt_attention: pointers must be aligned to their element size");
+        return fail(PTO_E_INVALID_ARG, "%s: pointers must be aligned to their element size", op);
     constexpr int64_t most = (1ll << 32) / (2 * pto::PA_KEYS) - 256;
     if (a->key_stride_t < 0 || a->key_stride_t > most || a->value_stride_t < 0 || a->value_stride_t > most || a->key_rope_stride_t < 0 || a->key_rope_stride_t > most)
-        return fail(PTO_E_INVALID_ARG, "prompt_attention: key and value token strides must be in [0, %lld]", (long long)most);
-    if (cu_count() <= 0) return fail(PTO_E_NO_DEVICE, "prompt_attention: no usable device is current");
+        return fail(PTO_E_INVALID_ARG, "%s: key and value token strides must be in [0, %lld]", op, (long long)most);
+    if (cu_count() <= 0) return fail(PTO_E_NO_DEVICE, "%s: no usable device is current", op);
     const PromptPlan pl = attention_plan(a, window, sinks);
     const size_t need = pl.o_bytes + pl.ml_bytes;
     if (need > 0 && (!a->workspace || a->workspace_bytes < need))
-        return fail(PTO_E_WORKSPACE, "prompt_attention: workspace of %zu bytes required, %zu given", need, a->workspace ? a->workspace_bytes : (size_t)0);
-    if (!aligned(a->workspace, 16)) return fail(PTO_E_INVALID_ARG, "prompt_attention: the workspace must be 16-byte aligned");
+        return fail(PTO_E_WORKSPACE, "%s: workspace of %zu bytes required, %zu given", op, need, a->workspace ? a->workspace_bytes : (size_t)0);
+    if (!aligned(a->workspace, 16)) return fail(PTO_E_INVALID_ARG, "%s: the workspace must be 16-byte aligned", op);
     if (pl.workgroups > 0x7ffffff0ll)
-        return fail(PTO_E_INVALID_ARG, "prompt_attention: the call exceeds the largest launch");
+        return fail(PTO_E_INVALID_ARG, "%s: the call exceeds the largest launch", op);
 
     pto::PaParams p{};
     p.q = static_cast<const uint16_t *>(a->query);
@@ -249,7 +249,7 @@ int attention_launch(const PtoPromptAttentionArgs *a, const int64_t window, cons
     p.cus = cu_count();
     p.scale_log2 = a->softmax_scale * 1.4426950408889634f;
     const hipError_t e = pto::prompt_attention_launch(p, static_cast<hipStream_t>(hip_stream));
-    if (e != hipSuccess) return fail(PTO_E_LAUNCH, "prompt_attention: launch failed: %s", hipGetErrorString(e));
+    if (e != hipSuccess) return fail(PTO_E_LAUNCH, "%s: launch failed: %s", op, hipGetErrorString(e));
     return PTO_OK;
 }
 
@@ -259,7 +259,7 @@ int window_check(const PtoPromptWindowArgs *a)
     if (a->window < 1 || a->window > MOST_TOKENS || a->sinks < 0 || a->sinks > MOST_TOKENS)
         return fail(PTO_E_INVALID_ARG, "prompt_window_attention: window must be in [1, 2^30], sinks in [0, 2^30]");
     if (!a->prompt.causal) return fail(PTO_E_INVALID_ARG, "prompt_window_attention: a window is causal");
-    return attention_check(&a->prompt);
+    return attention_check("prompt_window_attention", &a->prompt);
 }
 
 }  // namespace
@@ -382,7 +382,7 @@ int pto_cache_read_launch(const PtoCacheReadArgs *a, void *hip_stream)
 int pto_prompt_attention_workspace_bytes(const PtoPromptAttentionArgs *a, size_t *bytes)
 {
     if (!bytes) return fail(PTO_E_INVALID_ARG, "prompt_attention: bytes is NULL");
-    const int rc = attention_check(a);
+    const int rc = attention_check("prompt_attention", a);
     if (rc != PTO_OK) return rc;
     const PromptPlan pl = attention_plan(a, 0, 0);
     *bytes = pl.o_bytes + pl.ml_bytes;
@@ -392,7 +392,7 @@ int pto_prompt_attention_workspace_bytes(const PtoPromptAttentionArgs *a, size_t
 int pto_prompt_attention_plan(const PtoPromptAttentionArgs *a, PtoPromptPlan *plan)
 {
     if (!plan) return fail(PTO_E_INVALID_ARG, "prompt_attention: plan is NULL");
-    const int rc = attention_check(a);
+    const int rc = attention_check("prompt_attention", a);
     if (rc != PTO_OK) return rc;
     const PromptPlan pl = attention_plan(a, 0, 0);
     plan->rows_per_workgroup = pl.waves * pto::PA_WAVE_ROWS;
@@ -404,8 +404,8 @@ int pto_prompt_attention_plan(const PtoPromptAttentionArgs *a, PtoPromptPlan *pl
 
 int pto_prompt_attention_launch(const PtoPromptAttentionArgs *a, void *hip_stream)
 {
-    const int rc = attention_check(a);
-    return rc != PTO_OK ? rc : attention_launch(a, 0, 0, hip_stream);
+    const int rc = attention_check("prompt_attention", a);
+    return rc != PTO_OK ? rc : attention_launch("prompt_attention", a, 0, 0, hip_stream);
 }
 
 int pto_prompt_window_workspace_bytes(const PtoPromptWindowArgs *a, size_t *bytes)
@@ -421,7 +421,7 @@ int pto_prompt_window_workspace_bytes(const PtoPromptWindowArgs *a, size_t *byte
 int pto_prompt_window_launch(const PtoPromptWindowArgs *a, void *hip_stream)
 {
     const int rc = window_check(a);
-    return rc != PTO_OK ? rc : attention_launch(&a->prompt, a->window, a->sinks, hip_stream);
+    return rc != PTO_OK ? rc : attention_launch("prompt_window_attention", &a->prompt, a->window, a->sinks, hip_stream);
 }
 
 }  // extern "C"
