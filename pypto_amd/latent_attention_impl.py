@@ -32,7 +32,7 @@ from .sparse_flash_attention_quant_impl import KV_LORA_RANK, ROPE_DIM
 def _attend(op, query_nope, query_rope, parts, names, block_table, cu_seqlens_q, seq_lens, attention_out, softmax_scale, block_size, window, sinks,
             tree_mask, softmax_lse):
     C = _native.load()
-    check_window(window, sinks)
+    window, sinks = check_window(window, sinks)
     pad = list(parts) + [None] * (3 - len(parts))
     if C.latent_attention_call(query_nope, query_rope, *pad, block_table, cu_seqlens_q, seq_lens, attention_out, softmax_scale, block_size, window or 0, sinks,
                                tree_mask, softmax_lse):

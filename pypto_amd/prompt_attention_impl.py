@@ -14,6 +14,7 @@ output): the last dimension alone has to be contiguous.
 from __future__ import annotations
 
 import math
+from numbers import Integral
 
 import torch
 
@@ -120,7 +121,7 @@ def prompt_window_attention(query, key, value, cu_seqlens_q, cu_seqlens_k, atten
     C = _native.load()
     if window is None:
         raise ValueError("window: expected a whole number from 1 to 2^30, got None")
-    check_window(window, sinks)
+    window, sinks = check_window(window, sinks)
     if C.prompt_window_call(query, key, value, cu_seqlens_q, cu_seqlens_k, attention_out, softmax_scale, query_rope, key_rope, softmax_lse, window, sinks):
         return None
     args = _checked("prompt_window_attention", query, key, value, cu_seqlens_q, cu_seqlens_k, attention_out, softmax_scale, query_rope, key_rope, softmax_lse)
@@ -130,9 +131,11 @@ def prompt_window_attention(query, key, value, cu_seqlens_q, cu_seqlens_k, atten
 
 
 def check_window(window, sinks):
-    if window is not None and (not isinstance(window, int) or isinstance(window, bool) or not 1 <= window <= 1 << 30):
+    """Both as Python's own whole numbers (window None: none)."""
+    if window is not None and (not isinstance(window, Integral) or isinstance(window, bool) or not 1 <= window <= 1 << 30):
         raise ValueError(f"window: expected a whole number from 1 to 2^30, got {window!r}")
-    if not isinstance(sinks, int) or isinstance(sinks, bool) or not 0 <= sinks <= 1 << 30:
+    if not isinstance(sinks, Integral) or isinstance(sinks, bool) or not 0 <= sinks <= 1 << 30:
         raise ValueError(f"sinks: expected a whole number from 0 to 2^30, got {sinks!r}")
     if sinks and window is None:
         raise ValueError("sinks go with a window")
+    return None if window is None else int(window), int(sinks)
