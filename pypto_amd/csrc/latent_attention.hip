@@ -54,8 +54,8 @@ __device__ __forceinline__ float quarters_sum(const float x)
     return lo + hi;
 }
 
-// QUADS: pages and the cache hold whole fours of rows.
-template <bool QUADS>
+// QUADS: pages and the cache hold whole fours of rows.  CHOOSE: the form of 128 rows is launched behind this one, and p.form says whose call it is.
+template <bool QUADS, bool CHOOSE>
 __global__ __launch_bounds__(THREADS) void latent_attention_kernel(const LaParams p)
 {
     __shared__ __attribute__((aligned(16))) uint8_t pool[POOL];
@@ -67,7 +67,7 @@ __global__ __launch_bounds__(THREADS) void latent_attention_kernel(const LaParam
     const uint32_t pool_lds = (uint32_t)(uintptr_t)(lds_byte_t *)pool;
 
     __shared__ LineTable<THREADS> table;
-    const Line<LA_ROWS, THREADS> line(p, table);
+    const Line<LA_ROWS, THREADS, CHOOSE> line(p, table);
     if (!line.begin()) return;
     Place at;
     int i_begin, i_end;
@@ -523,10 +523,10 @@ hipError_t latent_attention_launch(const LaParams *narrow, const LaParams *wide,
 {
     hipError_t e = hipSuccess;
     if (narrow) {
-        if (narrow->bs % 4 == 0 && narrow->cache.rows % 4 == 0)
-            hipLaunchKernelGGL((latent_attention_kernel<true>), dim3((unsigned)narrow->groups), dim3(THREADS), 0, stream, *narrow);
-        else
-            hipLaunchKernelGGL((latent_attention_kernel<false>), dim3((unsigned)narrow->groups), dim3(THREADS), 0, stream, *narrow);
+        const bool quads = narrow->bs % 4 == 0 && narrow->cache.rows % 4 == 0;
+        const auto kernel = wide ? (quads ? latent_attention_kernel<true, true> : latent_attention_kernel<false, true>)
+                                 : (quads ? latent_attention_kernel<true, false> : latent_attention_kernel<false, false>);
+        hipLaunchKernelGGL(kernel, dim3((unsigned)narrow->groups), dim3(THREADS), 0, stream, *narrow);
         e = hipGetLastError();
         if (e != hipSuccess) return e;
     }

@@ -144,8 +144,8 @@ struct LineTable {
     int fresh, whole, piece;                               // whole: no other workgroup has a part of it; its piece's place
 };
 
-// The line of all units, and this workgroup's part of it.
-template <int ROWS, int THREADS>
+// The line of all units, and this workgroup's part of it.  CHOOSE: the call may be that of the other form, of LA_WIDE_ROWS.
+template <int ROWS, int THREADS, bool CHOOSE>
 struct Line {
     const LaParams &p;
     LineTable<THREADS> &t;
@@ -158,7 +158,6 @@ struct Line {
     __device__ __forceinline__ bool begin() const
     {
         const int tid = threadIdx.x, w = tid >> 6;
-        const bool choose = ROWS == LA_ROWS && p.form;     // (uniform)
         long long mine = 0, tiles = 0, wide = 0;           // wide: tiles, if rows came by LA_WIDE_ROWS
         for (int j = 0; j < p.per_entry; ++j) {
             const int b = tid * p.per_entry + j;
@@ -166,13 +165,16 @@ struct Line {
                 const Sequence c = sequence<ROWS>(p, b);
                 if (j == 0) t.q0[tid] = c.q0, t.n[tid] = c.n, t.keys[tid] = c.keys;
                 mine += (long long)c.row_tiles * (c.tiles + LA_OPEN), tiles += c.row_tiles;
-                if (choose) wide += (long long)((c.n * p.heads + LA_WIDE_ROWS - 1) / LA_WIDE_ROWS) * c.tiles;
+                if (CHOOSE) wide += (long long)((c.n * p.heads + LA_WIDE_ROWS - 1) / LA_WIDE_ROWS) * c.tiles;
             }
         }
         mine = wave_sums(mine);
         tiles = wave_sums(tiles);
-        if (choose) wide = wave_sums(wide);
-        if ((tid & 63) == 63) t.of_waves[w] = mine, t.tiles_of_waves[w] = tiles, t.wide_of_waves[w] = wide;
+        if (CHOOSE) wide = wave_sums(wide);
+        if ((tid & 63) == 63) {
+            t.of_waves[w] = mine, t.tiles_of_waves[w] = tiles;
+            if (CHOOSE) t.wide_of_waves[w] = wide;
+        }
         __syncthreads();
         for (int i = 0; i < w; ++i) mine += t.of_waves[i], tiles += t.tiles_of_waves[i];
         t.upto[tid] = mine;
@@ -181,7 +183,7 @@ struct Line {
         // (sequences that overlap, of beginnings that do not ascend, may be more than there are rows and joins for: then nothing is done)
         const int all_tiles = one(t.tiles_upto[THREADS - 1]);
         const long long units = all_tiles < 0 ? 0 : first_of(t.upto[THREADS - 1]);
-        if (choose) {                                      // is the call the other form's?  (see latent_plan)
+        if (CHOOSE) {                                      // is the call the other form's?  (see latent_plan)
             const long long here = units - (long long)LA_OPEN * all_tiles;
             wide = 0;
             for (int i = 0; i < THREADS / 64; ++i) wide += first_of(t.wide_of_waves[i]);

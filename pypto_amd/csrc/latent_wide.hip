@@ -80,7 +80,7 @@ __global__ __launch_bounds__(THREADS) void latent_attention_wide_kernel(const La
 
     __shared__ LineTable<THREADS> table;
     if (p.form && constant(p.form) == 0) return;           // (the other form had the call)
-    const Line<ROWS, THREADS> line(p, table);
+    const Line<ROWS, THREADS, false> line(p, table);
     if (!line.begin()) return;
     Place at;
     int i_begin, i_end;
