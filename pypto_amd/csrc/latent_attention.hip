@@ -17,11 +17,13 @@
 // to a workgroup, so the memory for them does not depend on lengths, which the host does not know.  Where lengths decide between this form and that of 128 rows
 // (latent_plan has the rule), both are launched; this one, the first, counts both's tiles, and returns if the call is the other's, or the other does.
 //
-// Bound, once it runs, by LDS: of a tile of 32 keys each of the eight waves reads half for its scores and an eighth of the values for all rows, and the tile is written,
-// 250 KB or 2000 of the 3000 clocks (1.45 us) that it takes; by a beginning of 9 us (sums over the sequences 2.2, its place in the line 1.1, requests 1.5, their
-// way 0.5, the first tile 3.3) and an end of 1.2 where pieces are short; and by the second launch, which reads what the first wrote.  Single tokens of 32
-// sequences over 2052 keys, 128 heads: 47.7 us, 18 GFLOP of products, 33 MB of pieces; 1 to 4 tokens of 90 sequences over 1016 keys, 16 heads: 41.6; a tree of 8 tokens
-// over 2900 keys, 16 heads: 21.6; one token with 128 heads over 30000 keys: 34.  On the way (the first of these): a look-up and a 64-bit address for each row 59, one of
+// No unit is busy half of the time.  Of a workgroup's time (single tokens of 32 sequences over 2052 keys, 128 heads; counters) vector instructions take 39 %, LDS 30,
+// scalar instructions 25, products 23, and its waves wait for 38 % of theirs.  A tile takes 3000 clocks (1.45 us); the selected keys' attention of 64 heads, with the same
+// products and LDS traffic, 2580, at 42, 40, 10, 30 and 41 %: it has pages in LDS before its loop, where this one makes a look-up, a division and addresses for each tile, 2.3
+// times as many scalar instructions in all, which is the likely difference.  Beside the tiles a beginning of 9 us (sums over the sequences 2.2, its place in the line 1.1, requests
+// 1.5, their way 0.5, the first tile 3.3) and an end of 1.2, where pieces are short most of the time; and the second launch, which reads what the first wrote.
+// The example 46.5 to 50 us, 17 GFLOP of products, 33 MB of pieces; 1 to 4 tokens of 90 sequences over 1016 keys, 16 heads: 42; a tree of 8 tokens over 2900 keys, 16
+// heads: 22; one token with 128 heads over 30000 keys: 37.  On the way (the first of these): a look-up and a 64-bit address for each row 59, one of
 // either for four neighbouring rows, pages asked for before rows, 51, boundaries moved to row tiles' edges for pieces of one tile instead of three 47.7.
 #include "latent_line.h"
 

@@ -61,8 +61,8 @@ static_assert((uint64_t)LA_KEYS * (uint64_t)(la_tiles_of(LA_MOST_KEYS) + LA_AHEA
 constexpr int LA_OPEN = 6;                // what a row tile's beginning and end cost, in tiles
 constexpr int LA_THREADS = 512;          // of a workgroup
 constexpr int LA_WIDE_ROWS = 128, LA_WIDE_THREADS = 256;    // the same of the form for many rows
-// Units of the shortest piece that the line is divided into: of 4 rather than 6, one token with 128 heads over 500 keys takes 20.6 us instead of 23.9, over 3000
-// 22.5 instead of 25.6; of 2 a tree of 8 tokens, 16 heads, over 2900 keys 28.7 instead of 23, as a row tile has too many pieces to join.
+// Units of the shortest piece that the line is divided into.  Of 2, 4 and 6, us: one token with 128 heads over 500 keys 17.1, 19.5 and 22.9, over 3000 24.3, 23.0 and 24.3; a tree of 8
+// tokens, 16 heads, over 2900 keys 23.4, 22.7 and 23.7; single tokens of 8 sequences over 1000, 16 heads, 25.2, 23.4 and 24.3; longer calls the same.
 constexpr int LA_LEAST = 4;
 
 struct LaParams {

@@ -89,9 +89,10 @@ def latent_attention(query_nope, query_rope, kv_cache, kr_cache, k_scale_cache, 
 
     A token sees the keys up to its own; with ``window`` of these the last ``window``, its own among them, and the first ``sinks`` of the sequence;
     with ``tree_mask`` (total_q, words) int64 the keys before the sequence's query tokens and those of query tokens j whose bit j % 64 of word
-    j / 64 is set.  Rows that see no key are zeros (softmax_lse -inf); rows of no sequence stay as they were.  What a row does not see may hold
-    anything, infinities and what is no number among it, and what lies behind a sequence's last key is never looked at.  Positions without a page
-    read as zeros, as in ``latent_cache_read``.
+    j / 64 is set (of fewer keys than query tokens the first tokens have none).  Rows that see no key are zeros (softmax_lse -inf); rows of no
+    sequence stay as they were.  What a row does not see may hold anything, infinities and what is no number among it, and has no part in its
+    results; the same goes for what lies behind a sequence's last key in its page.  Positions without a page read as zeros, as in
+    ``latent_cache_read``.
     """
     return _attend("latent_attention", query_nope, query_rope, (kv_cache, kr_cache, k_scale_cache), ("kv_cache", "kr_cache", "k_scale_cache"), block_table,
                    cu_seqlens_q, seq_lens, attention_out, softmax_scale, block_size, window, sinks, tree_mask, softmax_lse)
