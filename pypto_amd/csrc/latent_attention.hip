@@ -19,7 +19,7 @@
 //
 // No unit is busy half of the time.  Of a workgroup's time (single tokens of 32 sequences over 2052 keys, 128 heads; counters) vector instructions take 39 %, LDS 30,
 // scalar instructions 25, products 23, and its waves wait for 38 % of theirs.  A tile takes 3000 clocks (1.45 us); the selected keys' attention of 64 heads, with the same
-// products and LDS traffic, 2580, at 42, 40, 10, 30 and 41 %: it has pages in LDS before its loop, where this one makes a look-up, a division and addresses for each tile, 2.3
+// products and LDS traffic, 2580, at 42, 40, 10, 30 and 41 %: it has pages in LDS before its loop, where this one makes a look-up, a division and addresses for each tile, 3.3
 // times as many scalar instructions in all, which is the likely difference.  Beside the tiles a beginning of 9 us (sums over the sequences 2.2, its place in the line 1.1, requests
 // 1.5, their way 0.5, the first tile 3.3) and an end of 1.2, where pieces are short most of the time; and the second launch, which reads what the first wrote.
 // The example 46.5 to 50 us, 17 GFLOP of products, 33 MB of pieces; 1 to 4 tokens of 90 sequences over 1016 keys, 16 heads: 42; a tree of 8 tokens over 2900 keys, 16
